@@ -85,6 +85,7 @@ extern "C" {
 typedef struct aesir_ctx aesir_ctx;
 typedef struct aesir_kv aesir_kv;
 typedef struct aesir_model aesir_model;
+typedef struct aesir_kv4 aesir_kv4;
 
 /* Thread-local message of the last failing call on this thread (empty string if none). */
 const char *aesir_last_error(void);
@@ -95,8 +96,8 @@ int32_t aesir_abi_version(void);
  * Replaces MimirWell.__init__ (core/mimir_well.mojo:533-541), which allocates and zeroes a host
  * pool; here the pool is device memory, zeroed at creation. */
 int32_t aesir_ctx_create(int32_t device, int64_t well_bytes, aesir_ctx **out);
-/* Fails (AESIR_ERR_INVALID, context left intact) while a model created on it is alive: models hold
- * pointers into the context, so destroy them first. */
+/* Fails (AESIR_ERR_INVALID, context left intact) while a model or a paged 4-bit cache created on it is
+ * alive: they hold pointers into the context, so destroy them first. */
 int32_t aesir_ctx_destroy(aesir_ctx *ctx);
 int32_t aesir_ctx_synchronize(aesir_ctx *ctx);
 /* The context's hipStream_t, for callers that interleave their own work. */
@@ -263,6 +264,74 @@ int32_t aesir_kv_append(aesir_ctx *ctx, aesir_kv *kv, int64_t layer_idx, int64_t
 /* KVCache.get_k_slice / get_v_slice (:503-521): device pointer of row 0 of the layer. */
 int32_t aesir_kv_k_slice(const aesir_kv *kv, int64_t layer_idx, int64_t seq_len, void **dev_ptr);
 int32_t aesir_kv_v_slice(const aesir_kv *kv, int64_t layer_idx, int64_t seq_len, void **dev_ptr);
+
+/* ======================================================================= paged 4-bit KV cache
+ * Keys and values of many sequences for every layer of a model, in pages of 4-bit values that sequences
+ * can share. No counterpart in the reference, whose KVCache holds one sequence in f16.
+ *
+ * A row of one KV head is stored in groups of 32 neighbouring dims. With mn and mx the smallest and the
+ * largest f16 value of a group: d = the f16 nearest (mx - mn) / 15 (the next one below where mn + 15 d
+ * would pass 65504), q_i = the integer nearest (x_i - mn) / d, ties to even, at most 15 (0 where d = 0),
+ * and from then on the row is v_i = f16(mn + q_i d), rounded once: 5 bits an element, |v_i - x_i| at most
+ * d / 2 (15 * 2^-25 where that is more) and one f16 rounding. A group that holds an inf or a NaN reads as NaN
+ * throughout.
+ *
+ * Use: begin() makes room for new positions of some sequences and makes them the batch; then, layer by
+ * layer, append() stores the batch's new rows and attention() lets the batch's query rows attend. Rows are
+ * in batch order, each sequence's in position order, row r of a sequence seeing the positions up to its
+ * own. Tensors are f16 rows of `cols` elements from row to row, of which the first heads * head_dim count
+ * (so K, V and Q may be parts of one fused matrix); any 2-byte alignment, 16 bytes with cols a multiple of
+ * 8 being the fast one. Outputs must not overlap inputs.
+ *
+ * append() and attention() may be captured into a HIP graph on the context's stream. A replay there serves
+ * the batch of its time: it stores or attends for the first rows of it, as many as the captured call had,
+ * and does nothing when there is no batch. The other calls send host data to the device and are refused
+ * while the stream is being captured. fork, copy, truncate and compact end the batch. */
+
+/* Bytes of well that aesir_kv4_create takes for these sizes, or a negative error code. */
+int64_t aesir_kv4_well_bytes(int64_t num_layers, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                             int64_t max_seq_len, int64_t max_seqs, int64_t page_size, int64_t num_pages);
+/* A cache of num_pages pages of page_size positions (a power of two, 32 to 1024), for sequences 0 ..
+ * max_seqs - 1 (at most 4096) of up to max_seq_len positions; head_dim 32, 64, 128 or 256, n_heads query
+ * heads a multiple of n_kv_heads. Its memory is taken from the context's well. ctx may be NULL: such a cache keeps the
+ * tables only (begin, fork, copy, truncate, compact and the queries work, for planning without a GPU). */
+int32_t aesir_kv4_create(aesir_ctx *ctx, int64_t num_layers, int64_t n_heads, int64_t n_kv_heads,
+                         int64_t head_dim, int64_t max_seq_len, int64_t max_seqs, int64_t page_size,
+                         int64_t num_pages, aesir_kv4 **out);
+/* Frees the descriptor (waiting for the stream); the pages' memory belongs to the well. */
+int32_t aesir_kv4_destroy(aesir_kv4 *kv);
+/* Bytes of one page (all layers), free pages, and positions of a sequence; -1 for a bad argument. */
+int64_t aesir_kv4_page_bytes(const aesir_kv4 *kv);
+int64_t aesir_kv4_free_pages(const aesir_kv4 *kv);
+int64_t aesir_kv4_length(const aesir_kv4 *kv, int64_t seq);
+/* The pages of a sequence in position order: *n of them, the first cap in pages[]. */
+int32_t aesir_kv4_pages(const aesir_kv4 *kv, int64_t seq, int64_t *pages, int64_t cap, int64_t *n);
+
+/* Adds rows[i] >= 0 positions to sequence seqs[i] (each listed once) and makes the n sequences the batch.
+ * A last page that is shared and would be written to is copied first. The lowest free pages are taken;
+ * without enough of them AESIR_ERR_EXHAUSTED, and nothing has changed. */
+int32_t aesir_kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64_t n);
+/* Stores the batch's new rows of one layer: key and val have as many rows as begin() added. */
+int32_t aesir_kv4_append(aesir_kv4 *kv, int64_t layer, const void *key, int64_t key_rows, int64_t key_cols,
+                         const void *val, int64_t val_rows, int64_t val_cols);
+/* Attention of the batch's new rows over their sequences, scale 1 / sqrt(head_dim), f32 softmax and sums:
+ * query and output have as many rows as begin() added. The positions must have been appended. */
+int32_t aesir_kv4_attention(aesir_kv4 *kv, int64_t layer, const void *query, int64_t query_rows,
+                            int64_t query_cols, void *output, int64_t output_rows, int64_t output_cols);
+/* The f16 values that positions pos[i] .. pos[i] + rows[i] - 1 of sequences seqs[i] stand for, of layers
+ * layer .. layer + layers - 1: row (l * sum(rows) + r) of key and val is the r-th of the ranges' rows. */
+int32_t aesir_kv4_read(aesir_kv4 *kv, int64_t layer, int64_t layers, const int64_t *seqs, const int64_t *pos,
+                       const int64_t *rows, int64_t n, void *key, int64_t key_rows, int64_t key_cols, void *val,
+                       int64_t val_rows, int64_t val_cols);
+/* dst, an empty sequence, becomes src's continuation on the same pages (none is copied until written to). */
+int32_t aesir_kv4_fork(aesir_kv4 *kv, int64_t src, int64_t dst);
+/* dst, an empty sequence, becomes a copy of src on pages of its own. */
+int32_t aesir_kv4_copy(aesir_kv4 *kv, int64_t src, int64_t dst);
+/* Cuts a sequence to its first `length` positions and frees the pages that no sequence holds any more;
+ * length 0 frees the sequence. */
+int32_t aesir_kv4_truncate(aesir_kv4 *kv, int64_t seq, int64_t length);
+/* Moves pages so that the used ones are pages 0 .. *used_pages - 1 (used_pages may be NULL). */
+int32_t aesir_kv4_compact(aesir_kv4 *kv, int64_t *used_pages);
 
 /* ======================================================================= model + engine */
 typedef struct {

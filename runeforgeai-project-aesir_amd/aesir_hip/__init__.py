@@ -88,6 +88,21 @@ _sig("aesir_kv_destroy", [P])
 _sig("aesir_kv_append", [P, P, I64, I64, P, I64, P, I64])
 _sig("aesir_kv_k_slice", [P, I64, I64, C.POINTER(P)])
 _sig("aesir_kv_v_slice", [P, I64, I64, C.POINTER(P)])
+_sig("aesir_kv4_well_bytes", [I64] * 8, I64)
+_sig("aesir_kv4_create", [P] + [I64] * 8 + [C.POINTER(P)])
+_sig("aesir_kv4_destroy", [P])
+_sig("aesir_kv4_page_bytes", [P], I64)
+_sig("aesir_kv4_free_pages", [P], I64)
+_sig("aesir_kv4_length", [P, I64], I64)
+_sig("aesir_kv4_pages", [P, I64, P, I64, C.POINTER(I64)])
+_sig("aesir_kv4_begin", [P, P, P, I64])
+_sig("aesir_kv4_append", [P, I64, P, I64, I64, P, I64, I64])
+_sig("aesir_kv4_attention", [P, I64, P, I64, I64, P, I64, I64])
+_sig("aesir_kv4_read", [P, I64, I64, P, P, P, I64, P, I64, I64, P, I64, I64])
+_sig("aesir_kv4_fork", [P, I64, I64])
+_sig("aesir_kv4_copy", [P, I64, I64])
+_sig("aesir_kv4_truncate", [P, I64, I64])
+_sig("aesir_kv4_compact", [P, C.POINTER(I64)])
 _sig("aesir_model_create", [P, C.POINTER(_ModelConfig), C.POINTER(P)])
 _sig("aesir_model_create_typed", [P, C.POINTER(_ModelConfig), I32, C.POINTER(P)])
 _sig("aesir_model_create_mixed", [P, C.POINTER(_ModelConfig), P, I64, C.POINTER(P)])
@@ -191,10 +206,11 @@ class Context:
         _check(_L.aesir_ctx_create(device, int(well_bytes), C.byref(h)))
         self.h = h.value
         self._models = weakref.WeakSet()  # models hold pointers into the context: closed first
+        self._caches = weakref.WeakSet()  # and so do paged 4-bit caches
 
     def close(self):
         if self.h:
-            for m in list(self._models):
+            for m in list(self._models) + list(self._caches):
                 m.close()
             _check(_L.aesir_ctx_destroy(self.h))
             self.h = None
@@ -378,6 +394,103 @@ class KVCache:
         p = P()
         _check(_L.aesir_kv_v_slice(self.h, layer_idx, seq_len, C.byref(p)))
         return Tensor(self.ctx, p.value, seq_len, self.hidden_dim)
+
+
+def _i64s(values) -> "C.Array":
+    return (I64 * len(values))(*values)
+
+
+class KV4Cache:
+    """Keys and values of many sequences in pages of 4-bit values (aesir_kv4_*): begin() makes room for new
+    positions, then append() and attention() per layer; fork, copy, truncate and compact work on whole
+    sequences. ctx None keeps the page tables only, for planning without a GPU."""
+
+    def __init__(self, ctx, num_layers: int, n_heads: int, n_kv_heads: int, head_dim: int, max_seq_len: int, max_seqs: int,
+                 page_size: int, num_pages: int):
+        self.h = None
+        h = P()
+        _check(_L.aesir_kv4_create(ctx.h if ctx is not None else None, num_layers, n_heads, n_kv_heads, head_dim, max_seq_len,
+                                   max_seqs, page_size, num_pages, C.byref(h)))
+        self.ctx, self.h = ctx, h.value
+        self.num_layers, self.n_heads, self.n_kv_heads, self.head_dim = num_layers, n_heads, n_kv_heads, head_dim
+        self.max_seq_len, self.max_seqs, self.page_size, self.num_pages = max_seq_len, max_seqs, page_size, num_pages
+        if ctx is not None:
+            ctx._caches.add(self)
+
+    @staticmethod
+    def well_bytes(num_layers: int, n_heads: int, n_kv_heads: int, head_dim: int, max_seq_len: int, max_seqs: int,
+                   page_size: int, num_pages: int) -> int:
+        """Bytes of well that a cache of these sizes takes."""
+        n = _L.aesir_kv4_well_bytes(num_layers, n_heads, n_kv_heads, head_dim, max_seq_len, max_seqs, page_size, num_pages)
+        if n < 0:
+            raise AesirError(int(n), _L.aesir_last_error().decode())
+        return n
+
+    def close(self):
+        if self.h:
+            _check(_L.aesir_kv4_destroy(self.h))
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    @property
+    def page_bytes(self) -> int:
+        return _L.aesir_kv4_page_bytes(self.h)
+
+    @property
+    def free_pages(self) -> int:
+        return _L.aesir_kv4_free_pages(self.h)
+
+    def length(self, seq: int) -> int:
+        return _L.aesir_kv4_length(self.h, seq)
+
+    def pages(self, seq: int) -> list:
+        """The page ids of a sequence in position order."""
+        n = I64()
+        _check(_L.aesir_kv4_pages(self.h, seq, None, 0, C.byref(n)))
+        out = (I64 * max(1, n.value))()
+        _check(_L.aesir_kv4_pages(self.h, seq, out, n.value, C.byref(n)))
+        return list(out[: n.value])
+
+    def begin(self, seqs, rows):
+        """Adds rows[i] positions to sequence seqs[i] and makes these sequences the batch."""
+        if len(seqs) != len(rows):
+            raise ValueError("begin: as many row counts as sequences")
+        _check(_L.aesir_kv4_begin(self.h, _i64s(seqs), _i64s(rows), len(seqs)))
+
+    def append(self, layer: int, key: Tensor, val: Tensor):
+        """Stores the batch's new rows of one layer."""
+        _check(_L.aesir_kv4_append(self.h, layer, key.ptr, key.rows, key.cols, val.ptr, val.rows, val.cols))
+
+    def attention(self, layer: int, query: Tensor, output: Tensor):
+        """Attention of the batch's new rows over their sequences."""
+        _check(_L.aesir_kv4_attention(self.h, layer, query.ptr, query.rows, query.cols, output.ptr, output.rows, output.cols))
+
+    def read(self, layer: int, layers: int, seqs, pos, rows, key: Tensor, val: Tensor):
+        """The f16 values of position ranges, [layers][sum(rows)] rows."""
+        if not len(seqs) == len(pos) == len(rows):
+            raise ValueError("read: as many positions and row counts as sequences")
+        _check(_L.aesir_kv4_read(self.h, layer, layers, _i64s(seqs), _i64s(pos), _i64s(rows), len(seqs), key.ptr, key.rows,
+                                 key.cols, val.ptr, val.rows, val.cols))
+
+    def fork(self, src: int, dst: int):
+        _check(_L.aesir_kv4_fork(self.h, src, dst))
+
+    def copy(self, src: int, dst: int):
+        _check(_L.aesir_kv4_copy(self.h, src, dst))
+
+    def truncate(self, seq: int, length: int):
+        _check(_L.aesir_kv4_truncate(self.h, seq, length))
+
+    def compact(self) -> int:
+        """Moves the used pages to the lowest indices; their count."""
+        n = I64()
+        _check(_L.aesir_kv4_compact(self.h, C.byref(n)))
+        return n.value
 
 
 # ------------------------------------------------------------------ model / engine

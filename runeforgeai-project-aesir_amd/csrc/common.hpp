@@ -160,6 +160,7 @@ struct aesir_ctx {
     hipEvent_t ev_start = nullptr, ev_stop = nullptr;
     bool timer_running = false;
     int64_t live_models = 0;  // models created on this context and not yet destroyed
+    int64_t live_caches = 0;  // the same for paged 4-bit caches
     aesir::CtxScratch scratch;
     std::vector<aesir::RopeTable> rope_tables;
     int64_t *pinned_i64 = nullptr;  // small pinned staging area (64 entries)

@@ -161,6 +161,9 @@ int32_t aesir_ctx_destroy(aesir_ctx *ctx) {
     if (ctx->live_models > 0)  // a model keeps pointers into this context
         return fail(AESIR_ERR_INVALID, "aesir_ctx_destroy: %lld model(s) still alive; destroy them first",
                     (long long)ctx->live_models);
+    if (ctx->live_caches > 0)  // so does a paged 4-bit cache
+        return fail(AESIR_ERR_INVALID, "aesir_ctx_destroy: %lld KV4Cache(s) still alive; destroy them first",
+                    (long long)ctx->live_caches);
     (void)hipSetDevice(ctx->device);
     if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
     for (auto &t : ctx->rope_tables) (void)hipFree(t.dev);
