@@ -257,77 +257,416 @@ __global__ __launch_bounds__(kThreads) void kv4_copy_kernel(char *pool, int64_t 
 
 // ------------------------------------------------------------------ attention
 //
-// o = softmax(q k^T / sqrt(hd)) v of one row and query head over the positions up to the row's own. One wave per
-// (row, query head): 64 positions a step, a lane scores one of them, then owns dims lane, lane + 64, ..
+// o = softmax(q k^T / sqrt(hd)) v of the batch's new rows over the positions up to their own, on the matrix
+// cores. A column is one (row, query head of the KV head's group) pair; a unit of work is a tile of 16 NC columns
+// of one sequence and KV head and a split of its rounds of 32 keys. Four waves take the unit's rounds in turn, each
+// for all columns (a key is unpacked by one wave, once a unit), and meet in LDS at the end.
+//
+//   scores   S^T = K q^T: a 16-key tile's A operand is unpacked nibbles; lane (i, g) holds key 8 (i / 4) + 4 t + i % 4
+//            of the round (t = 0, 1) and the hd / 4 dims from g hd / 4, so one load brings its part of the row
+//            and one scale serves it. With that key order a lane's results are the scores of keys 8 g .. 8 g + 7
+//   softmax  f32, a running maximum and sum per column (over the lanes i, i + 16, ..: two permlane swaps); the
+//            accumulator is rescaled only in rounds that raise a maximum
+//   P V      O^T += V^T P^T: a lane's eight probabilities are the B operand as they are (its keys are consecutive), the A
+//            operand is eight positions of one dim: the V tiles' layout. A lane unpacks the dims of one 8-dim block
+//
+// Unpacking gives the exact f16 values that the cache stands for (one packed multiply-add per pair). Probabilities
+// are held as f16 times 2^15: 11 bits each against f32 sums, and only those under 2^-39 of the largest can vanish.
+// Positions behind the last visible key are zeroed (their scales), since P = 0 times a NaN there would spread; a
+// visible NaN value group (the only non-finite values there are) reaches just the columns that see it.
 struct Kv4AttnArgs {
     const h16 *q;
     h16 *out;
     int64_t q_stride, out_stride;
     int64_t layer;
     int32_t rows;  // rows of q and out
-    float scale;
+    int32_t vec;   // q and out rows 16-byte aligned
+    float scale;   // log2(e) / sqrt(hd)
 };
 
-__global__ __launch_bounds__(kWave) void kv4_attention_kernel(Kv4Dev c, Kv4AttnArgs a) {
-    __shared__ int row0[kMaxSeqs];
-    __shared__ float qs[256], ps[kWave];
-    const int n = c.head->n, total = min(c.head->total_rows, a.rows), lane = threadIdx.x;
-    for (int i = lane; i < n; i += kWave) row0[i] = c.row0[i];
-    __syncthreads();
-    const int groups = c.hd / kKv4Group;
-    for (int64_t u = blockIdx.x; u < (int64_t)total * c.nq; u += gridDim.x) {
-        const int row = (int)(u / c.nq), head = (int)(u % c.nq), kvh = head / (c.nq / c.nkv);
-        const Kv4Seq s = c.seqs[last_not_above(row0, n, row)];
-        const int seen = s.length - s.rows + (row - s.row0) + 1;
-        __syncthreads();
-        for (int d = lane; d < c.hd; d += kWave) qs[d] = (float)a.q[(int64_t)row * a.q_stride + head * c.hd + d];
-        float m = -INFINITY, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int p0 = 0; p0 < seen; p0 += kWave) {
-            __syncthreads();
-            const int pos = p0 + lane, here = min(seen - p0, kWave);
-            float sc = -INFINITY;
-            if (lane < here) {
-                const int slot = pos & (c.page_size() - 1);
-                const char *b = c.block(c.table[(int64_t)s.slot * c.table_stride + (pos >> c.page_shift)], a.layer, kvh);
-                float dot = 0.0f;
-                for (int g = 0; g < groups; g++) {
-                    const h16x2 ks = reinterpret_cast<const h16x2 *>(b + c.k_scale_off())[slot * groups + g];
-                    for (int j = 0; j < 4; j++) {
-                        const u32x4 v = kv4_decode(reinterpret_cast<const unsigned *>(b)[slot * (c.hd / 8) + 4 * g + j], ks.x, ks.y);
-                        for (int e = 0; e < 4; e++) {
-                            dot = fmaf((float)as_h2(v[e]).x, qs[32 * g + 8 * j + 2 * e], dot);
-                            dot = fmaf((float)as_h2(v[e]).y, qs[32 * g + 8 * j + 2 * e + 1], dot);
-                        }
-                    }
-                }
-                sc = dot * a.scale;
-            }
-            const float mn = fmaxf(m, wave_max(sc)), ref = mn == -INFINITY ? 0.0f : mn;
-            const float p = expf(sc - ref), al = expf(m - ref);
-            l = l * al + wave_sum(p);
-            m = mn;
-            ps[lane] = p;
-            __syncthreads();
-            for (int i = 0; i < 4; i++) {
-                const int d = lane + kWave * i;
-                if (d >= c.hd) break;
-                acc[i] *= al;
-                for (int r = 0; r < here; r++) {
-                    const int q = p0 + r, slot = q & (c.page_size() - 1);
-                    const char *b = c.block(c.table[(int64_t)s.slot * c.table_stride + (q >> c.page_shift)], a.layer, kvh);
-                    const unsigned w = reinterpret_cast<const unsigned *>(b + c.v_off())[(slot / 4 * (c.hd / 8) + d / 8) * 4 + slot % 4];
-                    const h16 vd = reinterpret_cast<const h16 *>(b + c.v_d_off())[d / 32 * c.page_size() + slot];
-                    const h16 vm = reinterpret_cast<const h16 *>(b + c.v_m_off())[d / 32 * c.page_size() + slot];
-                    const h16x2 v = kv4_pair(w, d % 8 / 2, both(vd), both(vm));
-                    acc[i] = fmaf(ps[r], (float)(d % 2 ? v.y : v.x), acc[i]);
+constexpr int kAWaves = 4;
+constexpr int kKeys = 32;  // keys per round
+
+// The four values (two neighbouring nibbles each half) of x at nibble p under scales d and offsets m per half.
+template <int P>
+__device__ __forceinline__ h16x2 kv4_values(unsigned x, h16x2 d, h16x2 m) {
+    h16x2 n;
+    if constexpr (P % 2 == 0) {
+        n = as_h2(((x >> (4 * P)) & 0x000F000Fu) | 0x64006400u) - both((h16)1024.0f);
+    } else {  // 1024 + 16 n: no shift, the multiply-add undoes both exactly
+        n = __builtin_elementwise_fma(as_h2(((x >> (4 * (P - 1))) & 0x00F000F0u) | 0x64006400u), both((h16)0.0625f), both((h16)-64.0f));
+    }
+    return __builtin_elementwise_fma(n, d, m);
+}
+
+template <int HD>
+struct Kv4Round {  // one lane's share of 32 keys
+    static constexpr int NJ = HD / 32, NG = NJ == 8 ? 2 : 1, NB = NJ == 8 ? 2 : 1;
+    unsigned k[2][NJ];
+    h16x2 ks[2][NG];
+    u32x4 v[NB][2], vd[NB], vm[NB];
+
+    __device__ __forceinline__ void load(const Kv4Dev &c, const char *b, int s0, int i, int g) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int key = s0 + 8 * (i / 4) + 4 * t + i % 4;
+            const char *p = b + key * (HD / 2) + g * (HD / 8);
+            if constexpr (NJ == 1) {
+                k[t][0] = *reinterpret_cast<const unsigned *>(p);
+            } else if constexpr (NJ == 2) {
+                const u32x2 x = *reinterpret_cast<const u32x2 *>(p);
+                k[t][0] = x.x;
+                k[t][1] = x.y;
+            } else {
+#pragma unroll
+                for (int j = 0; j < NJ; j += 4) {
+                    const u32x4 x = ld16(p + 4 * j);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) k[t][j + e] = x[e];
                 }
             }
+            const h16x2 *ps = reinterpret_cast<const h16x2 *>(b + c.k_scale_off()) + key * NJ + g * NJ / 4;
+#pragma unroll
+            for (int x = 0; x < NG; x++) ks[t][x] = ps[x];
         }
-        for (int i = 0; i < 4; i++) {
-            const int d = lane + kWave * i;
-            if (d < c.hd) a.out[(int64_t)row * a.out_stride + head * c.hd + d] = (h16)(acc[i] / l);
+#pragma unroll
+        for (int x = 0; x < NB; x++) {
+            const int block = NJ < 4 ? i % (4 * NJ) : i + 16 * x;
+#pragma unroll
+            for (int h = 0; h < 2; h++) v[x][h] = ld16(b + c.v_off() + ((s0 / 4 + 2 * g + h) * (HD / 8) + block) * 16);
+            vd[x] = ld16(b + c.v_d_off() + (block / 4 * c.page_size() + s0 + 8 * g) * 2);
+            vm[x] = ld16(b + c.v_m_off() + (block / 4 * c.page_size() + s0 + 8 * g) * 2);
         }
     }
+};
+
+// Index of the batch's last sequence whose first unit is <= unit; the whole wave calls it.
+template <int V>
+__device__ __forceinline__ int find_unit(const Kv4Seq *seqs, int n, int unit, int lane) {
+    int at = 0;
+    for (int base = 0; base < n; base += kWave) {
+        const bool below = base + lane < n && seqs[base + lane].item0[V] <= unit;
+        const int count = __popcll(__ballot(below));
+        if (count) at = base + count - 1;
+        if (count < kWave) break;
+    }
+    return __builtin_amdgcn_readfirstlane(at);
+}
+
+// The dim of accumulator (x, p, half) in matrix row r.
+template <int HD>
+__device__ __forceinline__ int out_dim(int r, int x, int p, int half) {
+    constexpr int NJ = HD / 32;
+    if constexpr (NJ < 4) return 8 * (r % (4 * NJ)) + 2 * (NJ * (r / (4 * NJ)) + p) + half;
+    return 8 * (r + 16 * x) + 2 * p + half;
+}
+
+template <int HD, int NC>
+__global__ __launch_bounds__(kAWaves *kWave) void kv4_attention_kernel(Kv4Dev c, Kv4AttnArgs a) {
+    constexpr int V = NC == 1 ? 0 : NC == 2 ? 1 : 2, W = 16 * NC;
+    constexpr int NJ = HD / 32, NP = NJ < 4 ? NJ : 4, NB = Kv4Round<HD>::NB, NG = Kv4Round<HD>::NG;
+    constexpr int LD = HD + 4;  // LDS row of a column
+    __shared__ float ml[kAWaves][W][2];
+    __shared__ __align__(16) float ox[kAWaves][16][LD];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const int G = c.nq / c.nkv, n = c.head->n, items = c.head->items[V];
+    for (int64_t u = blockIdx.x; u < (int64_t)items * c.nkv; u += gridDim.x) {
+        const int kvh = (int)(u % c.nkv), unit = (int)(u / c.nkv);
+        const Kv4Seq &s = c.seqs[find_unit<V>(c.seqs, n, unit, lane)];
+        const int local = unit - s.item0[V], splits = s.splits[V], cols = s.rows * G, tiles = (cols + W - 1) / W;
+        const int tile = tiles - 1 - local / splits, split = local % splits;
+        const int before = s.length - s.rows;
+        const int low = before + tile * W / G;                                    // last position of the first column
+        const int keys = before + min(s.rows - 1, (tile * W + W - 1) / G) + 1;     // positions the tile sees
+        const int rounds = (keys + kKeys - 1) / kKeys, per = (rounds + splits - 1) / splits;
+        const int r1 = min(rounds, (split + 1) * per);
+
+        // queries: column i of each 16, dims g HD / 4 + 8 j ..
+        u32x4 q[NC][NJ];
+        int limit[NC];
+#pragma unroll
+        for (int t = 0; t < NC; t++) {
+            const int col = tile * W + 16 * t + i, row = col / G;
+            const bool live = col < cols && s.row0 + row < a.rows;
+            limit[t] = live ? before + row : -1;
+            const h16 *p = a.q + (int64_t)(s.row0 + row) * a.q_stride + (kvh * G + col % G) * HD + g * (HD / 4);
+#pragma unroll
+            for (int j = 0; j < NJ; j++) q[t][j] = !live ? u32x4{0, 0, 0, 0} : a.vec ? ld16(p + 8 * j) : load8<false>(p + 8 * j);
+        }
+        f32x4 acc[NC][NB][NP][2];
+        float m[NC], l[NC];
+#pragma unroll
+        for (int t = 0; t < NC; t++) {
+            m[t] = -INFINITY;
+            l[t] = 0.0f;
+#pragma unroll
+            for (int x = 0; x < NB; x++)
+#pragma unroll
+                for (int p = 0; p < NP; p++) acc[t][x][p][0] = acc[t][x][p][1] = f32x4{0, 0, 0, 0};
+        }
+
+        const int32_t *table = c.table + (int64_t)s.slot * c.table_stride;
+        auto fetch = [&](int r, Kv4Round<HD> &d) {
+            const int pos = r * kKeys;
+            d.load(c, c.block(__builtin_amdgcn_readfirstlane(table[pos >> c.page_shift]), a.layer, kvh), pos & (c.page_size() - 1), i, g);
+        };
+        auto round = [&](int r, Kv4Round<HD> &d) {
+            f32x4 sc[2][NC];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+#pragma unroll
+                for (int x = 0; x < NC; x++) sc[t][x] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < NJ; j++) {
+                    const h16x2 dd = both(d.ks[t][j * NG / NJ].x), mm = both(d.ks[t][j * NG / NJ].y);
+                    const unsigned w = d.k[t][j];
+                    const u32x4 ka = {h2_bits(kv4_values<0>(w, dd, mm)), h2_bits(kv4_values<1>(w, dd, mm)),
+                                      h2_bits(kv4_values<2>(w, dd, mm)), h2_bits(kv4_values<3>(w, dd, mm))};
+#pragma unroll
+                    for (int x = 0; x < NC; x++) sc[t][x] = mfma16x16x32(ka, q[x][j], sc[t][x]);
+                }
+            }
+            const bool whole = r * kKeys + kKeys - 1 <= low;  // every column sees every key
+            const int k0 = r * kKeys + 8 * g;
+            unsigned bad[NB] = {};  // bit e: value group of key k0 + e is NaN (rounds that are not whole)
+            if (!whole) {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int x = 0; x < NC; x++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (k0 + 4 * t + e > limit[x]) sc[t][x][e] = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < NB; x++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const unsigned half = 0xFFFFu << (16 * (e % 2));
+                        const bool nan = ((d.vm[x][e / 2] >> (16 * (e % 2))) & 0x7FFFu) > 0x7C00u, hidden = k0 + e >= keys;
+                        if (nan || hidden) {
+                            d.vd[x][e / 2] &= ~half;
+                            d.vm[x][e / 2] &= ~half;
+                        }
+                        if (nan && !hidden) bad[x] |= 1u << e;
+                    }
+            }
+            u32x4 pb[NC];
+#pragma unroll
+            for (int x = 0; x < NC; x++) {
+                float mx = fmaxf(fmaxf(fmaxf(sc[0][x][0], sc[0][x][1]), fmaxf(sc[0][x][2], sc[0][x][3])),
+                                 fmaxf(fmaxf(sc[1][x][0], sc[1][x][1]), fmaxf(sc[1][x][2], sc[1][x][3])));
+                mx = swap_pair_max<32>(swap_pair_max<16>(mx));
+                if (__any(mx > m[x])) {
+                    const float up = fmaxf(m[x], mx), ref = up == -INFINITY ? 0.0f : up;
+                    const float al = __builtin_amdgcn_exp2f((m[x] - ref) * a.scale);
+                    l[x] *= al;
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+#pragma unroll
+                        for (int p = 0; p < NP; p++) {
+                            acc[x][b][p][0] *= al;
+                            acc[x][b][p][1] *= al;
+                        }
+                    m[x] = up;
+                }
+                const float ref = m[x] == -INFINITY ? 0.0f : m[x];
+                float pr[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    pr[e] = __builtin_amdgcn_exp2f((sc[e / 4][x][e % 4] - ref) * a.scale + 15.0f);
+                    l[x] += pr[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) pb[x][e] = h2_bits(h16x2{(h16)pr[2 * e], (h16)pr[2 * e + 1]});
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const int shift = NJ < 4 ? 4 * NJ * (i / (4 * NJ)) : 0;
+                unsigned lo[4], hi[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {  // positions 2 e, 2 e + 1: low halves (even dims) and high halves
+                    const unsigned w0 = d.v[b][e / 2][2 * (e % 2)] >> shift, w1 = d.v[b][e / 2][2 * (e % 2) + 1] >> shift;
+                    lo[e] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+                    hi[e] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+                }
+                auto step = [&](auto pc) {
+                    constexpr int P = decltype(pc)::value;
+                    if constexpr (P < NP) {
+                        u32x4 va, vb;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            va[e] = h2_bits(kv4_values<P>(lo[e], as_h2(d.vd[b][e]), as_h2(d.vm[b][e])));
+                            vb[e] = h2_bits(kv4_values<P>(hi[e], as_h2(d.vd[b][e]), as_h2(d.vm[b][e])));
+                        }
+#pragma unroll
+                        for (int x = 0; x < NC; x++) {
+                            acc[x][b][P][0] = mfma16x16x32(va, pb[x], acc[x][b][P][0]);
+                            acc[x][b][P][1] = mfma16x16x32(vb, pb[x], acc[x][b][P][1]);
+                        }
+                    }
+                };
+                step(std::integral_constant<int, 0>{});
+                step(std::integral_constant<int, 1>{});
+                step(std::integral_constant<int, 2>{});
+                step(std::integral_constant<int, 3>{});
+                if (!whole && __any(bad[b] != 0)) {  // NaN for the columns that see a NaN group, in its dims
+                    u32x4 ia;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) ia[e] = (bad[b] >> (2 * e) & 1 ? 0x3C00u : 0u) | (bad[b] >> (2 * e + 1) & 1 ? 0x3C000000u : 0u);
+#pragma unroll
+                    for (int x = 0; x < NC; x++) {
+                        u32x4 ib;
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            ib[e] = (k0 + 2 * e <= limit[x] ? 0x3C00u : 0u) | (k0 + 2 * e + 1 <= limit[x] ? 0x3C000000u : 0u);
+                        const f32x4 seen = mfma16x16x32(ia, ib, f32x4{0, 0, 0, 0});
+#pragma unroll
+                        for (int p = 0; p < NP; p++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (seen[e] > 0.0f) acc[x][b][p][0][e] = acc[x][b][p][1][e] = NAN;
+                    }
+                }
+            }
+        };
+        int r = split * per + wave;
+        if (r < r1) {  // the next round's loads are issued before a round is computed
+            Kv4Round<HD> cur, next;
+            fetch(r, cur);
+            for (; r + kAWaves < r1; r += kAWaves) {
+                fetch(r + kAWaves, next);
+                round(r, cur);
+                cur = next;
+            }
+            round(r, cur);
+        }
+
+        // the waves meet: maxima and sums of all columns, then 16 columns of accumulators at a time
+#pragma unroll
+        for (int t = 0; t < NC; t++) {
+            l[t] = swap_pair_sum<16>(l[t], l[t]);
+            l[t] = swap_pair_sum<32>(l[t], l[t]);
+            if (g == 0) {
+                ml[wave][16 * t + i][0] = m[t];
+                ml[wave][16 * t + i][1] = l[t];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NC; t++) {
+            float up = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kAWaves; w++) up = fmaxf(up, ml[w][16 * t + i][0]);
+            const float ref = up == -INFINITY ? 0.0f : up, mine = __builtin_amdgcn_exp2f((m[t] - ref) * a.scale);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int x = 0; x < NB; x++)
+#pragma unroll
+                    for (int p = 0; p < NP; p++) {
+                        float *o = &ox[wave][i][out_dim<HD>(4 * g + e, x, p, 0)];
+                        o[0] = acc[t][x][p][0][e] * mine;
+                        o[1] = acc[t][x][p][1][e] * mine;
+                    }
+            __syncthreads();
+            // thread: HD / 16 dims of one column
+            constexpr int D = HD / 16;
+            const int col = threadIdx.x / 16, dim = threadIdx.x % 16 * D, gc = tile * W + 16 * t + col, row = gc / G;
+            if (gc < cols && s.row0 + row < a.rows) {
+                float M = -INFINITY, L = 0.0f, o[D];
+#pragma unroll
+                for (int w = 0; w < kAWaves; w++) M = fmaxf(M, ml[w][16 * t + col][0]);
+                const float mref = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+                for (int w = 0; w < kAWaves; w++) L += ml[w][16 * t + col][1] * __builtin_amdgcn_exp2f((ml[w][16 * t + col][0] - mref) * a.scale);
+#pragma unroll
+                for (int d = 0; d < D; d++) o[d] = (ox[0][col][dim + d] + ox[1][col][dim + d]) + (ox[2][col][dim + d] + ox[3][col][dim + d]);
+                if (splits == 1) {
+                    h16 *p = a.out + (int64_t)(s.row0 + row) * a.out_stride + (kvh * G + gc % G) * HD + dim;
+                    h16 r16[D];
+#pragma unroll
+                    for (int d = 0; d < D; d++) r16[d] = (h16)(o[d] / L);
+                    if (a.vec) {
+                        __builtin_memcpy(__builtin_assume_aligned(p, 2 * D < 16 ? 2 * D : 16), r16, sizeof r16);
+                    } else {
+                        for (int d = 0; d < D; d++) p[d] = r16[d];
+                    }
+                } else {
+                    const int64_t at = ((int64_t)(s.part0[V] + local) * c.nkv + kvh) * W + 16 * t + col;
+                    if (threadIdx.x % 16 == 0) *reinterpret_cast<float2 *>(c.part_ml + 2 * at) = float2{M, L};
+                    __builtin_memcpy(__builtin_assume_aligned(c.part + at * HD + dim, 4 * D < 16 ? 4 * D : 16), o, sizeof o);
+                }
+            }
+            __syncthreads();  // ox (and, before the next unit, ml) is rewritten
+        }
+    }
+}
+
+// The splits of a column joined: o = sum_s 2^(scale (m_s - M)) acc_s / sum_s 2^(scale (m_s - M)) l_s. One workgroup
+// per (row, query head); its waves take the splits in turn.
+template <int HD>
+__global__ __launch_bounds__(kAWaves *kWave) void kv4_merge_kernel(Kv4Dev c, Kv4AttnArgs a, int v) {
+    constexpr int D = HD >= kWave ? HD / kWave : 1;  // dims per lane
+    __shared__ float ox[kAWaves][HD], lx[kAWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int G = c.nq / c.nkv, n = c.head->n, total = min(c.head->total_rows, a.rows), W = 16 << v;
+    for (int64_t u = blockIdx.x; u < (int64_t)total * c.nq; u += gridDim.x) {
+        const int row = (int)(u / c.nq), head = (int)(u % c.nq);
+        int at = 0;
+        for (int base = 0; base < n; base += kWave) {
+            const int count = __popcll(__ballot(base + lane < n && c.row0[base + lane] <= row));
+            if (count) at = base + count - 1;
+            if (count < kWave) break;
+        }
+        const Kv4Seq &s = c.seqs[__builtin_amdgcn_readfirstlane(at)];
+        const int splits = s.splits[v];
+        if (splits == 1) continue;  // uniform over the workgroup
+        const int col = (row - s.row0) * G + head % G, tiles = (s.rows * G + W - 1) / W;
+        // partial of split x: ((part0 + (tiles - 1 - col / W) splits + x) nkv + KV head) W + col % W
+        const int64_t first = ((int64_t)(s.part0[v] + (tiles - 1 - col / W) * splits) * c.nkv + head / G) * W + col % W;
+        const int64_t step = (int64_t)c.nkv * W;
+        float M = -INFINITY;
+        for (int x = lane; x < splits; x += kWave) M = fmaxf(M, c.part_ml[2 * (first + x * step)]);
+        M = wave_max(M);
+        const float ref = M == -INFINITY ? 0.0f : M;
+        float o[D] = {}, L = 0.0f;
+        for (int x = wave; x < splits; x += kAWaves) {
+            const float2 e = *reinterpret_cast<const float2 *>(c.part_ml + 2 * (first + x * step));
+            const float w = __builtin_amdgcn_exp2f((e.x - ref) * a.scale);
+            L += w * e.y;
+            const float *p = c.part + (first + x * step) * HD + lane * D;
+            if (HD >= kWave || lane < HD) {
+#pragma unroll
+                for (int d = 0; d < D; d++) o[d] += w * p[d];
+            }
+        }
+        if (HD >= kWave || lane < HD) {
+#pragma unroll
+            for (int d = 0; d < D; d++) ox[wave][lane * D + d] = o[d];
+        }
+        if (lane == 0) lx[wave] = L;
+        __syncthreads();
+        for (int d = threadIdx.x; d < HD; d += kAWaves * kWave)
+            a.out[(int64_t)row * a.out_stride + head * HD + d] =
+                (h16)(((ox[0][d] + ox[1][d]) + (ox[2][d] + ox[3][d])) / ((lx[0] + lx[1]) + (lx[2] + lx[3])));
+        __syncthreads();
+    }
+}
+
+template <int HD>
+int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, int v, int64_t items, bool merge, int64_t rows) {
+    const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>(items * c.nkv, 1), 1 << 20)), block(kAWaves * kWave);
+    if (v == 0)
+        hipLaunchKernelGGL((kv4_attention_kernel<HD, 1>), grid, block, 0, st, c, a);
+    else if (v == 1)
+        hipLaunchKernelGGL((kv4_attention_kernel<HD, 2>), grid, block, 0, st, c, a);
+    else if constexpr (HD < 256)
+        hipLaunchKernelGGL((kv4_attention_kernel<HD, 4>), grid, block, 0, st, c, a);
+    AESIR_LAUNCH_CHECK("kv4_attention_kernel");
+    if (!merge) return AESIR_OK;
+    hipLaunchKernelGGL(kv4_merge_kernel<HD>, dim3((unsigned)std::min<int64_t>(rows * c.nq, 1 << 20)), block, 0, st, c, a, v);
+    AESIR_LAUNCH_CHECK("kv4_merge_kernel");
+    return AESIR_OK;
 }
 
 }  // namespace aesir
@@ -350,7 +689,9 @@ struct aesir_kv4 {
     char *ring = nullptr;  // pinned staging, handed out front to back
     int64_t ring_at = 0;
     bool batch = false;
-    int64_t batch_rows = 0;
+    int64_t batch_rows = 0, batch_cols = 0;     // new rows; most columns of one sequence
+    Kv4Head plan{};                             // the batch's descriptor
+    bool plan_splits[kKv4Widths] = {};          // whether any sequence is split, per width
 
     aesir_kv4(int64_t num_pages, int64_t page_size, int64_t max_seqs) : book(num_pages, page_size, max_seqs) {}
 };
@@ -359,12 +700,15 @@ namespace {
 
 constexpr int64_t kRingBytes = 1 << 20;
 constexpr int64_t kMaxPages = (int64_t)1 << 30;
+constexpr int64_t kPartCols = 32768;  // columns of split partials
+constexpr int64_t kUnits = 1024;      // workgroups that attention is split for: four on each of 256 CUs
+constexpr int64_t kMinRounds = 8;     // rounds of 32 keys that a split has at least
 
 struct Kv4Sizes {
-    int64_t page_bytes, pool, table, seqs, row0, ranges, moves, part;
+    int64_t page_bytes, pool, table, seqs, row0, ranges, moves, part, part_ml;
     int64_t total() const {
         int64_t t = 0;
-        for (int64_t b : {pool, table, (int64_t)sizeof(Kv4Head), seqs, row0, ranges, moves, part}) t += (b + 255) / 256 * 256;
+        for (int64_t b : {pool, table, (int64_t)sizeof(Kv4Head), seqs, row0, ranges, moves, part, part_ml}) t += (b + 255) / 256 * 256;
         return t + 256;  // the well's own alignment
     }
 };
@@ -391,7 +735,8 @@ int32_t kv4_sizes(int64_t layers, int64_t nq, int64_t nkv, int64_t hd, int64_t m
     z->row0 = max_seqs * 4;
     z->ranges = max_seqs * (int64_t)sizeof(Kv4Range);
     z->moves = pages * (int64_t)sizeof(PageMove);
-    z->part = 256;
+    z->part = kPartCols * hd * 4;
+    z->part_ml = kPartCols * 8;
     return AESIR_OK;
 }
 
@@ -525,6 +870,32 @@ bool aligned16(const void *p, int64_t cols) { return ((uintptr_t)p & 15) == 0 &&
 
 unsigned grid_for(int64_t threads) { return (unsigned)std::min<int64_t>(std::max<int64_t>((threads + kThreads - 1) / kThreads, 1), 1 << 20); }
 
+// Units of attention work for column tiles of width 16 << v: every sequence's rounds cut into equal splits, so
+// that the batch gives about kUnits workgroups with kMinRounds rounds or more, and the partials fit.
+void plan_width(const aesir_kv4 *kv, int v, std::vector<Kv4Seq> &ds, Kv4Head &h, bool *split) {
+    const int64_t W = 16 << v, G = kv->nq / kv->nkv;
+    int64_t work = 0;
+    auto tiles = [&](const Kv4Seq &s) { return (s.rows * G + W - 1) / W; };
+    auto rounds = [&](const Kv4Seq &s) { return ((int64_t)s.length + kKeys - 1) / kKeys; };
+    for (const Kv4Seq &s : ds) work += tiles(s) * rounds(s) * kv->nkv;
+    int64_t chunk = std::max<int64_t>(kMinRounds, (work + kUnits - 1) / kUnits);
+    for (;; chunk *= 2) {
+        int64_t items = 0, parts = 0;
+        for (Kv4Seq &s : ds) {
+            const int64_t n = std::max<int64_t>(1, (rounds(s) + chunk - 1) / chunk);
+            s.splits[v] = (int32_t)n;
+            s.item0[v] = (int32_t)items;
+            s.part0[v] = (int32_t)parts;
+            items += tiles(s) * n;
+            if (n > 1) parts += tiles(s) * n;
+        }
+        if (parts * kv->nkv * W > kPartCols) continue;  // ends: one split needs no partials
+        h.items[v] = (int32_t)items;
+        *split = parts > 0;
+        return;
+    }
+}
+
 int32_t kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64_t n) {
     if (n < 0 || n > kv->book.max_seqs()) return fail(AESIR_ERR_INVALID, "KV4Cache.begin: bad sequence count");
     if (n > 0 && (!seqs || !rows)) return fail(AESIR_ERR_INVALID, "KV4Cache.begin: null argument");
@@ -566,7 +937,11 @@ int32_t kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64
     }
     kv->batch = true;
     kv->batch_rows = total;
+    kv->batch_cols = 0;
+    for (int64_t i = 0; i < n; i++) kv->batch_cols = std::max(kv->batch_cols, rows[i] * (kv->nq / kv->nkv));
     if (!kv->ctx) return AESIR_OK;
+    for (int v = 0; v < kKv4Widths; v++) plan_width(kv, v, ds, h, &kv->plan_splits[v]);
+    kv->plan = h;
     const Run runs[3] = {{kv->head, &h, (int64_t)sizeof h},
                          {kv->seqs, ds.data(), n * (int64_t)sizeof(Kv4Seq)},
                          {kv->row0, row0.data(), n * 4}};
@@ -613,10 +988,10 @@ int32_t aesir_kv4_create(aesir_ctx *ctx, int64_t num_layers, int64_t n_heads, in
             return AESIR_OK;
         }
         const int64_t mark = ctx->well_offset;
-        void *p[8] = {};
-        const int64_t bytes[8] = {z.pool, z.table, (int64_t)sizeof(Kv4Head), z.seqs, z.row0, z.ranges, z.moves, z.part};
+        void *p[9] = {};
+        const int64_t bytes[9] = {z.pool, z.table, (int64_t)sizeof(Kv4Head), z.seqs, z.row0, z.ranges, z.moves, z.part, z.part_ml};
         int32_t rc = AESIR_OK;
-        for (int i = 0; i < 8 && rc == AESIR_OK; i++) rc = well_alloc_bytes(ctx, bytes[i], &p[i]);
+        for (int i = 0; i < 9 && rc == AESIR_OK; i++) rc = well_alloc_bytes(ctx, bytes[i], &p[i]);
         if (rc == AESIR_OK && hipHostMalloc((void **)&kv->ring, kRingBytes, hipHostMallocDefault) != hipSuccess)
             rc = fail(AESIR_ERR_HIP, "hipHostMalloc of the cache's staging memory failed");
         if (rc != AESIR_OK) {
@@ -645,6 +1020,7 @@ int32_t aesir_kv4_create(aesir_ctx *ctx, int64_t num_layers, int64_t n_heads, in
         d.seqs = kv->seqs;
         d.row0 = kv->row0;
         d.part = (float *)p[7];
+        d.part_ml = (float *)p[8];
         kv->batch = true;  // clears the descriptor: the well's memory may have been used before
         rc = end_batch(kv);
         if (rc != AESIR_OK) {
@@ -725,11 +1101,20 @@ int32_t aesir_kv4_attention(aesir_kv4 *kv, int64_t layer, const void *query, int
         return fail(AESIR_ERR_SHAPE, "KV4Cache.attention: query/output rows narrower than heads * head_dim");
     if (!query || !output) return fail(AESIR_ERR_INVALID, "KV4Cache.attention: null tensor pointer");
     const Kv4AttnArgs a{(const h16 *)query, (h16 *)output, query_cols, output_cols, layer, (int32_t)query_rows,
-                        (float)(1.0 / std::sqrt((double)kv->hd))};
-    hipLaunchKernelGGL(kv4_attention_kernel, dim3((unsigned)std::min<int64_t>(query_rows * kv->nq, 1 << 20)), dim3(kWave), 0,
-                       kv->ctx->stream, kv->dev, a);
-    AESIR_LAUNCH_CHECK("kv4_attention_kernel");
-    return AESIR_OK;
+                        aligned16(query, query_cols) && aligned16(output, output_cols),
+                        (float)(1.4426950408889634 / std::sqrt((double)kv->hd))};
+    // the narrowest tile that holds a sequence's columns, up to 64 (32 at head_dim 256, by its registers)
+    const int v = kv->batch_cols <= 16 ? 0 : kv->batch_cols <= 32 || kv->hd == 256 ? 1 : 2;
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    AESIR_HIP_TRY(hipStreamIsCapturing(kv->ctx->stream, &st));
+    // a captured call may meet a batch that is split, whatever this one is
+    const bool merge = kv->plan_splits[v] || st != hipStreamCaptureStatusNone;
+    switch (kv->hd) {
+        case 32: return launch_attention<32>(kv->ctx->stream, kv->dev, a, v, kv->plan.items[v], merge, query_rows);
+        case 64: return launch_attention<64>(kv->ctx->stream, kv->dev, a, v, kv->plan.items[v], merge, query_rows);
+        case 128: return launch_attention<128>(kv->ctx->stream, kv->dev, a, v, kv->plan.items[v], merge, query_rows);
+        default: return launch_attention<256>(kv->ctx->stream, kv->dev, a, v, kv->plan.items[v], merge, query_rows);
+    }
 }
 
 int32_t aesir_kv4_read(aesir_kv4 *kv, int64_t layer, int64_t layers, const int64_t *seqs, const int64_t *pos, const int64_t *rows,

@@ -51,7 +51,7 @@ struct Kv4Dev {
     const Kv4Head *head;
     const Kv4Seq *seqs;
     const int32_t *row0;  // [max_seqs] first rows of the batch's sequences, or of the ranges
-    float *part;
+    float *part, *part_ml;  // split partials of a column: accumulators [hd], and (maximum, sum)
 
     __host__ __device__ int page_size() const { return 1 << page_shift; }
     __host__ __device__ int64_t head_bytes() const { return (int64_t)page_size() * hd / 4 * 5; }
