@@ -287,14 +287,21 @@ struct Kv4AttnArgs {
 constexpr int kAWaves = 4;
 constexpr int kKeys = 32;  // keys per round
 
-// The four values (two neighbouring nibbles each half) of x at nibble p under scales d and offsets m per half.
+// Masks and exponents of the unpacking, one in a scalar and one in a vector register: as literals each pair would
+// take an AND and an OR, since one instruction takes no two literals here.
+struct Kv4Magic {
+    unsigned low = 0x000F000Fu, high = 0x00F000F0u, one = 0x64006400u;
+    __device__ __forceinline__ Kv4Magic() { asm("" : "+s"(low), "+s"(high), "+v"(one)); }
+};
+
+// The values of nibble P of both halves of x under scales d and offsets m.
 template <int P>
-__device__ __forceinline__ h16x2 kv4_values(unsigned x, h16x2 d, h16x2 m) {
+__device__ __forceinline__ h16x2 kv4_values(const Kv4Magic &c, unsigned x, h16x2 d, h16x2 m) {
     h16x2 n;
     if constexpr (P % 2 == 0) {
-        n = as_h2(((x >> (4 * P)) & 0x000F000Fu) | 0x64006400u) - both((h16)1024.0f);
+        n = as_h2(((x >> (4 * P)) & c.low) | c.one) - both((h16)1024.0f);
     } else {  // 1024 + 16 n: no shift, the multiply-add undoes both exactly
-        n = __builtin_elementwise_fma(as_h2(((x >> (4 * (P - 1))) & 0x00F000F0u) | 0x64006400u), both((h16)0.0625f), both((h16)-64.0f));
+        n = __builtin_elementwise_fma(as_h2(((x >> (4 * (P - 1))) & c.high) | c.one), both((h16)0.0625f), both((h16)-64.0f));
     }
     return __builtin_elementwise_fma(n, d, m);
 }
@@ -362,13 +369,14 @@ __device__ __forceinline__ int out_dim(int r, int x, int p, int half) {
 }
 
 template <int HD, int NC>
-__global__ __launch_bounds__(kAWaves *kWave) void kv4_attention_kernel(Kv4Dev c, Kv4AttnArgs a) {
+__global__ __launch_bounds__(kAWaves *kWave, NC == 1 && HD <= 128 ? 3 : 1) void kv4_attention_kernel(Kv4Dev c, Kv4AttnArgs a) {
     constexpr int V = NC == 1 ? 0 : NC == 2 ? 1 : 2, W = 16 * NC;
     constexpr int NJ = HD / 32, NP = NJ < 4 ? NJ : 4, NB = Kv4Round<HD>::NB, NG = Kv4Round<HD>::NG;
     constexpr int LD = HD + 4;  // LDS row of a column
     __shared__ float ml[kAWaves][W][2];
     __shared__ __align__(16) float ox[kAWaves][16][LD];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int G = c.nq / c.nkv, n = c.head->n, items = c.head->items[V];
     for (int64_t u = blockIdx.x; u < (int64_t)items * c.nkv; u += gridDim.x) {
         const int kvh = (int)(u % c.nkv), unit = (int)(u / c.nkv);
@@ -405,12 +413,13 @@ __global__ __launch_bounds__(kAWaves *kWave) void kv4_attention_kernel(Kv4Dev c,
                 for (int p = 0; p < NP; p++) acc[t][x][p][0] = acc[t][x][p][1] = f32x4{0, 0, 0, 0};
         }
 
+        const Kv4Magic magic;
         const int32_t *table = c.table + (int64_t)s.slot * c.table_stride;
         auto fetch = [&](int r, Kv4Round<HD> &d) {
             const int pos = r * kKeys;
             d.load(c, c.block(__builtin_amdgcn_readfirstlane(table[pos >> c.page_shift]), a.layer, kvh), pos & (c.page_size() - 1), i, g);
         };
-        auto round = [&](int r, Kv4Round<HD> &d) {
+        auto round = [&](int r, Kv4Round<HD> &d, auto all) {  // all: every column sees every key of the round
             f32x4 sc[2][NC];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
@@ -420,16 +429,16 @@ __global__ __launch_bounds__(kAWaves *kWave) void kv4_attention_kernel(Kv4Dev c,
                 for (int j = 0; j < NJ; j++) {
                     const h16x2 dd = both(d.ks[t][j * NG / NJ].x), mm = both(d.ks[t][j * NG / NJ].y);
                     const unsigned w = d.k[t][j];
-                    const u32x4 ka = {h2_bits(kv4_values<0>(w, dd, mm)), h2_bits(kv4_values<1>(w, dd, mm)),
-                                      h2_bits(kv4_values<2>(w, dd, mm)), h2_bits(kv4_values<3>(w, dd, mm))};
+                    const u32x4 ka = {h2_bits(kv4_values<0>(magic, w, dd, mm)), h2_bits(kv4_values<1>(magic, w, dd, mm)),
+                                      h2_bits(kv4_values<2>(magic, w, dd, mm)), h2_bits(kv4_values<3>(magic, w, dd, mm))};
 #pragma unroll
                     for (int x = 0; x < NC; x++) sc[t][x] = mfma16x16x32(ka, q[x][j], sc[t][x]);
                 }
             }
-            const bool whole = r * kKeys + kKeys - 1 <= low;  // every column sees every key
+            constexpr bool whole = decltype(all)::value;
             const int k0 = r * kKeys + 8 * g;
-            unsigned bad[NB] = {};  // bit e: value group of key k0 + e is NaN (rounds that are not whole)
-            if (!whole) {
+            unsigned bad[NB] = {};  // bit e: the value group of key k0 + e is NaN
+            if constexpr (!whole) {
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -473,7 +482,7 @@ __global__ __launch_bounds__(kAWaves *kWave) void kv4_attention_kernel(Kv4Dev c,
                 float pr[8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    pr[e] = __builtin_amdgcn_exp2f((sc[e / 4][x][e % 4] - ref) * a.scale + 15.0f);
+                    pr[e] = __builtin_amdgcn_exp2f(fmaf(sc[e / 4][x][e % 4] - ref, a.scale, 15.0f));
                     l[x] += pr[e];
                 }
 #pragma unroll
@@ -495,8 +504,8 @@ __global__ __launch_bounds__(kAWaves *kWave) void kv4_attention_kernel(Kv4Dev c,
                         u32x4 va, vb;
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            va[e] = h2_bits(kv4_values<P>(lo[e], as_h2(d.vd[b][e]), as_h2(d.vm[b][e])));
-                            vb[e] = h2_bits(kv4_values<P>(hi[e], as_h2(d.vd[b][e]), as_h2(d.vm[b][e])));
+                            va[e] = h2_bits(kv4_values<P>(magic, lo[e], as_h2(d.vd[b][e]), as_h2(d.vm[b][e])));
+                            vb[e] = h2_bits(kv4_values<P>(magic, hi[e], as_h2(d.vd[b][e]), as_h2(d.vm[b][e])));
                         }
 #pragma unroll
                         for (int x = 0; x < NC; x++) {
@@ -509,7 +518,7 @@ __global__ __launch_bounds__(kAWaves *kWave) void kv4_attention_kernel(Kv4Dev c,
                 step(std::integral_constant<int, 1>{});
                 step(std::integral_constant<int, 2>{});
                 step(std::integral_constant<int, 3>{});
-                if (!whole && __any(bad[b] != 0)) {  // NaN for the columns that see a NaN group, in its dims
+                if constexpr (!whole) if (__any(bad[b] != 0)) {  // NaN for the columns that see a NaN group, in its dims
                     u32x4 ia;
 #pragma unroll
                     for (int e = 0; e < 4; e++) ia[e] = (bad[b] >> (2 * e) & 1 ? 0x3C00u : 0u) | (bad[b] >> (2 * e + 1) & 1 ? 0x3C000000u : 0u);
@@ -530,15 +539,29 @@ __global__ __launch_bounds__(kAWaves *kWave) void kv4_attention_kernel(Kv4Dev c,
             }
         };
         int r = split * per + wave;
-        if (r < r1) {  // the next round's loads are issued before a round is computed
-            Kv4Round<HD> cur, next;
-            fetch(r, cur);
-            for (; r + kAWaves < r1; r += kAWaves) {
-                fetch(r + kAWaves, next);
-                round(r, cur);
-                cur = next;
+        // A round's loads are issued before the round ahead of it is computed, on a path of their own each, so that
+        // the waits count them. The loop takes rounds that every column sees whole; at most two are left, since
+        // the columns of a tile differ by less than a round of every wave.
+        static_assert(W / kKeys < kAWaves, "rounds a tile may see in part");
+        if (r < r1) {
+            const int whole = min(r1, (low + 1) / kKeys);
+            const std::true_type all;
+            const std::false_type part;
+            Kv4Round<HD> d0, d1;
+            fetch(r, d0);
+            for (; r + 2 * kAWaves < r1 && r + kAWaves < whole; r += 2 * kAWaves) {
+                fetch(r + kAWaves, d1);
+                round(r, d0, all);
+                fetch(r + 2 * kAWaves, d0);
+                round(r + kAWaves, d1, all);
             }
-            round(r, cur);
+            if (r + kAWaves < r1) {
+                fetch(r + kAWaves, d1);
+                round(r, d0, part);
+                round(r + kAWaves, d1, part);
+            } else {
+                round(r, d0, part);
+            }
         }
 
         // the waves meet: maxima and sums of all columns, then 16 columns of accumulators at a time
