@@ -19,40 +19,54 @@ constexpr int kThreads = 256;
 // hold too little.
 struct Kv4Upload {
     const uint32_t *src;
-    uint32_t *dst[3];   // contiguous runs, in the order of src
-    int32_t words[3];
-    int32_t *table;     // then `updates` pairs (table entry, page)
+    uint32_t *dst;      // `words` words of src, then `fill` words of kNone
+    int32_t words, fill;
+    int32_t *table;     // `updates` pairs (table entry, page) behind them in src
     int32_t updates;
 };
 
 __global__ __launch_bounds__(kThreads) void kv4_upload_kernel(Kv4Upload u) {
-    const int all = u.words[0] + u.words[1] + u.words[2];
+    const int all = u.words + u.fill;
     for (int i = blockIdx.x * kThreads + threadIdx.x; i < all + u.updates; i += gridDim.x * kThreads) {
-        if (i >= all) {
-            const uint32_t *e = u.src + all + 2 * (int64_t)(i - all);
+        if (i < u.words) {
+            u.dst[i] = u.src[i];
+        } else if (i < all) {
+            u.dst[i] = kNone;
+        } else {
+            const uint32_t *e = u.src + u.words + 2 * (int64_t)(i - all);
             u.table[e[0]] = (int32_t)e[1];
-            continue;
         }
-        int j = i, run = 0;
-        while (j >= u.words[run]) j -= u.words[run++];
-        u.dst[run][j] = u.src[i];
     }
 }
 
-// Index of the last of n ascending values that is <= x (the first is 0, x >= 0), from LDS.
-__device__ __forceinline__ int last_not_above(const int *v, int n, int x) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (v[mid] <= x)
-            lo = mid;
-        else
-            hi = mid;
+// The record {slot, length or position, rows, first row} that a lane's row belongs to, of records in row order ended by
+// ones of kNone; rows 0 past the last. Lanes hold a record each and answer the wave's distinct rows (few: the rows of a wave
+// are neighbours) one after another, so that the only memory latency is the one load of the records.
+__device__ __forceinline__ i32x4 find_row(const char *records, int stride, int row, int lane) {
+    i32x4 mine = {0, 0, 0, 0};
+    uint64_t open = __ballot(true);
+    for (int base = 0; open; base += kWave) {
+        const i32x4 r = *reinterpret_cast<const i32x4 *>(records + (int64_t)(base + lane) * stride);
+        const bool last = __builtin_amdgcn_readlane(r[3], kWave - 1) == kNone;  // no further records
+        uint64_t todo = open;
+        while (todo) {
+            const int x = __builtin_amdgcn_readlane(row, __builtin_ctzll(todo));
+            const int at = __popcll(__ballot(r[3] <= x)) - 1;  // the last record that starts at or before row x
+            const uint64_t same = __ballot(row == x);
+            if (at >= 0) {
+                const i32x4 f = {__builtin_amdgcn_readlane(r[0], at), __builtin_amdgcn_readlane(r[1], at),
+                                 __builtin_amdgcn_readlane(r[2], at), __builtin_amdgcn_readlane(r[3], at)};
+                if (row == x) mine = f;
+            }
+            if (last || at < kWave - 1) open &= ~same;
+            todo &= ~same;
+        }
     }
-    return lo;
+    if (row - mine[3] >= mine[2]) mine[2] = 0;
+    return mine;
 }
 
-constexpr int kMaxSeqs = 4096;  // a batch's first rows fit LDS
+constexpr int kMaxSeqs = 4096;
 
 // ------------------------------------------------------------------ append
 //
@@ -126,6 +140,17 @@ __device__ __forceinline__ Kv4Code kv4_encode(u32x4 x) {
     return c;
 }
 
+// What a thread of the append and read kernels works on: four rows of one head are 4 hd / 8 neighbouring threads.
+struct Kv4Place {
+    int row, head, chunk;
+    __device__ __forceinline__ Kv4Place(const Kv4Dev &c, unsigned u) {
+        const unsigned per_row = c.hd / 8, g = u / per_row, g4 = g / 4;
+        chunk = (int)(u % per_row);
+        head = (int)(g4 % c.nkv);
+        row = (int)(g4 / c.nkv * 4 + g % 4);
+    }
+};
+
 struct Kv4AppendArgs {
     const h16 *k, *v;
     int64_t k_stride, v_stride;
@@ -147,22 +172,15 @@ __device__ __forceinline__ u32x4 load8(const h16 *p) {
 
 template <bool VEC>
 __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Dev c, Kv4AppendArgs a) {
-    __shared__ int row0[kMaxSeqs];
-    const int n = c.head->n, total = min(c.head->total_rows, a.rows);
-    for (int i = threadIdx.x; i < n; i += kThreads) row0[i] = c.row0[i];
-    __syncthreads();
-    const int per_row = c.hd / 8;                                       // threads per row and head
-    const int64_t units = ((int64_t)total + 3) / 4 * c.nkv * 4 * per_row;  // four rows of one head together
-    for (int64_t u = (int64_t)blockIdx.x * kThreads + threadIdx.x; u < units; u += (int64_t)gridDim.x * kThreads) {
-        const int chunk = (int)(u % per_row);
-        const int64_t g = u / per_row;
-        const int row = (int)(g / (4 * c.nkv)) * 4 + (int)(g % 4), head = (int)(g / 4 % c.nkv);
-        if (row >= total) continue;  // uniform over the quad
+    const int lane = threadIdx.x & 63;
+    const Kv4Place q(c, blockIdx.x * kThreads + threadIdx.x);
+    const int per_row = c.hd / 8, row = q.row, head = q.head, chunk = q.chunk;
+    const i32x4 s = find_row(reinterpret_cast<const char *>(c.seqs), sizeof(Kv4Seq), row, lane);
+    if (row < a.rows && s[2] > 0) {  // uniform over the quad
         const u32x4 kx = load8<VEC>(a.k + (int64_t)row * a.k_stride + head * c.hd + 8 * chunk);
         const u32x4 vx = load8<VEC>(a.v + (int64_t)row * a.v_stride + head * c.hd + 8 * chunk);
-        const Kv4Seq &s = c.seqs[last_not_above(row0, n, row)];
-        const int pos = s.length - s.rows + (row - s.row0), slot = pos & (c.page_size() - 1);
-        char *b = c.block(c.table[(int64_t)s.slot * c.table_stride + (pos >> c.page_shift)], a.layer, head);
+        const int pos = s[1] - s[2] + (row - s[3]), slot = pos & (c.page_size() - 1);
+        char *b = c.block(c.table[(int64_t)s[0] * c.table_stride + (pos >> c.page_shift)], a.layer, head);
         const Kv4Code ck = kv4_encode(kx), cv = kv4_encode(vx);
         reinterpret_cast<unsigned *>(b)[slot * per_row + chunk] = ck.word;
         reinterpret_cast<unsigned *>(b + c.v_off())[(slot / 4 * per_row + chunk) * 4 + slot % 4] = cv.word;
@@ -183,7 +201,7 @@ struct Kv4ReadArgs {
     int64_t k_stride, v_stride;
     int64_t layer, layers;
     const Kv4Range *ranges;
-    int32_t n, rows, all_rows, first_row;  // ranges, their rows, output rows of a layer, first output row
+    int32_t all_rows, first_row;  // output rows of a layer, first output row
 };
 
 template <bool VEC>
@@ -208,19 +226,15 @@ __device__ __forceinline__ u32x4 kv4_decode(unsigned w, h16 d, h16 m) {
 
 template <bool VEC>
 __global__ __launch_bounds__(kThreads) void kv4_read_kernel(Kv4Dev c, Kv4ReadArgs a) {
-    __shared__ int row0[kMaxSeqs];
-    for (int i = threadIdx.x; i < a.n; i += kThreads) row0[i] = a.ranges[i].row0;
-    __syncthreads();
-    const int per_row = c.hd / 8;
-    const int64_t per_layer = ((int64_t)a.rows + 3) / 4 * c.nkv * 4 * per_row, units = per_layer * a.layers;
-    for (int64_t u = (int64_t)blockIdx.x * kThreads + threadIdx.x; u < units; u += (int64_t)gridDim.x * kThreads) {
-        const int64_t layer = u / per_layer, x = u % per_layer, g = x / per_row;
-        const int chunk = (int)(x % per_row);
-        const int row = (int)(g / (4 * c.nkv)) * 4 + (int)(g % 4), head = (int)(g / 4 % c.nkv);
-        if (row >= a.rows) continue;
-        const Kv4Range r = a.ranges[last_not_above(row0, a.n, row)];
-        const int pos = r.pos + (row - r.row0), slot = pos & (c.page_size() - 1), grp = chunk / 4;
-        const char *b = c.block(c.table[(int64_t)r.slot * c.table_stride + (pos >> c.page_shift)], a.layer + layer, head);
+    const int lane = threadIdx.x & 63, per_row = c.hd / 8;
+    const Kv4Place q(c, blockIdx.x * kThreads + threadIdx.x);
+    const int row = q.row, head = q.head, chunk = q.chunk;
+    const i32x4 r = find_row(reinterpret_cast<const char *>(a.ranges), sizeof(Kv4Range), row, lane);
+    if (r[2] == 0) return;
+    const int pos = r[1] + (row - r[3]), slot = pos & (c.page_size() - 1), grp = chunk / 4;
+    const int64_t page = c.table[(int64_t)r[0] * c.table_stride + (pos >> c.page_shift)];
+    for (int64_t layer = blockIdx.y; layer < a.layers; layer += gridDim.y) {
+        const char *b = c.block(page, a.layer + layer, head);
         const unsigned kw = reinterpret_cast<const unsigned *>(b)[slot * per_row + chunk];
         const unsigned vw = reinterpret_cast<const unsigned *>(b + c.v_off())[(slot / 4 * per_row + chunk) * 4 + slot % 4];
         const h16x2 ks = reinterpret_cast<const h16x2 *>(b + c.k_scale_off())[slot * (c.hd / kKv4Group) + grp];
@@ -284,7 +298,8 @@ struct Kv4AttnArgs {
     float scale;   // log2(e) / sqrt(hd)
 };
 
-constexpr int kAWaves = 4;
+constexpr int kMergeWaves = 4;
+constexpr int64_t kFewUnits = 512;  // workgroups up to which a unit takes eight waves
 constexpr int kKeys = 32;  // keys per round
 
 // Masks and exponents of the unpacking, one in a scalar and one in a vector register: as literals each pair would
@@ -306,6 +321,25 @@ __device__ __forceinline__ h16x2 kv4_values(const Kv4Magic &c, unsigned x, h16x2
     return __builtin_elementwise_fma(n, d, m);
 }
 
+// A lane's place in the blocks of a cache: byte offsets of its share of a round behind the round's own.
+template <int HD>
+struct Kv4Lane {
+    static constexpr int NJ = HD / 32, NB = NJ == 8 ? 2 : 1;
+    unsigned k, ks, v[NB], vs[NB];  // keys 8 (i / 4) + i % 4 (the second tile's four behind); 8-dim blocks and their scales
+
+    __device__ __forceinline__ Kv4Lane(const Kv4Dev &c, int i, int g) {
+        const int key = 8 * (i / 4) + i % 4;
+        k = key * (HD / 2) + g * (HD / 8);
+        ks = c.k_scale_off() + (key * NJ + g * NJ / 4) * 4;
+#pragma unroll
+        for (int x = 0; x < NB; x++) {
+            const int block = NJ < 4 ? i % (4 * NJ) : i + 16 * x;
+            v[x] = c.v_off() + (2 * g * (HD / 8) + block) * 16;
+            vs[x] = c.v_d_off() + (block / 4 * c.page_size() + 8 * g) * 2;
+        }
+    }
+};
+
 template <int HD>
 struct Kv4Round {  // one lane's share of 32 keys
     static constexpr int NJ = HD / 32, NG = NJ == 8 ? 2 : 1, NB = NJ == 8 ? 2 : 1;
@@ -313,11 +347,12 @@ struct Kv4Round {  // one lane's share of 32 keys
     h16x2 ks[2][NG];
     u32x4 v[NB][2], vd[NB], vm[NB];
 
-    __device__ __forceinline__ void load(const Kv4Dev &c, const char *b, int s0, int i, int g) {
+    // b: the block (uniform), s0: the round's first position in its page
+    __device__ __forceinline__ void load(const char *b, int s0, const Kv4Lane<HD> &o, int m_off) {
+        const char *rows = b + s0 * (HD / 2), *scales = b + s0 * NJ * 4, *vscales = b + s0 * 2;
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const int key = s0 + 8 * (i / 4) + 4 * t + i % 4;
-            const char *p = b + key * (HD / 2) + g * (HD / 8);
+            const char *p = rows + (size_t)(o.k + t * 2 * HD);
             if constexpr (NJ == 1) {
                 k[t][0] = *reinterpret_cast<const unsigned *>(p);
             } else if constexpr (NJ == 2) {
@@ -332,32 +367,47 @@ struct Kv4Round {  // one lane's share of 32 keys
                     for (int e = 0; e < 4; e++) k[t][j + e] = x[e];
                 }
             }
-            const h16x2 *ps = reinterpret_cast<const h16x2 *>(b + c.k_scale_off()) + key * NJ + g * NJ / 4;
+            const h16x2 *ps = reinterpret_cast<const h16x2 *>(scales + (size_t)(o.ks + t * 16 * NJ));
 #pragma unroll
             for (int x = 0; x < NG; x++) ks[t][x] = ps[x];
         }
 #pragma unroll
         for (int x = 0; x < NB; x++) {
-            const int block = NJ < 4 ? i % (4 * NJ) : i + 16 * x;
 #pragma unroll
-            for (int h = 0; h < 2; h++) v[x][h] = ld16(b + c.v_off() + ((s0 / 4 + 2 * g + h) * (HD / 8) + block) * 16);
-            vd[x] = ld16(b + c.v_d_off() + (block / 4 * c.page_size() + s0 + 8 * g) * 2);
-            vm[x] = ld16(b + c.v_m_off() + (block / 4 * c.page_size() + s0 + 8 * g) * 2);
+            for (int h = 0; h < 2; h++) v[x][h] = ld16(rows + (size_t)(o.v[x] + h * 2 * HD));
+            vd[x] = ld16(vscales + (size_t)o.vs[x]);
+            vm[x] = ld16(vscales + m_off + (size_t)o.vs[x]);
         }
     }
 };
 
-// Index of the batch's last sequence whose first unit is <= unit; the whole wave calls it.
+// What a unit of attention work needs of its sequence.
+struct Kv4Unit {
+    int slot, length, rows, row0;    // the sequence
+    int splits, part, local;         // splits of a tile, partial slot, (tile, split) index in the sequence
+};
+
+// The sequence of a unit (a row with `by_row`) of column width V; rows 0 past the last. Lanes hold a record each; the
+// whole wave calls it.
 template <int V>
-__device__ __forceinline__ int find_unit(const Kv4Seq *seqs, int n, int unit, int lane) {
-    int at = 0;
-    for (int base = 0; base < n; base += kWave) {
-        const bool below = base + lane < n && seqs[base + lane].item0[V] <= unit;
-        const int count = __popcll(__ballot(below));
-        if (count) at = base + count - 1;
-        if (count < kWave) break;
+__device__ __forceinline__ Kv4Unit find_unit(const Kv4Seq *seqs, int unit, bool by_row, int lane) {
+    Kv4Unit r{};
+    for (int base = 0;; base += kWave) {
+        const i32x4 *p = reinterpret_cast<const i32x4 *>(seqs + base + lane);
+        const i32x4 s = p[0], plan = p[1 + V];
+        const int at = __popcll(__ballot((by_row ? s[3] : plan[0]) <= unit)) - 1;
+        if (at >= 0) {
+            r.slot = __builtin_amdgcn_readlane(s[0], at);
+            r.length = __builtin_amdgcn_readlane(s[1], at);
+            r.rows = __builtin_amdgcn_readlane(s[2], at);
+            r.row0 = __builtin_amdgcn_readlane(s[3], at);
+            r.local = unit - __builtin_amdgcn_readlane(plan[0], at);
+            r.splits = __builtin_amdgcn_readlane(plan[1], at);
+            r.part = __builtin_amdgcn_readlane(plan[2], at);
+        }
+        if (at < kWave - 1) break;
     }
-    return __builtin_amdgcn_readfirstlane(at);
+    return r;
 }
 
 // The dim of accumulator (x, p, half) in matrix row r.
@@ -368,26 +418,35 @@ __device__ __forceinline__ int out_dim(int r, int x, int p, int half) {
     return 8 * (r + 16 * x) + 2 * p + half;
 }
 
-template <int HD, int NC>
-__global__ __launch_bounds__(kAWaves *kWave, NC == 1 && HD <= 128 ? 3 : 1) void kv4_attention_kernel(Kv4Dev c, Kv4AttnArgs a) {
+template <int HD, int NC, int NW>
+__global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1) void kv4_attention_kernel(Kv4Dev c, Kv4AttnArgs a) {
     constexpr int V = NC == 1 ? 0 : NC == 2 ? 1 : 2, W = 16 * NC;
     constexpr int NJ = HD / 32, NP = NJ < 4 ? NJ : 4, NB = Kv4Round<HD>::NB, NG = Kv4Round<HD>::NG;
     constexpr int LD = HD + 4;  // LDS row of a column
-    __shared__ float ml[kAWaves][W][2];
-    __shared__ __align__(16) float ox[kAWaves][16][LD];
+    __shared__ float ml[NW][W][2];
+    __shared__ __align__(16) float ox[NW][16][LD];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int G = c.nq / c.nkv, n = c.head->n, items = c.head->items[V];
-    for (int64_t u = blockIdx.x; u < (int64_t)items * c.nkv; u += gridDim.x) {
-        const int kvh = (int)(u % c.nkv), unit = (int)(u / c.nkv);
-        const Kv4Seq &s = c.seqs[find_unit<V>(c.seqs, n, unit, lane)];
-        const int local = unit - s.item0[V], splits = s.splits[V], cols = s.rows * G, tiles = (cols + W - 1) / W;
-        const int tile = tiles - 1 - local / splits, split = local % splits;
+    const int G = c.nq / c.nkv;
+    const Kv4Lane<HD> place(c, i, g);
+    const int m_off = c.v_m_off() - c.v_d_off();
+    const Kv4Magic magic;
+    for (unsigned u = blockIdx.x;; u += gridDim.x) {
+        const int kvh = (int)(u % (unsigned)c.nkv), unit = (int)(u / (unsigned)c.nkv);
+        const Kv4Unit s = find_unit<V>(c.seqs, unit, false, lane);
+        const int splits = s.splits, cols = s.rows * G, tiles = (cols + W - 1) / W;
+        if (s.local >= tiles * splits) break;  // past the last unit (no batch: the first)
+        const int tile = tiles - 1 - s.local / splits, split = s.local % splits;
         const int before = s.length - s.rows;
         const int low = before + tile * W / G;                                    // last position of the first column
         const int keys = before + min(s.rows - 1, (tile * W + W - 1) / G) + 1;     // positions the tile sees
         const int rounds = (keys + kKeys - 1) / kKeys, per = (rounds + splits - 1) / splits;
-        const int r1 = min(rounds, (split + 1) * per);
+        const int r0 = split * per + wave, r1 = min(rounds, (split + 1) * per);
+
+        // pages of this wave's next 64 rounds, one a lane
+        const int32_t *table = c.table + (int64_t)s.slot * c.table_stride;
+        auto page_ids = [&](int r) { return table[min(r + lane * NW, rounds - 1) * kKeys >> c.page_shift]; };
+        int pages = page_ids(r0);
 
         // queries: column i of each 16, dims g HD / 4 + 8 j ..
         u32x4 q[NC][NJ];
@@ -413,13 +472,12 @@ __global__ __launch_bounds__(kAWaves *kWave, NC == 1 && HD <= 128 ? 3 : 1) void 
                 for (int p = 0; p < NP; p++) acc[t][x][p][0] = acc[t][x][p][1] = f32x4{0, 0, 0, 0};
         }
 
-        const Kv4Magic magic;
-        const int32_t *table = c.table + (int64_t)s.slot * c.table_stride;
-        auto fetch = [&](int r, Kv4Round<HD> &d) {
-            const int pos = r * kKeys;
-            d.load(c, c.block(__builtin_amdgcn_readfirstlane(table[pos >> c.page_shift]), a.layer, kvh), pos & (c.page_size() - 1), i, g);
+        const char *head_base = c.pool + a.layer * c.layer_bytes + kvh * c.head_bytes();
+        auto fetch = [&](int x, Kv4Round<HD> &d) {  // the wave's x-th round
+            const int page = __builtin_amdgcn_readlane(pages, x & (kWave - 1));
+            d.load(head_base + page * c.page_bytes, (r0 + x * NW) * kKeys & (c.page_size() - 1), place, m_off);
         };
-        auto round = [&](int r, Kv4Round<HD> &d, auto all) {  // all: every column sees every key of the round
+        auto round = [&](int r, Kv4Round<HD> &d) {
             f32x4 sc[2][NC];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
@@ -435,10 +493,10 @@ __global__ __launch_bounds__(kAWaves *kWave, NC == 1 && HD <= 128 ? 3 : 1) void 
                     for (int x = 0; x < NC; x++) sc[t][x] = mfma16x16x32(ka, q[x][j], sc[t][x]);
                 }
             }
-            constexpr bool whole = decltype(all)::value;
+            const bool whole = r * kKeys + kKeys - 1 <= low;  // every column sees every key (uniform)
             const int k0 = r * kKeys + 8 * g;
             unsigned bad[NB] = {};  // bit e: the value group of key k0 + e is NaN
-            if constexpr (!whole) {
+            if (!whole) {
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -518,7 +576,7 @@ __global__ __launch_bounds__(kAWaves *kWave, NC == 1 && HD <= 128 ? 3 : 1) void 
                 step(std::integral_constant<int, 1>{});
                 step(std::integral_constant<int, 2>{});
                 step(std::integral_constant<int, 3>{});
-                if constexpr (!whole) if (__any(bad[b] != 0)) {  // NaN for the columns that see a NaN group, in its dims
+                if (!whole && __any(bad[b] != 0)) {  // NaN for the columns that see a NaN group, in its dims
                     u32x4 ia;
 #pragma unroll
                     for (int e = 0; e < 4; e++) ia[e] = (bad[b] >> (2 * e) & 1 ? 0x3C00u : 0u) | (bad[b] >> (2 * e + 1) & 1 ? 0x3C000000u : 0u);
@@ -538,29 +596,18 @@ __global__ __launch_bounds__(kAWaves *kWave, NC == 1 && HD <= 128 ? 3 : 1) void 
                 }
             }
         };
-        int r = split * per + wave;
-        // A round's loads are issued before the round ahead of it is computed, on a path of their own each, so that
-        // the waits count them. The loop takes rounds that every column sees whole; at most two are left, since
-        // the columns of a tile differ by less than a round of every wave.
-        static_assert(W / kKeys < kAWaves, "rounds a tile may see in part");
-        if (r < r1) {
-            const int whole = min(r1, (low + 1) / kKeys);
-            const std::true_type all;
-            const std::false_type part;
-            Kv4Round<HD> d0, d1;
-            fetch(r, d0);
-            for (; r + 2 * kAWaves < r1 && r + kAWaves < whole; r += 2 * kAWaves) {
-                fetch(r + kAWaves, d1);
-                round(r, d0, all);
-                fetch(r + 2 * kAWaves, d0);
-                round(r + kAWaves, d1, all);
-            }
-            if (r + kAWaves < r1) {
-                fetch(r + kAWaves, d1);
-                round(r, d0, part);
-                round(r + kAWaves, d1, part);
-            } else {
-                round(r, d0, part);
+        // A round's loads are issued before the round ahead of it is computed. The last round issues its own again (they
+        // hit the cache): a load on one path only would make every wait behind it wait for all.
+        const int mine = r0 < r1 ? (r1 - r0 + NW - 1) / NW : 0;
+        if (mine > 0) {
+            Kv4Round<HD> cur, next;
+            fetch(0, cur);
+            for (int x = 0; x < mine; x++) {
+                const int y = min(x + 1, mine - 1);
+                if ((y & (kWave - 1)) == 0 && y > x) pages = page_ids(r0 + y * NW);
+                fetch(y, next);
+                round(r0 + x * NW, cur);
+                cur = next;
             }
         }
 
@@ -579,8 +626,8 @@ __global__ __launch_bounds__(kAWaves *kWave, NC == 1 && HD <= 128 ? 3 : 1) void 
         for (int t = 0; t < NC; t++) {
             float up = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kAWaves; w++) up = fmaxf(up, ml[w][16 * t + i][0]);
-            const float ref = up == -INFINITY ? 0.0f : up, mine = __builtin_amdgcn_exp2f((m[t] - ref) * a.scale);
+            for (int w = 0; w < NW; w++) up = fmaxf(up, ml[w][16 * t + i][0]);
+            const float ref = up == -INFINITY ? 0.0f : up, scale = __builtin_amdgcn_exp2f((m[t] - ref) * a.scale);
 #pragma unroll
             for (int e = 0; e < 4; e++)
 #pragma unroll
@@ -588,22 +635,24 @@ __global__ __launch_bounds__(kAWaves *kWave, NC == 1 && HD <= 128 ? 3 : 1) void 
 #pragma unroll
                     for (int p = 0; p < NP; p++) {
                         float *o = &ox[wave][i][out_dim<HD>(4 * g + e, x, p, 0)];
-                        o[0] = acc[t][x][p][0][e] * mine;
-                        o[1] = acc[t][x][p][1][e] * mine;
+                        o[0] = acc[t][x][p][0][e] * scale;
+                        o[1] = acc[t][x][p][1][e] * scale;
                     }
             __syncthreads();
-            // thread: HD / 16 dims of one column
-            constexpr int D = HD / 16;
-            const int col = threadIdx.x / 16, dim = threadIdx.x % 16 * D, gc = tile * W + 16 * t + col, row = gc / G;
+            // thread: D dims of one column
+            constexpr int T = NW * 4, D = HD / T;
+            const int col = threadIdx.x / T, dim = threadIdx.x % T * D, gc = tile * W + 16 * t + col, row = gc / G;
             if (gc < cols && s.row0 + row < a.rows) {
-                float M = -INFINITY, L = 0.0f, o[D];
+                float M = -INFINITY, L = 0.0f, o[D] = {};
 #pragma unroll
-                for (int w = 0; w < kAWaves; w++) M = fmaxf(M, ml[w][16 * t + col][0]);
+                for (int w = 0; w < NW; w++) M = fmaxf(M, ml[w][16 * t + col][0]);
                 const float mref = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-                for (int w = 0; w < kAWaves; w++) L += ml[w][16 * t + col][1] * __builtin_amdgcn_exp2f((ml[w][16 * t + col][0] - mref) * a.scale);
+                for (int w = 0; w < NW; w++) {
+                    L += ml[w][16 * t + col][1] * __builtin_amdgcn_exp2f((ml[w][16 * t + col][0] - mref) * a.scale);
 #pragma unroll
-                for (int d = 0; d < D; d++) o[d] = (ox[0][col][dim + d] + ox[1][col][dim + d]) + (ox[2][col][dim + d] + ox[3][col][dim + d]);
+                    for (int d = 0; d < D; d++) o[d] += ox[w][col][dim + d];
+                }
                 if (splits == 1) {
                     h16 *p = a.out + (int64_t)(s.row0 + row) * a.out_stride + (kvh * G + gc % G) * HD + dim;
                     h16 r16[D];
@@ -615,8 +664,8 @@ __global__ __launch_bounds__(kAWaves *kWave, NC == 1 && HD <= 128 ? 3 : 1) void 
                         for (int d = 0; d < D; d++) p[d] = r16[d];
                     }
                 } else {
-                    const int64_t at = ((int64_t)(s.part0[V] + local) * c.nkv + kvh) * W + 16 * t + col;
-                    if (threadIdx.x % 16 == 0) *reinterpret_cast<float2 *>(c.part_ml + 2 * at) = float2{M, L};
+                    const int64_t at = ((int64_t)(s.part + s.local) * c.nkv + kvh) * W + 16 * t + col;
+                    if (threadIdx.x % T == 0) *reinterpret_cast<float2 *>(c.part_ml + 2 * at) = float2{M, L};
                     __builtin_memcpy(__builtin_assume_aligned(c.part + at * HD + dim, 4 * D < 16 ? 4 * D : 16), o, sizeof o);
                 }
             }
@@ -626,70 +675,94 @@ __global__ __launch_bounds__(kAWaves *kWave, NC == 1 && HD <= 128 ? 3 : 1) void 
 }
 
 // The splits of a column joined: o = sum_s 2^(scale (m_s - M)) acc_s / sum_s 2^(scale (m_s - M)) l_s. One workgroup
-// per (row, query head); its waves take the splits in turn.
-template <int HD>
-__global__ __launch_bounds__(kAWaves *kWave) void kv4_merge_kernel(Kv4Dev c, Kv4AttnArgs a, int v) {
-    constexpr int D = HD >= kWave ? HD / kWave : 1;  // dims per lane
-    __shared__ float ox[kAWaves][HD], lx[kAWaves];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int G = c.nq / c.nkv, n = c.head->n, total = min(c.head->total_rows, a.rows), W = 16 << v;
-    for (int64_t u = blockIdx.x; u < (int64_t)total * c.nq; u += gridDim.x) {
-        const int row = (int)(u / c.nq), head = (int)(u % c.nq);
-        int at = 0;
-        for (int base = 0; base < n; base += kWave) {
-            const int count = __popcll(__ballot(base + lane < n && c.row0[base + lane] <= row));
-            if (count) at = base + count - 1;
-            if (count < kWave) break;
-        }
-        const Kv4Seq &s = c.seqs[__builtin_amdgcn_readfirstlane(at)];
-        const int splits = s.splits[v];
-        if (splits == 1) continue;  // uniform over the workgroup
-        const int col = (row - s.row0) * G + head % G, tiles = (s.rows * G + W - 1) / W;
-        // partial of split x: ((part0 + (tiles - 1 - col / W) splits + x) nkv + KV head) W + col % W
-        const int64_t first = ((int64_t)(s.part0[v] + (tiles - 1 - col / W) * splits) * c.nkv + head / G) * W + col % W;
-        const int64_t step = (int64_t)c.nkv * W;
-        float M = -INFINITY;
-        for (int x = lane; x < splits; x += kWave) M = fmaxf(M, c.part_ml[2 * (first + x * step)]);
-        M = wave_max(M);
-        const float ref = M == -INFINITY ? 0.0f : M;
-        float o[D] = {}, L = 0.0f;
-        for (int x = wave; x < splits; x += kAWaves) {
-            const float2 e = *reinterpret_cast<const float2 *>(c.part_ml + 2 * (first + x * step));
-            const float w = __builtin_amdgcn_exp2f((e.x - ref) * a.scale);
-            L += w * e.y;
-            const float *p = c.part + (first + x * step) * HD + lane * D;
-            if (HD >= kWave || lane < HD) {
+// per (row, query head); its waves take the splits in turn, eight a step, all requested before their weights are known.
+template <int HD, int V>
+__global__ __launch_bounds__(kMergeWaves *kWave) void kv4_merge_kernel(Kv4Dev c, Kv4AttnArgs a) {
+    constexpr int D = HD >= kWave ? HD / kWave : 1, W = 16 << V, B = 8;  // dims per lane
+    __shared__ float ox[kMergeWaves][HD];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int G = c.nq / c.nkv;
+    const int row = (int)(blockIdx.x / (unsigned)c.nq), head = (int)(blockIdx.x % (unsigned)c.nq);
+    const Kv4Unit s = find_unit<V>(c.seqs, row, true, lane);
+    const int splits = s.splits;
+    if (row - s.row0 >= s.rows || splits <= 1) return;  // uniform over the workgroup
+    const int col = (row - s.row0) * G + head % G, tiles = (s.rows * G + W - 1) / W;
+    const int64_t first = ((int64_t)(s.part + (tiles - 1 - col / W) * splits) * c.nkv + head / G) * W + col % W;
+    const int64_t step = (int64_t)c.nkv * W;
+    const int dim = HD >= kWave ? lane * D : lane % HD;
+    float M = -INFINITY, L = 0.0f, o[D] = {};
+    for (int base = 0; base < splits; base += kMergeWaves * B) {
+        float p[B][D];
+        float2 e[B];
 #pragma unroll
-                for (int d = 0; d < D; d++) o[d] += w * p[d];
-            }
+        for (int j = 0; j < B; j++) {
+            const int64_t at = first + min(base + wave + kMergeWaves * j, splits - 1) * step;
+            e[j] = *reinterpret_cast<const float2 *>(c.part_ml + 2 * at);
+            __builtin_memcpy(p[j], __builtin_assume_aligned(c.part + at * HD + dim, 4 * D < 16 ? 4 * D : 16), sizeof p[j]);
         }
-        if (HD >= kWave || lane < HD) {
+        float up = M;
 #pragma unroll
-            for (int d = 0; d < D; d++) ox[wave][lane * D + d] = o[d];
+        for (int j = 0; j < B; j++) up = fmaxf(up, e[j].x);  // (the last one again where there are fewer)
+        const float ref = up == -INFINITY ? 0.0f : up, al = __builtin_amdgcn_exp2f((M - ref) * a.scale);
+        L *= al;
+#pragma unroll
+        for (int d = 0; d < D; d++) o[d] *= al;
+#pragma unroll
+        for (int j = 0; j < B; j++) {
+            if (base + wave + kMergeWaves * j >= splits) break;
+            const float w = __builtin_amdgcn_exp2f((e[j].x - ref) * a.scale);
+            L += w * e[j].y;
+#pragma unroll
+            for (int d = 0; d < D; d++) o[d] += w * p[j][d];
         }
-        if (lane == 0) lx[wave] = L;
-        __syncthreads();
-        for (int d = threadIdx.x; d < HD; d += kAWaves * kWave)
-            a.out[(int64_t)row * a.out_stride + head * HD + d] =
-                (h16)(((ox[0][d] + ox[1][d]) + (ox[2][d] + ox[3][d])) / ((lx[0] + lx[1]) + (lx[2] + lx[3])));
-        __syncthreads();
+        M = up;
+    }
+    __shared__ float mx[kMergeWaves], lx[kMergeWaves];
+    if (HD >= kWave || lane < HD) {
+#pragma unroll
+        for (int d = 0; d < D; d++) ox[wave][dim + d] = o[d];
+    }
+    if (lane == 0) {
+        mx[wave] = M;
+        lx[wave] = L;
+    }
+    __syncthreads();
+    float up = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kMergeWaves; w++) up = fmaxf(up, mx[w]);
+    const float ref = up == -INFINITY ? 0.0f : up;
+    for (int d = threadIdx.x; d < HD; d += kMergeWaves * kWave) {
+        float x = 0.0f, l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kMergeWaves; w++) {
+            const float z = __builtin_amdgcn_exp2f((mx[w] - ref) * a.scale);
+            x += z * ox[w][d];
+            l += z * lx[w];
+        }
+        a.out[(int64_t)row * a.out_stride + head * HD + d] = (h16)(x / l);
     }
 }
 
-template <int HD>
-int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, int v, int64_t items, bool merge, int64_t rows) {
-    const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>(items * c.nkv, 1), 1 << 20)), block(kAWaves * kWave);
-    if (v == 0)
-        hipLaunchKernelGGL((kv4_attention_kernel<HD, 1>), grid, block, 0, st, c, a);
-    else if (v == 1)
-        hipLaunchKernelGGL((kv4_attention_kernel<HD, 2>), grid, block, 0, st, c, a);
-    else if constexpr (HD < 256)
-        hipLaunchKernelGGL((kv4_attention_kernel<HD, 4>), grid, block, 0, st, c, a);
+template <int HD, int V>
+int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, int64_t units, bool merge) {
+    const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>(units * c.nkv, 1), 1 << 30));
+    // few units: eight waves each, so that a CU's one or two have enough loads in flight
+    if (V < 2 && units * c.nkv <= kFewUnits)
+        hipLaunchKernelGGL((kv4_attention_kernel<HD, 1 << V, V < 2 ? 8 : 4>), grid, dim3((V < 2 ? 8 : 4) * kWave), 0, st, c, a);
+    else
+        hipLaunchKernelGGL((kv4_attention_kernel<HD, 1 << V, 4>), grid, dim3(4 * kWave), 0, st, c, a);
     AESIR_LAUNCH_CHECK("kv4_attention_kernel");
     if (!merge) return AESIR_OK;
-    hipLaunchKernelGGL(kv4_merge_kernel<HD>, dim3((unsigned)std::min<int64_t>(rows * c.nq, 1 << 20)), block, 0, st, c, a, v);
+    hipLaunchKernelGGL((kv4_merge_kernel<HD, V>), dim3((unsigned)(a.rows * c.nq)), dim3(kMergeWaves * kWave), 0, st, c, a);
     AESIR_LAUNCH_CHECK("kv4_merge_kernel");
     return AESIR_OK;
+}
+
+template <int HD>
+int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, int v, int64_t units, bool merge) {
+    if (v == 0) return launch_attention<HD, 0>(st, c, a, units, merge);
+    if (HD == 256 || v == 1) return launch_attention<HD, 1>(st, c, a, units, merge);
+    return launch_attention<HD, HD == 256 ? 1 : 2>(st, c, a, units, merge);
 }
 
 }  // namespace aesir
@@ -704,17 +777,15 @@ struct aesir_kv4 {
     PageBook book;
     Kv4Dev dev{};
     int32_t *table = nullptr;
-    Kv4Head *head = nullptr;
     Kv4Seq *seqs = nullptr;
-    int32_t *row0 = nullptr;
     Kv4Range *ranges = nullptr;
     PageMove *moves = nullptr;
     char *ring = nullptr;  // pinned staging, handed out front to back
     int64_t ring_at = 0;
     bool batch = false;
     int64_t batch_rows = 0, batch_cols = 0;     // new rows; most columns of one sequence
-    Kv4Head plan{};                             // the batch's descriptor
-    bool plan_splits[kKv4Widths] = {};          // whether any sequence is split, per width
+    int64_t units[kKv4Widths] = {};             // attention's units of a KV head, per column width
+    bool split[kKv4Widths] = {};                // and whether any sequence is split
 
     aesir_kv4(int64_t num_pages, int64_t page_size, int64_t max_seqs) : book(num_pages, page_size, max_seqs) {}
 };
@@ -724,14 +795,14 @@ namespace {
 constexpr int64_t kRingBytes = 1 << 20;
 constexpr int64_t kMaxPages = (int64_t)1 << 30;
 constexpr int64_t kPartCols = 32768;  // columns of split partials
-constexpr int64_t kUnits = 1024;      // workgroups that attention is split for: four on each of 256 CUs
-constexpr int64_t kMinRounds = 8;     // rounds of 32 keys that a split has at least
+constexpr int64_t kUnits = 2304;      // workgroups that attention is split for: nine on each of 256 CUs
+constexpr int64_t kMinRounds = 32;    // rounds of 32 keys that a split has at least
 
 struct Kv4Sizes {
-    int64_t page_bytes, pool, table, seqs, row0, ranges, moves, part, part_ml;
+    int64_t page_bytes, pool, table, seqs, ranges, moves, part, part_ml;
     int64_t total() const {
         int64_t t = 0;
-        for (int64_t b : {pool, table, (int64_t)sizeof(Kv4Head), seqs, row0, ranges, moves, part, part_ml}) t += (b + 255) / 256 * 256;
+        for (int64_t b : {pool, table, seqs, ranges, moves, part, part_ml}) t += (b + 255) / 256 * 256;
         return t + 256;  // the well's own alignment
     }
 };
@@ -754,9 +825,8 @@ int32_t kv4_sizes(int64_t layers, int64_t nq, int64_t nkv, int64_t hd, int64_t m
     z->pool = mul_checked(z->page_bytes, pages);
     if (z->pool < 0 || z->pool > (int64_t)1 << 50) return fail(AESIR_ERR_UNSUPPORTED, "KV4Cache: a dimension is too large");
     z->table = stride * max_seqs * 4;
-    z->seqs = max_seqs * (int64_t)sizeof(Kv4Seq);
-    z->row0 = max_seqs * 4;
-    z->ranges = max_seqs * (int64_t)sizeof(Kv4Range);
+    z->seqs = (max_seqs + kWave) * (int64_t)sizeof(Kv4Seq);
+    z->ranges = (max_seqs + kWave) * (int64_t)sizeof(Kv4Range);
     z->moves = pages * (int64_t)sizeof(PageMove);
     z->part = kPartCols * hd * 4;
     z->part_ml = kPartCols * 8;
@@ -806,35 +876,26 @@ int32_t stage(aesir_kv4 *kv, int64_t bytes, char **out) {
 struct Run {
     void *dst;
     const void *src;
-    int64_t bytes;
+    int64_t bytes, fill;  // bytes of src, then fill bytes of kNone
 };
 
-int32_t launch_upload(aesir_kv4 *kv, const Run *runs, int n_runs, const uint32_t *updates, int64_t n_updates) {
-    int64_t bytes = n_updates * 8;
-    for (int i = 0; i < n_runs; i++) bytes += runs[i].bytes;
-    if (bytes == 0) return AESIR_OK;
+int32_t launch_upload(aesir_kv4 *kv, const Run &run, const uint32_t *updates, int64_t n_updates) {
+    if (run.bytes + run.fill + n_updates == 0) return AESIR_OK;
     char *p = nullptr;
-    AESIR_TRY(stage(kv, bytes, &p));
-    Kv4Upload u{};
-    u.src = (const uint32_t *)p;
-    u.table = kv->table;
-    u.updates = (int32_t)n_updates;
-    for (int i = 0; i < n_runs; i++) {
-        std::memcpy(p, runs[i].src, (size_t)runs[i].bytes);
-        p += runs[i].bytes;
-        u.dst[i] = (uint32_t *)runs[i].dst;
-        u.words[i] = (int32_t)(runs[i].bytes / 4);
-    }
-    if (n_updates) std::memcpy(p, updates, (size_t)n_updates * 8);
-    const int64_t threads = bytes / 4 - n_updates;
+    AESIR_TRY(stage(kv, run.bytes + n_updates * 8, &p));
+    if (run.bytes) std::memcpy(p, run.src, (size_t)run.bytes);
+    if (n_updates) std::memcpy(p + run.bytes, updates, (size_t)n_updates * 8);
+    const Kv4Upload u{(const uint32_t *)p, (uint32_t *)run.dst, (int32_t)(run.bytes / 4), (int32_t)(run.fill / 4), kv->table,
+                      (int32_t)n_updates};
+    const int64_t threads = u.words + u.fill + n_updates;
     const unsigned blocks = (unsigned)std::min<int64_t>(256, (threads + kThreads - 1) / kThreads);
     hipLaunchKernelGGL(kv4_upload_kernel, dim3(blocks), dim3(kThreads), 0, kv->ctx->stream, u);
     AESIR_LAUNCH_CHECK("kv4_upload_kernel");
     return AESIR_OK;
 }
 
-// Brings the device's table rows of the listed sequences up to date, with `runs` in the last launch.
-int32_t upload(aesir_kv4 *kv, const int64_t *seqs, int64_t n, const Run *runs, int n_runs) {
+// Brings the device's table rows of the listed sequences up to date, with `run` in the last launch.
+int32_t upload(aesir_kv4 *kv, const int64_t *seqs, int64_t n, const Run &run) {
     const int64_t most = kRingBytes / 4 / 8;
     std::vector<uint32_t> e;
     for (int64_t i = 0; i < n; i++) {
@@ -843,13 +904,19 @@ int32_t upload(aesir_kv4 *kv, const int64_t *seqs, int64_t n, const Run *runs, i
             e.push_back((uint32_t)(seqs[i] * kv->dev.table_stride + j));
             e.push_back((uint32_t)s.pages[(size_t)j]);
             if ((int64_t)e.size() == 2 * most) {
-                AESIR_TRY(launch_upload(kv, nullptr, 0, e.data(), most));
+                AESIR_TRY(launch_upload(kv, Run{}, e.data(), most));
                 e.clear();
             }
         }
         kv->book.mark_synced(seqs[i]);
     }
-    return launch_upload(kv, runs, n_runs, e.data(), (int64_t)e.size() / 2);
+    return launch_upload(kv, run, e.data(), (int64_t)e.size() / 2);
+}
+
+// n records and, behind them, at least one and up to a multiple of 64 of kNone.
+template <class T>
+Run records(T *dst, const T *src, int64_t n) {
+    return {dst, src, n * (int64_t)sizeof(T), (kWave - n % kWave) * (int64_t)sizeof(T)};
 }
 
 // Uploads the moves and copies the pages.
@@ -858,8 +925,8 @@ int32_t copy_pages(aesir_kv4 *kv, const std::vector<PageMove> &moves) {
     const int64_t most = kRingBytes / 4 / (int64_t)sizeof(PageMove);
     for (int64_t at = 0; at < (int64_t)moves.size(); at += most) {
         const int64_t n = std::min<int64_t>(most, (int64_t)moves.size() - at);
-        const Run r{kv->moves + at, moves.data() + at, n * (int64_t)sizeof(PageMove)};
-        AESIR_TRY(launch_upload(kv, &r, 1, nullptr, 0));
+        const Run r{kv->moves + at, moves.data() + at, n * (int64_t)sizeof(PageMove), 0};
+        AESIR_TRY(launch_upload(kv, r, nullptr, 0));
     }
     if (moves.empty()) return AESIR_OK;
     const int64_t units = (kv->dev.page_bytes + kCopyChunk - 1) / kCopyChunk * (int64_t)moves.size();
@@ -875,9 +942,7 @@ int32_t end_batch(aesir_kv4 *kv) {
     kv->batch = false;
     kv->batch_rows = 0;
     if (!kv->ctx) return AESIR_OK;
-    const Kv4Head none{};
-    const Run r{kv->head, &none, (int64_t)sizeof none};
-    return launch_upload(kv, &r, 1, nullptr, 0);
+    return launch_upload(kv, records<Kv4Seq>(kv->seqs, nullptr, 0), nullptr, 0);
 }
 
 template <class F>
@@ -891,11 +956,12 @@ int32_t guarded(const char *what, F f) {
 
 bool aligned16(const void *p, int64_t cols) { return ((uintptr_t)p & 15) == 0 && cols % 8 == 0; }
 
-unsigned grid_for(int64_t threads) { return (unsigned)std::min<int64_t>(std::max<int64_t>((threads + kThreads - 1) / kThreads, 1), 1 << 20); }
+// Workgroups of the append and read kernels: a thread per 8 dims of a row, whole groups of four rows.
+int64_t threads_for(const aesir_kv4 *kv, int64_t rows) { return ((rows + 3) / 4 * kv->nkv * (kv->hd / 2) + kThreads - 1) / kThreads; }
 
 // Units of attention work for column tiles of width 16 << v: every sequence's rounds cut into equal splits, so
 // that the batch gives about kUnits workgroups with kMinRounds rounds or more, and the partials fit.
-void plan_width(const aesir_kv4 *kv, int v, std::vector<Kv4Seq> &ds, Kv4Head &h, bool *split) {
+int64_t plan_width(const aesir_kv4 *kv, int v, std::vector<Kv4Seq> &ds, bool *split) {
     const int64_t W = 16 << v, G = kv->nq / kv->nkv;
     int64_t work = 0;
     auto tiles = [&](const Kv4Seq &s) { return (s.rows * G + W - 1) / W; };
@@ -906,16 +972,13 @@ void plan_width(const aesir_kv4 *kv, int v, std::vector<Kv4Seq> &ds, Kv4Head &h,
         int64_t items = 0, parts = 0;
         for (Kv4Seq &s : ds) {
             const int64_t n = std::max<int64_t>(1, (rounds(s) + chunk - 1) / chunk);
-            s.splits[v] = (int32_t)n;
-            s.item0[v] = (int32_t)items;
-            s.part0[v] = (int32_t)parts;
+            s.plan[v] = {(int32_t)items, (int32_t)n, (int32_t)parts, 0};
             items += tiles(s) * n;
             if (n > 1) parts += tiles(s) * n;
         }
         if (parts * kv->nkv * W > kPartCols) continue;  // ends: one split needs no partials
-        h.items[v] = (int32_t)items;
         *split = parts > 0;
-        return;
+        return items;
     }
 }
 
@@ -934,19 +997,15 @@ int32_t kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64
                         (long long)kv->max_seq_len);
         total += rows[i];
     }
-    if (total > INT32_MAX / kv->nq) return fail(AESIR_ERR_UNSUPPORTED, "KV4Cache.begin: too many rows");
+    if (total > INT32_MAX / (kv->nq * kv->hd / 8)) return fail(AESIR_ERR_UNSUPPORTED, "KV4Cache.begin: too many rows");
     const int64_t need = kv->book.pages_needed(seqs, rows, n);
     if (need > kv->book.free_pages())
         return fail(AESIR_ERR_EXHAUSTED, "KV4Cache.begin: %lld pages needed, %lld free", (long long)need,
                     (long long)kv->book.free_pages());
     std::vector<PageMove> copies;
     std::vector<Kv4Seq> ds((size_t)n);
-    std::vector<int32_t> row0((size_t)n);
     copies.reserve((size_t)n);
     for (int64_t i = 0; i < n; i++) kv->book.reserve(seqs[i], kv->book.seq(seqs[i]).length + rows[i]);
-    Kv4Head h{};
-    h.n = (int32_t)n;
-    h.total_rows = (int32_t)total;
     int64_t at = 0;
     for (int64_t i = 0; i < n; i++) {
         kv->book.grow(seqs[i], rows[i], copies);
@@ -955,7 +1014,7 @@ int32_t kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64
         s.slot = (int32_t)seqs[i];
         s.length = (int32_t)kv->book.seq(seqs[i]).length;
         s.rows = (int32_t)rows[i];
-        s.row0 = row0[(size_t)i] = (int32_t)at;
+        s.row0 = (int32_t)at;
         at += rows[i];
     }
     kv->batch = true;
@@ -963,12 +1022,8 @@ int32_t kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64
     kv->batch_cols = 0;
     for (int64_t i = 0; i < n; i++) kv->batch_cols = std::max(kv->batch_cols, rows[i] * (kv->nq / kv->nkv));
     if (!kv->ctx) return AESIR_OK;
-    for (int v = 0; v < kKv4Widths; v++) plan_width(kv, v, ds, h, &kv->plan_splits[v]);
-    kv->plan = h;
-    const Run runs[3] = {{kv->head, &h, (int64_t)sizeof h},
-                         {kv->seqs, ds.data(), n * (int64_t)sizeof(Kv4Seq)},
-                         {kv->row0, row0.data(), n * 4}};
-    AESIR_TRY(upload(kv, seqs, n, runs, 3));
+    for (int v = 0; v < kKv4Widths; v++) kv->units[v] = plan_width(kv, v, ds, &kv->split[v]);
+    AESIR_TRY(upload(kv, seqs, n, records(kv->seqs, ds.data(), n)));
     return copy_pages(kv, copies);
 }
 
@@ -1011,10 +1066,10 @@ int32_t aesir_kv4_create(aesir_ctx *ctx, int64_t num_layers, int64_t n_heads, in
             return AESIR_OK;
         }
         const int64_t mark = ctx->well_offset;
-        void *p[9] = {};
-        const int64_t bytes[9] = {z.pool, z.table, (int64_t)sizeof(Kv4Head), z.seqs, z.row0, z.ranges, z.moves, z.part, z.part_ml};
+        void *p[7] = {};
+        const int64_t bytes[7] = {z.pool, z.table, z.seqs, z.ranges, z.moves, z.part, z.part_ml};
         int32_t rc = AESIR_OK;
-        for (int i = 0; i < 9 && rc == AESIR_OK; i++) rc = well_alloc_bytes(ctx, bytes[i], &p[i]);
+        for (int i = 0; i < 7 && rc == AESIR_OK; i++) rc = well_alloc_bytes(ctx, bytes[i], &p[i]);
         if (rc == AESIR_OK && hipHostMalloc((void **)&kv->ring, kRingBytes, hipHostMallocDefault) != hipSuccess)
             rc = fail(AESIR_ERR_HIP, "hipHostMalloc of the cache's staging memory failed");
         if (rc != AESIR_OK) {
@@ -1024,11 +1079,9 @@ int32_t aesir_kv4_create(aesir_ctx *ctx, int64_t num_layers, int64_t n_heads, in
         }
         kv->ctx = ctx;
         kv->table = (int32_t *)p[1];
-        kv->head = (Kv4Head *)p[2];
-        kv->seqs = (Kv4Seq *)p[3];
-        kv->row0 = (int32_t *)p[4];
-        kv->ranges = (Kv4Range *)p[5];
-        kv->moves = (PageMove *)p[6];
+        kv->seqs = (Kv4Seq *)p[2];
+        kv->ranges = (Kv4Range *)p[3];
+        kv->moves = (PageMove *)p[4];
         Kv4Dev &d = kv->dev;
         d.pool = (char *)p[0];
         d.page_bytes = z.page_bytes;
@@ -1039,11 +1092,9 @@ int32_t aesir_kv4_create(aesir_ctx *ctx, int64_t num_layers, int64_t n_heads, in
         d.nq = (int32_t)n_heads;
         d.table = kv->table;
         d.table_stride = (max_seq_len + page_size - 1) / page_size;
-        d.head = kv->head;
         d.seqs = kv->seqs;
-        d.row0 = kv->row0;
-        d.part = (float *)p[7];
-        d.part_ml = (float *)p[8];
+        d.part = (float *)p[5];
+        d.part_ml = (float *)p[6];
         kv->batch = true;  // clears the descriptor: the well's memory may have been used before
         rc = end_batch(kv);
         if (rc != AESIR_OK) {
@@ -1103,7 +1154,7 @@ int32_t aesir_kv4_append(aesir_kv4 *kv, int64_t layer, const void *key, int64_t 
         return fail(AESIR_ERR_SHAPE, "KV4Cache.append: key/val rows narrower than kv_heads * head_dim");
     if (!key || !val) return fail(AESIR_ERR_INVALID, "KV4Cache.append: null tensor pointer");
     const Kv4AppendArgs a{(const h16 *)key, (const h16 *)val, key_cols, val_cols, layer, (int32_t)key_rows};
-    const dim3 grid(grid_for((key_rows + 3) / 4 * kv->nkv * (kv->hd / 2)));
+    const dim3 grid((unsigned)threads_for(kv, key_rows));
     if (aligned16(key, key_cols) && aligned16(val, val_cols))
         hipLaunchKernelGGL(kv4_append_kernel<true>, grid, dim3(kThreads), 0, kv->ctx->stream, kv->dev, a);
     else
@@ -1131,12 +1182,12 @@ int32_t aesir_kv4_attention(aesir_kv4 *kv, int64_t layer, const void *query, int
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     AESIR_HIP_TRY(hipStreamIsCapturing(kv->ctx->stream, &st));
     // a captured call may meet a batch that is split, whatever this one is
-    const bool merge = kv->plan_splits[v] || st != hipStreamCaptureStatusNone;
+    const bool merge = kv->split[v] || st != hipStreamCaptureStatusNone;
     switch (kv->hd) {
-        case 32: return launch_attention<32>(kv->ctx->stream, kv->dev, a, v, kv->plan.items[v], merge, query_rows);
-        case 64: return launch_attention<64>(kv->ctx->stream, kv->dev, a, v, kv->plan.items[v], merge, query_rows);
-        case 128: return launch_attention<128>(kv->ctx->stream, kv->dev, a, v, kv->plan.items[v], merge, query_rows);
-        default: return launch_attention<256>(kv->ctx->stream, kv->dev, a, v, kv->plan.items[v], merge, query_rows);
+        case 32: return launch_attention<32>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge);
+        case 64: return launch_attention<64>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge);
+        case 128: return launch_attention<128>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge);
+        default: return launch_attention<256>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge);
     }
 }
 
@@ -1154,7 +1205,7 @@ int32_t aesir_kv4_read(aesir_kv4 *kv, int64_t layer, int64_t layers, const int64
             return fail(AESIR_ERR_INVALID, "KV4Cache.read: range [%lld, +%lld) outside sequence %lld of %lld positions",
                         (long long)pos[i], (long long)rows[i], (long long)seqs[i], (long long)len);
         total += rows[i];
-        if (total > INT32_MAX) return fail(AESIR_ERR_UNSUPPORTED, "KV4Cache.read: too many rows");
+        if (total > INT32_MAX / (kv->nkv * kv->hd / 8)) return fail(AESIR_ERR_UNSUPPORTED, "KV4Cache.read: too many rows");
     }
     if (key_rows != total * layers || val_rows != total * layers)
         return fail(AESIR_ERR_SHAPE, "KV4Cache.read: %lld rows are asked for", (long long)(total * layers));
@@ -1175,11 +1226,10 @@ int32_t aesir_kv4_read(aesir_kv4 *kv, int64_t layer, int64_t layers, const int64
                 count += rows[i];
             }
             if (count == 0) continue;
-            const Run run{kv->ranges, r.data(), m * (int64_t)sizeof(Kv4Range)};
-            AESIR_TRY(upload(kv, seqs + at, m, &run, 1));
+            AESIR_TRY(upload(kv, seqs + at, m, records(kv->ranges, r.data(), m)));
             const Kv4ReadArgs a{(h16 *)key, (h16 *)val, key_cols,     val_cols,       layer,         layers,
-                                kv->ranges, (int32_t)m, (int32_t)count, (int32_t)total, (int32_t)first};
-            const dim3 grid(grid_for((count + 3) / 4 * kv->nkv * (kv->hd / 2) * layers));
+                                kv->ranges, (int32_t)total, (int32_t)first};
+            const dim3 grid((unsigned)threads_for(kv, count), (unsigned)std::min<int64_t>(layers, 65535));
             if (vec)
                 hipLaunchKernelGGL(kv4_read_kernel<true>, grid, dim3(kThreads), 0, kv->ctx->stream, kv->dev, a);
             else

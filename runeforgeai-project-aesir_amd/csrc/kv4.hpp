@@ -23,20 +23,17 @@ constexpr int kKv4Group = 32;  // dims per scale
 // every launch reads the plan of its own width, so a captured launch stays right for any later batch.
 constexpr int kKv4Widths = 3;
 
-struct Kv4Head {  // the batch (64 bytes)
-    int32_t n, total_rows;
-    int32_t items[kKv4Widths];  // (sequence, column tile, split) units of each width
-    int32_t pad[11];
-};
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kNone = 0x7FFFFFFF;  // in every field of the records behind the last one
 
 struct Kv4Seq {  // one sequence of the batch (64 bytes)
     int32_t slot, length, rows, row0;  // length counts the new rows
-    int32_t item0[kKv4Widths];         // first unit
-    int32_t splits[kKv4Widths];        // splits of every column tile
-    int32_t part0[kKv4Widths];         // first partial slot (splits > 1)
-    int32_t pad[3];
+    struct {
+        int32_t unit0, splits, part0, pad;  // first (column tile, split) unit, splits of each tile, first partial slot
+    } plan[kKv4Widths];
 };
-static_assert(sizeof(Kv4Head) == 64 && sizeof(Kv4Seq) == 64, "descriptor");
+static_assert(sizeof(Kv4Seq) == 64, "descriptor");
 
 struct Kv4Range {  // rows to read back: positions pos .. pos + rows - 1 of a sequence, to output rows row0 ..
     int32_t slot, pos, rows, row0;
@@ -48,9 +45,7 @@ struct Kv4Dev {
     int32_t page_shift, hd, nkv, nq;
     const int32_t *table;  // [max_seqs][table_stride] page ids
     int64_t table_stride;
-    const Kv4Head *head;
-    const Kv4Seq *seqs;
-    const int32_t *row0;  // [max_seqs] first rows of the batch's sequences, or of the ranges
+    const Kv4Seq *seqs;    // in row order, ended by records of kNone
     float *part, *part_ml;  // split partials of a column: accumulators [hd], and (maximum, sum)
 
     __host__ __device__ int page_size() const { return 1 << page_shift; }
