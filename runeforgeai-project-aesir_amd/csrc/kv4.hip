@@ -295,6 +295,7 @@ struct Kv4AttnArgs {
     int64_t layer;
     int32_t rows;  // rows of q and out
     int32_t vec;   // q and out rows 16-byte aligned
+    int32_t only;  // leave out sequences of other column classes (they have launches of their own)
     float scale;   // log2(e) / sqrt(hd)
 };
 
@@ -349,35 +350,92 @@ struct Kv4Round {  // one lane's share of 32 keys
 
     // b: the block (uniform), s0: the round's first position in its page
     __device__ __forceinline__ void load(const char *b, int s0, const Kv4Lane<HD> &o, int m_off) {
-        const char *rows = b + s0 * (HD / 2), *scales = b + s0 * NJ * 4, *vscales = b + s0 * 2;
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const char *p = rows + (size_t)(o.k + t * 2 * HD);
-            if constexpr (NJ == 1) {
-                k[t][0] = *reinterpret_cast<const unsigned *>(p);
-            } else if constexpr (NJ == 2) {
-                const u32x2 x = *reinterpret_cast<const u32x2 *>(p);
-                k[t][0] = x.x;
-                k[t][1] = x.y;
-            } else {
+        for (int t = 0; t < 2; t++) load_k(b, s0, o, t);
 #pragma unroll
-                for (int j = 0; j < NJ; j += 4) {
-                    const u32x4 x = ld16(p + 4 * j);
+        for (int x = 0; x < NB; x++) load_v(b, s0, o, m_off, x);
+    }
+    __device__ __forceinline__ void load_k(const char *b, int s0, const Kv4Lane<HD> &o, int t) {  // 16 keys
+        const char *p = b + s0 * (HD / 2) + (size_t)(o.k + t * 2 * HD);
+        if constexpr (NJ == 1) {
+            k[t][0] = *reinterpret_cast<const unsigned *>(p);
+        } else if constexpr (NJ == 2) {
+            const u32x2 x = *reinterpret_cast<const u32x2 *>(p);
+            k[t][0] = x.x;
+            k[t][1] = x.y;
+        } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) k[t][j + e] = x[e];
-                }
+            for (int j = 0; j < NJ; j += 4) {
+                const u32x4 x = ld16(p + 4 * j);
+#pragma unroll
+                for (int e = 0; e < 4; e++) k[t][j + e] = x[e];
             }
-            const h16x2 *ps = reinterpret_cast<const h16x2 *>(scales + (size_t)(o.ks + t * 16 * NJ));
-#pragma unroll
-            for (int x = 0; x < NG; x++) ks[t][x] = ps[x];
         }
+        const h16x2 *ps = reinterpret_cast<const h16x2 *>(b + s0 * NJ * 4 + (size_t)(o.ks + t * 16 * NJ));
 #pragma unroll
-        for (int x = 0; x < NB; x++) {
+        for (int x = 0; x < NG; x++) ks[t][x] = ps[x];
+    }
+    __device__ __forceinline__ void load_v(const char *b, int s0, const Kv4Lane<HD> &o, int m_off, int x) {  // 16 8-dim blocks
+        const char *rows = b + s0 * (HD / 2), *scales = b + s0 * 2;
 #pragma unroll
-            for (int h = 0; h < 2; h++) v[x][h] = ld16(rows + (size_t)(o.v[x] + h * 2 * HD));
-            vd[x] = ld16(vscales + (size_t)o.vs[x]);
-            vm[x] = ld16(vscales + m_off + (size_t)o.vs[x]);
+        for (int h = 0; h < 2; h++) v[x][h] = ld16(rows + (size_t)(o.v[x] + h * 2 * HD));
+        vd[x] = ld16(scales + (size_t)o.vs[x]);
+        vm[x] = ld16(scales + m_off + (size_t)o.vs[x]);
+    }
+
+    // The A operand of key tile t's dims 8 j .. of the lane's share.
+    __device__ __forceinline__ u32x4 key_operand(const Kv4Magic &c, int t, int j) const {
+        const h16x2 d = both(ks[t][j * NG / NJ].x), m = both(ks[t][j * NG / NJ].y);
+        return {h2_bits(kv4_values<0>(c, k[t][j], d, m)), h2_bits(kv4_values<1>(c, k[t][j], d, m)),
+                h2_bits(kv4_values<2>(c, k[t][j], d, m)), h2_bits(kv4_values<3>(c, k[t][j], d, m))};
+    }
+
+    // Zeroes the values of keys k0 + e >= keys and of NaN groups among the others; bit e of the result: key k0 + e's
+    // group of value block x is NaN.
+    __device__ __forceinline__ unsigned hide(int x, int k0, int keys) {
+        unsigned bad = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const unsigned half = 0xFFFFu << (16 * (e % 2));
+            const bool nan = ((vm[x][e / 2] >> (16 * (e % 2))) & 0x7FFFu) > 0x7C00u, hidden = k0 + e >= keys;
+            if (nan || hidden) {
+                vd[x][e / 2] &= ~half;
+                vm[x][e / 2] &= ~half;
+            }
+            if (nan && !hidden) bad |= 1u << e;
         }
+        return bad;
+    }
+
+    // f(p, half, A operand) for every accumulator of value block x: eight positions of one dim each.
+    template <class F>
+    __device__ __forceinline__ void value_operands(const Kv4Magic &c, int x, int i, F f) const {
+        constexpr int NP = NJ < 4 ? NJ : 4;
+        const int shift = NJ < 4 ? 4 * NJ * (i / (4 * NJ)) : 0;
+        unsigned lo[4], hi[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {  // positions 2 e, 2 e + 1: low halves (even dims) and high halves
+            const unsigned w0 = v[x][e / 2][2 * (e % 2)] >> shift, w1 = v[x][e / 2][2 * (e % 2) + 1] >> shift;
+            lo[e] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+            hi[e] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+        }
+        auto step = [&](auto pc) {
+            constexpr int P = decltype(pc)::value;
+            if constexpr (P < NP) {
+                u32x4 a, b;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    a[e] = h2_bits(kv4_values<P>(c, lo[e], as_h2(vd[x][e]), as_h2(vm[x][e])));
+                    b[e] = h2_bits(kv4_values<P>(c, hi[e], as_h2(vd[x][e]), as_h2(vm[x][e])));
+                }
+                f(P, 0, a);
+                f(P, 1, b);
+            }
+        };
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+        step(std::integral_constant<int, 2>{});
+        step(std::integral_constant<int, 3>{});
     }
 };
 
@@ -410,6 +468,115 @@ __device__ __forceinline__ Kv4Unit find_unit(const Kv4Seq *seqs, int unit, bool 
     return r;
 }
 
+// Two f16 per dword, 1 where bit 2 e (2 e + 1) of `bits` is set, as an operand of eight positions.
+__device__ __forceinline__ u32x4 ones_operand(unsigned bits) {
+    u32x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; e++) r[e] = (bits >> (2 * e) & 1 ? 0x3C00u : 0u) | (bits >> (2 * e + 1) & 1 ? 0x3C000000u : 0u);
+    return r;
+}
+
+// One wave's columns: 16 NC of them, column i of each 16 in lanes i, i + 16, ..
+template <int HD, int NC>
+struct Kv4Cols {
+    static constexpr int NJ = HD / 32, NP = NJ < 4 ? NJ : 4, NB = NJ == 8 ? 2 : 1;
+    u32x4 q[NC][NJ];  // dims g HD / 4 + 8 j .. of the column's query
+    int limit[NC];    // last position the column sees, -1 for none
+    f32x4 acc[NC][NB][NP][2];
+    float m[NC], l[NC];  // running maximum (the column's), sum (the lane's share, times 2^15 as acc)
+
+    __device__ __forceinline__ void start(const Kv4AttnArgs &a, const Kv4Unit &s, int first, int G, int kvh, int i, int g) {
+#pragma unroll
+        for (int t = 0; t < NC; t++) {
+            const int col = first + 16 * t + i, row = col / G;
+            const bool live = col < s.rows * G && s.row0 + row < a.rows;
+            limit[t] = live ? s.length - s.rows + row : -1;
+            const h16 *p = a.q + (int64_t)(s.row0 + row) * a.q_stride + (kvh * G + col % G) * HD + g * (HD / 4);
+#pragma unroll
+            for (int j = 0; j < NJ; j++) q[t][j] = !live ? u32x4{0, 0, 0, 0} : a.vec ? ld16(p + 8 * j) : load8<false>(p + 8 * j);
+            m[t] = -INFINITY;
+            l[t] = 0.0f;
+#pragma unroll
+            for (int x = 0; x < NB; x++)
+#pragma unroll
+                for (int p = 0; p < NP; p++) acc[t][x][p][0] = acc[t][x][p][1] = f32x4{0, 0, 0, 0};
+        }
+    }
+
+    // Scores of keys k0 .. k0 + 7 (key 4 t + e in sc[t][.][e]) that a column does not see.
+    __device__ __forceinline__ void mask(f32x4 (&sc)[2][NC], int k0) const {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int x = 0; x < NC; x++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (k0 + 4 * t + e > limit[x]) sc[t][x][e] = -INFINITY;
+    }
+
+    // The round's softmax step; the probabilities as P V's B operand.
+    __device__ __forceinline__ void softmax(const f32x4 (&sc)[2][NC], float scale, u32x4 (&pb)[NC]) {
+#pragma unroll
+        for (int x = 0; x < NC; x++) {
+            float mx = fmaxf(fmaxf(fmaxf(sc[0][x][0], sc[0][x][1]), fmaxf(sc[0][x][2], sc[0][x][3])),
+                             fmaxf(fmaxf(sc[1][x][0], sc[1][x][1]), fmaxf(sc[1][x][2], sc[1][x][3])));
+            mx = swap_pair_max<32>(swap_pair_max<16>(mx));
+            if (__any(mx > m[x])) {
+                const float up = fmaxf(m[x], mx), ref = up == -INFINITY ? 0.0f : up;
+                const float al = __builtin_amdgcn_exp2f((m[x] - ref) * scale);
+                l[x] *= al;
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int p = 0; p < NP; p++) {
+                        acc[x][b][p][0] *= al;
+                        acc[x][b][p][1] *= al;
+                    }
+                m[x] = up;
+            }
+            const float ref = m[x] == -INFINITY ? 0.0f : m[x];
+            float pr[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                pr[e] = __builtin_amdgcn_exp2f(fmaf(sc[e / 4][x][e % 4] - ref, scale, 15.0f));
+                l[x] += pr[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) pb[x][e] = h2_bits(h16x2{(h16)pr[2 * e], (h16)pr[2 * e + 1]});
+        }
+    }
+
+    // NaN for the columns that see a NaN group of value block b, in its dims; bad: the operand of ones at such positions.
+    __device__ __forceinline__ void spread_nan(int b, u32x4 bad, int k0) {
+#pragma unroll
+        for (int x = 0; x < NC; x++) {
+            const int n = min(max(limit[x] - k0 + 1, 0), 8);  // positions the column sees
+            const f32x4 seen = mfma16x16x32(bad, ones_operand((1u << n) - 1), f32x4{0, 0, 0, 0});
+#pragma unroll
+            for (int p = 0; p < NP; p++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (seen[e] > 0.0f) acc[x][b][p][0][e] = acc[x][b][p][1][e] = NAN;
+        }
+    }
+
+    __device__ __forceinline__ void sum_lanes() {
+#pragma unroll
+        for (int t = 0; t < NC; t++) {
+            l[t] = swap_pair_sum<16>(l[t], l[t]);
+            l[t] = swap_pair_sum<32>(l[t], l[t]);
+        }
+    }
+};
+
+// The column tile width of a launch for sequences of many or few columns ((row, query head of a group) pairs), and which
+// one a sequence takes: the narrowest that holds its columns, up to 64; more go to the kernel that shares unpacked keys
+// among eight waves of columns (256 wide, 128 at head_dim 256, where 64 would not fit the registers).
+__host__ __device__ constexpr int kv4_width(int v, int hd) { return v < 3 ? 16 << v : hd == 256 ? 128 : 256; }
+__host__ __device__ constexpr int kv4_class(int64_t cols, int hd) {
+    return cols <= 16 ? 0 : cols <= 32 ? 1 : cols <= 64 && hd < 256 ? 2 : 3;
+}
+
 // The dim of accumulator (x, p, half) in matrix row r.
 template <int HD>
 __device__ __forceinline__ int out_dim(int r, int x, int p, int half) {
@@ -421,7 +588,7 @@ __device__ __forceinline__ int out_dim(int r, int x, int p, int half) {
 template <int HD, int NC, int NW>
 __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1) void kv4_attention_kernel(Kv4Dev c, Kv4AttnArgs a) {
     constexpr int V = NC == 1 ? 0 : NC == 2 ? 1 : 2, W = 16 * NC;
-    constexpr int NJ = HD / 32, NP = NJ < 4 ? NJ : 4, NB = Kv4Round<HD>::NB, NG = Kv4Round<HD>::NG;
+    constexpr int NJ = HD / 32, NP = NJ < 4 ? NJ : 4, NB = Kv4Round<HD>::NB;
     constexpr int LD = HD + 4;  // LDS row of a column
     __shared__ float ml[NW][W][2];
     __shared__ __align__(16) float ox[NW][16][LD];
@@ -436,6 +603,7 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
         const Kv4Unit s = find_unit<V>(c.seqs, unit, false, lane);
         const int splits = s.splits, cols = s.rows * G, tiles = (cols + W - 1) / W;
         if (s.local >= tiles * splits) break;  // past the last unit (no batch: the first)
+        if (a.only && kv4_class(cols, HD) != V) continue;
         const int tile = tiles - 1 - s.local / splits, split = s.local % splits;
         const int before = s.length - s.rows;
         const int low = before + tile * W / G;                                    // last position of the first column
@@ -447,30 +615,8 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
         const int32_t *table = c.table + (int64_t)s.slot * c.table_stride;
         auto page_ids = [&](int r) { return table[min(r + lane * NW, rounds - 1) * kKeys >> c.page_shift]; };
         int pages = page_ids(r0);
-
-        // queries: column i of each 16, dims g HD / 4 + 8 j ..
-        u32x4 q[NC][NJ];
-        int limit[NC];
-#pragma unroll
-        for (int t = 0; t < NC; t++) {
-            const int col = tile * W + 16 * t + i, row = col / G;
-            const bool live = col < cols && s.row0 + row < a.rows;
-            limit[t] = live ? before + row : -1;
-            const h16 *p = a.q + (int64_t)(s.row0 + row) * a.q_stride + (kvh * G + col % G) * HD + g * (HD / 4);
-#pragma unroll
-            for (int j = 0; j < NJ; j++) q[t][j] = !live ? u32x4{0, 0, 0, 0} : a.vec ? ld16(p + 8 * j) : load8<false>(p + 8 * j);
-        }
-        f32x4 acc[NC][NB][NP][2];
-        float m[NC], l[NC];
-#pragma unroll
-        for (int t = 0; t < NC; t++) {
-            m[t] = -INFINITY;
-            l[t] = 0.0f;
-#pragma unroll
-            for (int x = 0; x < NB; x++)
-#pragma unroll
-                for (int p = 0; p < NP; p++) acc[t][x][p][0] = acc[t][x][p][1] = f32x4{0, 0, 0, 0};
-        }
+        Kv4Cols<HD, NC> own;
+        own.start(a, s, tile * W, G, kvh, i, g);
 
         const char *head_base = c.pool + a.layer * c.layer_bytes + kvh * c.head_bytes();
         auto fetch = [&](int x, Kv4Round<HD> &d) {  // the wave's x-th round
@@ -485,115 +631,28 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
                 for (int x = 0; x < NC; x++) sc[t][x] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int j = 0; j < NJ; j++) {
-                    const h16x2 dd = both(d.ks[t][j * NG / NJ].x), mm = both(d.ks[t][j * NG / NJ].y);
-                    const unsigned w = d.k[t][j];
-                    const u32x4 ka = {h2_bits(kv4_values<0>(magic, w, dd, mm)), h2_bits(kv4_values<1>(magic, w, dd, mm)),
-                                      h2_bits(kv4_values<2>(magic, w, dd, mm)), h2_bits(kv4_values<3>(magic, w, dd, mm))};
+                    const u32x4 ka = d.key_operand(magic, t, j);
 #pragma unroll
-                    for (int x = 0; x < NC; x++) sc[t][x] = mfma16x16x32(ka, q[x][j], sc[t][x]);
+                    for (int x = 0; x < NC; x++) sc[t][x] = mfma16x16x32(ka, own.q[x][j], sc[t][x]);
                 }
             }
             const bool whole = r * kKeys + kKeys - 1 <= low;  // every column sees every key (uniform)
             const int k0 = r * kKeys + 8 * g;
-            unsigned bad[NB] = {};  // bit e: the value group of key k0 + e is NaN
+            unsigned bad[NB] = {};
             if (!whole) {
+                own.mask(sc, k0);
 #pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int x = 0; x < NC; x++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (k0 + 4 * t + e > limit[x]) sc[t][x][e] = -INFINITY;
-#pragma unroll
-                for (int x = 0; x < NB; x++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const unsigned half = 0xFFFFu << (16 * (e % 2));
-                        const bool nan = ((d.vm[x][e / 2] >> (16 * (e % 2))) & 0x7FFFu) > 0x7C00u, hidden = k0 + e >= keys;
-                        if (nan || hidden) {
-                            d.vd[x][e / 2] &= ~half;
-                            d.vm[x][e / 2] &= ~half;
-                        }
-                        if (nan && !hidden) bad[x] |= 1u << e;
-                    }
+                for (int x = 0; x < NB; x++) bad[x] = d.hide(x, k0, keys);
             }
             u32x4 pb[NC];
-#pragma unroll
-            for (int x = 0; x < NC; x++) {
-                float mx = fmaxf(fmaxf(fmaxf(sc[0][x][0], sc[0][x][1]), fmaxf(sc[0][x][2], sc[0][x][3])),
-                                 fmaxf(fmaxf(sc[1][x][0], sc[1][x][1]), fmaxf(sc[1][x][2], sc[1][x][3])));
-                mx = swap_pair_max<32>(swap_pair_max<16>(mx));
-                if (__any(mx > m[x])) {
-                    const float up = fmaxf(m[x], mx), ref = up == -INFINITY ? 0.0f : up;
-                    const float al = __builtin_amdgcn_exp2f((m[x] - ref) * a.scale);
-                    l[x] *= al;
-#pragma unroll
-                    for (int b = 0; b < NB; b++)
-#pragma unroll
-                        for (int p = 0; p < NP; p++) {
-                            acc[x][b][p][0] *= al;
-                            acc[x][b][p][1] *= al;
-                        }
-                    m[x] = up;
-                }
-                const float ref = m[x] == -INFINITY ? 0.0f : m[x];
-                float pr[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    pr[e] = __builtin_amdgcn_exp2f(fmaf(sc[e / 4][x][e % 4] - ref, a.scale, 15.0f));
-                    l[x] += pr[e];
-                }
-#pragma unroll
-                for (int e = 0; e < 4; e++) pb[x][e] = h2_bits(h16x2{(h16)pr[2 * e], (h16)pr[2 * e + 1]});
-            }
+            own.softmax(sc, a.scale, pb);
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                const int shift = NJ < 4 ? 4 * NJ * (i / (4 * NJ)) : 0;
-                unsigned lo[4], hi[4];
+                d.value_operands(magic, b, i, [&](int p, int half, u32x4 va) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) {  // positions 2 e, 2 e + 1: low halves (even dims) and high halves
-                    const unsigned w0 = d.v[b][e / 2][2 * (e % 2)] >> shift, w1 = d.v[b][e / 2][2 * (e % 2) + 1] >> shift;
-                    lo[e] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
-                    hi[e] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
-                }
-                auto step = [&](auto pc) {
-                    constexpr int P = decltype(pc)::value;
-                    if constexpr (P < NP) {
-                        u32x4 va, vb;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            va[e] = h2_bits(kv4_values<P>(magic, lo[e], as_h2(d.vd[b][e]), as_h2(d.vm[b][e])));
-                            vb[e] = h2_bits(kv4_values<P>(magic, hi[e], as_h2(d.vd[b][e]), as_h2(d.vm[b][e])));
-                        }
-#pragma unroll
-                        for (int x = 0; x < NC; x++) {
-                            acc[x][b][P][0] = mfma16x16x32(va, pb[x], acc[x][b][P][0]);
-                            acc[x][b][P][1] = mfma16x16x32(vb, pb[x], acc[x][b][P][1]);
-                        }
-                    }
-                };
-                step(std::integral_constant<int, 0>{});
-                step(std::integral_constant<int, 1>{});
-                step(std::integral_constant<int, 2>{});
-                step(std::integral_constant<int, 3>{});
-                if (!whole && __any(bad[b] != 0)) {  // NaN for the columns that see a NaN group, in its dims
-                    u32x4 ia;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) ia[e] = (bad[b] >> (2 * e) & 1 ? 0x3C00u : 0u) | (bad[b] >> (2 * e + 1) & 1 ? 0x3C000000u : 0u);
-#pragma unroll
-                    for (int x = 0; x < NC; x++) {
-                        u32x4 ib;
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            ib[e] = (k0 + 2 * e <= limit[x] ? 0x3C00u : 0u) | (k0 + 2 * e + 1 <= limit[x] ? 0x3C000000u : 0u);
-                        const f32x4 seen = mfma16x16x32(ia, ib, f32x4{0, 0, 0, 0});
-#pragma unroll
-                        for (int p = 0; p < NP; p++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                if (seen[e] > 0.0f) acc[x][b][p][0][e] = acc[x][b][p][1][e] = NAN;
-                    }
-                }
+                    for (int x = 0; x < NC; x++) own.acc[x][b][p][half] = mfma16x16x32(va, pb[x], own.acc[x][b][p][half]);
+                });
+                if (!whole && __any(bad[b] != 0)) own.spread_nan(b, ones_operand(bad[b]), k0);
             }
         };
         // A round's loads are issued before the round ahead of it is computed. The last round issues its own again (they
@@ -612,13 +671,12 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
         }
 
         // the waves meet: maxima and sums of all columns, then 16 columns of accumulators at a time
+        own.sum_lanes();
 #pragma unroll
         for (int t = 0; t < NC; t++) {
-            l[t] = swap_pair_sum<16>(l[t], l[t]);
-            l[t] = swap_pair_sum<32>(l[t], l[t]);
             if (g == 0) {
-                ml[wave][16 * t + i][0] = m[t];
-                ml[wave][16 * t + i][1] = l[t];
+                ml[wave][16 * t + i][0] = own.m[t];
+                ml[wave][16 * t + i][1] = own.l[t];
             }
         }
         __syncthreads();
@@ -627,7 +685,7 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
             float up = -INFINITY;
 #pragma unroll
             for (int w = 0; w < NW; w++) up = fmaxf(up, ml[w][16 * t + i][0]);
-            const float ref = up == -INFINITY ? 0.0f : up, scale = __builtin_amdgcn_exp2f((m[t] - ref) * a.scale);
+            const float ref = up == -INFINITY ? 0.0f : up, scale = __builtin_amdgcn_exp2f((own.m[t] - ref) * a.scale);
 #pragma unroll
             for (int e = 0; e < 4; e++)
 #pragma unroll
@@ -635,8 +693,8 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
 #pragma unroll
                     for (int p = 0; p < NP; p++) {
                         float *o = &ox[wave][i][out_dim<HD>(4 * g + e, x, p, 0)];
-                        o[0] = acc[t][x][p][0][e] * scale;
-                        o[1] = acc[t][x][p][1][e] * scale;
+                        o[0] = own.acc[t][x][p][0][e] * scale;
+                        o[1] = own.acc[t][x][p][1][e] * scale;
                     }
             __syncthreads();
             // thread: D dims of one column
@@ -674,11 +732,184 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
     }
 }
 
+// Prompts: units of 256 columns (128 at head_dim 256), eight waves with 32 (16) of them each. The waves unpack RS rounds of keys
+// and values between them, each operand once, into LDS in the order in which the matrix instructions take them (1 KB an
+// operand, 16 bytes a lane, no bank conflicts); every wave then runs those rounds over its own columns, so unpacking costs
+// an eighth a column and the waves never meet but at the barrier between stages. Two stages of LDS: the next is loaded
+// during one and unpacked behind it.
+template <int HD>
+__global__ __launch_bounds__(8 * kWave) void kv4_prompt_kernel(Kv4Dev c, Kv4AttnArgs a) {
+    constexpr int V = 3, W = kv4_width(V, HD), NC = W / 128, NJ = HD / 32, NP = NJ < 4 ? NJ : 4, NB = Kv4Round<HD>::NB;
+    constexpr int RS = HD == 256 ? 2 : 4, PARTS = 8 / RS;  // rounds per stage; waves that unpack a round
+    constexpr int NK = 2 * NJ;                             // key operands of a round, and value operands
+    __shared__ __align__(16) u32x4 lds[2][RS][2 * NK][kWave];
+    __shared__ __align__(16) u32x4 bad_at[2][RS][NB][kWave];
+    __shared__ int any_bad[2][RS][NB];
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int G = c.nq / c.nkv;
+    const Kv4Lane<HD> place(c, i, g);
+    const int m_off = c.v_m_off() - c.v_d_off();
+    const Kv4Magic magic;
+    const int mr = wave / PARTS, part = wave % PARTS;  // the round of a stage this wave unpacks, and what of it
+    for (unsigned u = blockIdx.x;; u += gridDim.x) {
+        const int kvh = (int)(u % (unsigned)c.nkv), unit = (int)(u / (unsigned)c.nkv);
+        const Kv4Unit s = find_unit<V>(c.seqs, unit, false, lane);
+        const int splits = s.splits, cols = s.rows * G, tiles = (cols + W - 1) / W;
+        if (s.local >= tiles * splits) break;
+        if (a.only && kv4_class(cols, HD) != V) continue;
+        const int tile = tiles - 1 - s.local / splits, split = s.local % splits;
+        const int before = s.length - s.rows;
+        const int low = before + tile * W / G, keys = before + min(s.rows - 1, (tile * W + W - 1) / G) + 1;
+        const int rounds = (keys + kKeys - 1) / kKeys, per = ((rounds + splits - 1) / splits + RS - 1) / RS * RS;
+        const int r0 = split * per, r1 = min(rounds, r0 + per), stages = r0 < r1 ? (r1 - r0 + RS - 1) / RS : 0;
+        // this wave's columns: the first sees positions up to low_w, all together keys_w (none: 0)
+        const int first = tile * W + wave * 16 * NC;
+        const int low_w = before + first / G;
+        const int keys_w = first < cols ? before + min(s.rows - 1, (first + 16 * NC - 1) / G) + 1 : 0;
+
+        const int32_t *table = c.table + (int64_t)s.slot * c.table_stride;
+        auto page_ids = [&](int st) { return table[min(r0 + (st + lane) * RS + mr, rounds - 1) * kKeys >> c.page_shift]; };
+        int pages = page_ids(0);
+        Kv4Cols<HD, NC> own;
+        own.start(a, s, first, G, kvh, i, g);
+        const char *head_base = c.pool + a.layer * c.layer_bytes + kvh * c.head_bytes();
+
+        Kv4Round<HD> d;
+        auto fetch = [&](int st) {  // (rounds past the last one's page repeat it; their keys are hidden below)
+            if ((st & (kWave - 1)) == 0 && st > 0) pages = page_ids(st);
+            const int page = __builtin_amdgcn_readlane(pages, st & (kWave - 1));
+            const char *b = head_base + page * c.page_bytes;
+            const int s0 = min(r0 + st * RS + mr, rounds - 1) * kKeys & (c.page_size() - 1);
+            if constexpr (PARTS == 2) {
+                if (part == 0) {
+                    d.load_k(b, s0, place, 0);
+                    d.load_k(b, s0, place, 1);
+                } else {
+                    d.load_v(b, s0, place, m_off, 0);
+                }
+            } else {
+                if (part == 0) d.load_k(b, s0, place, 0);
+                if (part == 1) d.load_k(b, s0, place, 1);
+                if (part == 2) d.load_v(b, s0, place, m_off, 0);
+                if (part == 3) d.load_v(b, s0, place, m_off, NB - 1);
+            }
+        };
+        auto unpack = [&](int st) {
+            u32x4(&to)[2 * NK][kWave] = lds[st & 1][mr];
+            const int r = r0 + st * RS + mr;
+            auto key = [&](int t) {
+#pragma unroll
+                for (int j = 0; j < NJ; j++) to[t * NJ + j][lane] = d.key_operand(magic, t, j);
+            };
+            auto value = [&](int x) {
+                if (r * kKeys + kKeys - 1 > low) {  // not seen whole by every column of the tile
+                    const unsigned bad = d.hide(x, r * kKeys + 8 * g, keys);
+                    const bool any = __any(bad != 0);
+                    if (any) bad_at[st & 1][mr][x][lane] = ones_operand(bad);
+                    if (lane == 0) any_bad[st & 1][mr][x] = any;
+                }
+                d.value_operands(magic, x, i, [&](int p, int half, u32x4 v) { to[NK + (x * NP + p) * 2 + half][lane] = v; });
+            };
+            if constexpr (PARTS == 2) {
+                if (part == 0) {
+                    key(0);
+                    key(1);
+                } else {
+                    value(0);
+                }
+            } else {
+                if (part == 0) key(0);
+                if (part == 1) key(1);
+                if (part == 2) value(0);
+                if (part == 3) value(NB - 1);
+            }
+        };
+
+        if (stages > 0) {
+            fetch(0);
+            unpack(0);
+        }
+        for (int st = 0; st < stages; st++) {
+            if (st + 1 < stages) fetch(st + 1);
+            __syncthreads();  // stage st is in LDS, and stage st - 1 is used up
+            for (int x = 0; x < RS; x++) {
+                const int r = r0 + st * RS + x;
+                if (r >= r1 || r * kKeys >= keys_w) break;
+                const u32x4(&from)[2 * NK][kWave] = lds[st & 1][x];
+                f32x4 sc[2][NC];
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+#pragma unroll
+                    for (int y = 0; y < NC; y++) sc[t][y] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) {
+                        const u32x4 ka = from[t * NJ + j][lane];
+#pragma unroll
+                        for (int y = 0; y < NC; y++) sc[t][y] = mfma16x16x32(ka, own.q[y][j], sc[t][y]);
+                    }
+                }
+                const int k0 = r * kKeys + 8 * g;
+                if (r * kKeys + kKeys - 1 > low_w) own.mask(sc, k0);
+                u32x4 pb[NC];
+                own.softmax(sc, a.scale, pb);
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+#pragma unroll
+                    for (int p = 0; p < NP; p++)
+#pragma unroll
+                        for (int half = 0; half < 2; half++) {
+                            const u32x4 va = from[NK + (b * NP + p) * 2 + half][lane];
+#pragma unroll
+                            for (int y = 0; y < NC; y++) own.acc[y][b][p][half] = mfma16x16x32(va, pb[y], own.acc[y][b][p][half]);
+                        }
+                    if (r * kKeys + kKeys - 1 > low && __builtin_amdgcn_readfirstlane(any_bad[st & 1][x][b]))
+                        own.spread_nan(b, bad_at[st & 1][x][b][lane], k0);
+                }
+            }
+            if (st + 1 < stages) unpack(st + 1);
+        }
+        __syncthreads();  // the next unit's first stage is written over this one's
+
+        own.sum_lanes();
+        constexpr int D = 2 * NP;  // neighbouring dims of a lane
+#pragma unroll
+        for (int t = 0; t < NC; t++) {
+            const int col = first + 16 * t + i, row = col / G;
+            if (own.limit[t] < 0) continue;
+            const int64_t at = ((int64_t)(s.part + s.local) * c.nkv + kvh) * W + col % W;
+            if (splits > 1 && g == 0) *reinterpret_cast<float2 *>(c.part_ml + 2 * at) = float2{own.m[t], own.l[t]};
+#pragma unroll
+            for (int x = 0; x < NB; x++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float o[D];
+#pragma unroll
+                    for (int d2 = 0; d2 < D; d2++) o[d2] = own.acc[t][x][d2 / 2][d2 % 2][e];
+                    const int dim = out_dim<HD>(4 * g + e, x, 0, 0);
+                    if (splits == 1) {
+                        h16 *p = a.out + (int64_t)(s.row0 + row) * a.out_stride + (kvh * G + col % G) * HD + dim;
+                        h16 r16[D];
+#pragma unroll
+                        for (int d2 = 0; d2 < D; d2++) r16[d2] = (h16)(o[d2] / own.l[t]);
+                        if (a.vec) {
+                            __builtin_memcpy(__builtin_assume_aligned(p, 2 * D), r16, sizeof r16);
+                        } else {
+                            for (int d2 = 0; d2 < D; d2++) p[d2] = r16[d2];
+                        }
+                    } else {
+                        __builtin_memcpy(__builtin_assume_aligned(c.part + at * HD + dim, 4 * D < 16 ? 4 * D : 16), o, sizeof o);
+                    }
+                }
+        }
+    }
+}
+
 // The splits of a column joined: o = sum_s 2^(scale (m_s - M)) acc_s / sum_s 2^(scale (m_s - M)) l_s. One workgroup
 // per (row, query head); its waves take the splits in turn, eight a step, all requested before their weights are known.
 template <int HD, int V>
 __global__ __launch_bounds__(kMergeWaves *kWave) void kv4_merge_kernel(Kv4Dev c, Kv4AttnArgs a) {
-    constexpr int D = HD >= kWave ? HD / kWave : 1, W = 16 << V, B = 8;  // dims per lane
+    constexpr int D = HD >= kWave ? HD / kWave : 1, W = kv4_width(V, HD), B = 8;  // dims per lane
     __shared__ float ox[kMergeWaves][HD];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int G = c.nq / c.nkv;
@@ -686,6 +917,7 @@ __global__ __launch_bounds__(kMergeWaves *kWave) void kv4_merge_kernel(Kv4Dev c,
     const Kv4Unit s = find_unit<V>(c.seqs, row, true, lane);
     const int splits = s.splits;
     if (row - s.row0 >= s.rows || splits <= 1) return;  // uniform over the workgroup
+    if (a.only && kv4_class(s.rows * G, HD) != V) return;
     const int col = (row - s.row0) * G + head % G, tiles = (s.rows * G + W - 1) / W;
     const int64_t first = ((int64_t)(s.part + (tiles - 1 - col / W) * splits) * c.nkv + head / G) * W + col % W;
     const int64_t step = (int64_t)c.nkv * W;
@@ -747,7 +979,9 @@ template <int HD, int V>
 int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, int64_t units, bool merge) {
     const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>(units * c.nkv, 1), 1 << 30));
     // few units: eight waves each, so that a CU's one or two have enough loads in flight
-    if (V < 2 && units * c.nkv <= kFewUnits)
+    if constexpr (V == 3)
+        hipLaunchKernelGGL(kv4_prompt_kernel<HD>, grid, dim3(8 * kWave), 0, st, c, a);
+    else if (V < 2 && units * c.nkv <= kFewUnits)
         hipLaunchKernelGGL((kv4_attention_kernel<HD, 1 << V, V < 2 ? 8 : 4>), grid, dim3((V < 2 ? 8 : 4) * kWave), 0, st, c, a);
     else
         hipLaunchKernelGGL((kv4_attention_kernel<HD, 1 << V, 4>), grid, dim3(4 * kWave), 0, st, c, a);
@@ -760,9 +994,12 @@ int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, 
 
 template <int HD>
 int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, int v, int64_t units, bool merge) {
-    if (v == 0) return launch_attention<HD, 0>(st, c, a, units, merge);
-    if (HD == 256 || v == 1) return launch_attention<HD, 1>(st, c, a, units, merge);
-    return launch_attention<HD, HD == 256 ? 1 : 2>(st, c, a, units, merge);
+    switch (v) {
+        case 0: return launch_attention<HD, 0>(st, c, a, units, merge);
+        case 1: return launch_attention<HD, 1>(st, c, a, units, merge);
+        case 2: return launch_attention<HD, HD == 256 ? 1 : 2>(st, c, a, units, merge);  // (no class 2 at 256)
+        default: return launch_attention<HD, 3>(st, c, a, units, merge);
+    }
 }
 
 }  // namespace aesir
@@ -783,7 +1020,8 @@ struct aesir_kv4 {
     char *ring = nullptr;  // pinned staging, handed out front to back
     int64_t ring_at = 0;
     bool batch = false;
-    int64_t batch_rows = 0, batch_cols = 0;     // new rows; most columns of one sequence
+    int64_t batch_rows = 0;
+    bool in_class[kKv4Widths] = {};             // whether the batch has sequences of a column class
     int64_t units[kKv4Widths] = {};             // attention's units of a KV head, per column width
     bool split[kKv4Widths] = {};                // and whether any sequence is split
 
@@ -795,8 +1033,10 @@ namespace {
 constexpr int64_t kRingBytes = 1 << 20;
 constexpr int64_t kMaxPages = (int64_t)1 << 30;
 constexpr int64_t kPartCols = 32768;  // columns of split partials
-constexpr int64_t kUnits = 2304;      // workgroups that attention is split for: nine on each of 256 CUs
-constexpr int64_t kMinRounds = 32;    // rounds of 32 keys that a split has at least
+// Workgroups that a class is split for (nine of four waves or two of eight on each of 256 CUs), and the rounds of 32 keys
+// that a split has at least.
+constexpr int64_t kUnits[kKv4Widths] = {2304, 2304, 2304, 512};
+constexpr int64_t kMinRounds[kKv4Widths] = {32, 32, 32, 8};
 
 struct Kv4Sizes {
     int64_t page_bytes, pool, table, seqs, ranges, moves, part, part_ml;
@@ -959,15 +1199,16 @@ bool aligned16(const void *p, int64_t cols) { return ((uintptr_t)p & 15) == 0 &&
 // Workgroups of the append and read kernels: a thread per 8 dims of a row, whole groups of four rows.
 int64_t threads_for(const aesir_kv4 *kv, int64_t rows) { return ((rows + 3) / 4 * kv->nkv * (kv->hd / 2) + kThreads - 1) / kThreads; }
 
-// Units of attention work for column tiles of width 16 << v: every sequence's rounds cut into equal splits, so
-// that the batch gives about kUnits workgroups with kMinRounds rounds or more, and the partials fit.
+// Units of attention work for the column tiles of class v: every sequence's rounds cut into equal splits, so that the
+// class's own sequences give about kUnits workgroups with kMinRounds rounds or more, and the partials fit.
 int64_t plan_width(const aesir_kv4 *kv, int v, std::vector<Kv4Seq> &ds, bool *split) {
-    const int64_t W = 16 << v, G = kv->nq / kv->nkv;
+    const int64_t W = kv4_width(v, (int)kv->hd), G = kv->nq / kv->nkv;
     int64_t work = 0;
     auto tiles = [&](const Kv4Seq &s) { return (s.rows * G + W - 1) / W; };
     auto rounds = [&](const Kv4Seq &s) { return ((int64_t)s.length + kKeys - 1) / kKeys; };
-    for (const Kv4Seq &s : ds) work += tiles(s) * rounds(s) * kv->nkv;
-    int64_t chunk = std::max<int64_t>(kMinRounds, (work + kUnits - 1) / kUnits);
+    for (const Kv4Seq &s : ds)
+        if (!kv->in_class[v] || kv4_class(s.rows * G, (int)kv->hd) == v) work += tiles(s) * rounds(s) * kv->nkv;
+    int64_t chunk = std::max<int64_t>(kMinRounds[v], (work + kUnits[v] - 1) / kUnits[v]);
     for (;; chunk *= 2) {
         int64_t items = 0, parts = 0;
         for (Kv4Seq &s : ds) {
@@ -1019,8 +1260,9 @@ int32_t kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64
     }
     kv->batch = true;
     kv->batch_rows = total;
-    kv->batch_cols = 0;
-    for (int64_t i = 0; i < n; i++) kv->batch_cols = std::max(kv->batch_cols, rows[i] * (kv->nq / kv->nkv));
+    for (bool &b : kv->in_class) b = false;
+    for (int64_t i = 0; i < n; i++)
+        if (rows[i] > 0) kv->in_class[kv4_class(rows[i] * (kv->nq / kv->nkv), (int)kv->hd)] = true;
     if (!kv->ctx) return AESIR_OK;
     for (int v = 0; v < kKv4Widths; v++) kv->units[v] = plan_width(kv, v, ds, &kv->split[v]);
     AESIR_TRY(upload(kv, seqs, n, records(kv->seqs, ds.data(), n)));
@@ -1174,21 +1416,31 @@ int32_t aesir_kv4_attention(aesir_kv4 *kv, int64_t layer, const void *query, int
     if (query_cols < kv->nq * kv->hd || output_cols < kv->nq * kv->hd)
         return fail(AESIR_ERR_SHAPE, "KV4Cache.attention: query/output rows narrower than heads * head_dim");
     if (!query || !output) return fail(AESIR_ERR_INVALID, "KV4Cache.attention: null tensor pointer");
-    const Kv4AttnArgs a{(const h16 *)query, (h16 *)output, query_cols, output_cols, layer, (int32_t)query_rows,
-                        aligned16(query, query_cols) && aligned16(output, output_cols),
-                        (float)(1.4426950408889634 / std::sqrt((double)kv->hd))};
-    // the narrowest tile that holds a sequence's columns, up to 64 (32 at head_dim 256, by its registers)
-    const int v = kv->batch_cols <= 16 ? 0 : kv->batch_cols <= 32 || kv->hd == 256 ? 1 : 2;
+    Kv4AttnArgs a{(const h16 *)query, (h16 *)output, query_cols, output_cols, layer, (int32_t)query_rows,
+                  aligned16(query, query_cols) && aligned16(output, output_cols), 1,
+                  (float)(1.4426950408889634 / std::sqrt((double)kv->hd))};
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     AESIR_HIP_TRY(hipStreamIsCapturing(kv->ctx->stream, &st));
-    // a captured call may meet a batch that is split, whatever this one is
-    const bool merge = kv->split[v] || st != hipStreamCaptureStatusNone;
-    switch (kv->hd) {
-        case 32: return launch_attention<32>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge);
-        case 64: return launch_attention<64>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge);
-        case 128: return launch_attention<128>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge);
-        default: return launch_attention<256>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge);
+    const bool captured = st != hipStreamCaptureStatusNone;
+    // A launch for the sequences of each class there is. A captured call may meet any batch later: one launch for all
+    // sequences, by its own batch's widest class, and the merge.
+    a.only = !captured;
+    int widest = 0;
+    for (int v = 0; v < kKv4Widths; v++)
+        if (kv->in_class[v]) widest = v;
+    for (int v = captured ? widest : 0; v <= widest; v++) {
+        if (!kv->in_class[v]) continue;
+        const bool merge = kv->split[v] || captured;
+        int32_t rc;
+        switch (kv->hd) {
+            case 32: rc = launch_attention<32>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge); break;
+            case 64: rc = launch_attention<64>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge); break;
+            case 128: rc = launch_attention<128>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge); break;
+            default: rc = launch_attention<256>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge); break;
+        }
+        AESIR_TRY(rc);
     }
+    return AESIR_OK;
 }
 
 int32_t aesir_kv4_read(aesir_kv4 *kv, int64_t layer, int64_t layers, const int64_t *seqs, const int64_t *pos, const int64_t *rows,

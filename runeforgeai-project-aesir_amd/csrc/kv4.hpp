@@ -19,21 +19,21 @@ namespace aesir {
 
 constexpr int kKv4Group = 32;  // dims per scale
 
-// Attention work is planned for three widths of a column tile (16, 32 and 64 (row, query head) columns);
-// every launch reads the plan of its own width, so a captured launch stays right for any later batch.
-constexpr int kKv4Widths = 3;
+// Attention work is planned for four widths of a column tile ((row, query head) columns; kv4.hip's classes). Every
+// launch reads the plan of its own width, so a captured launch stays right for any later batch.
+constexpr int kKv4Widths = 4;
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kNone = 0x7FFFFFFF;  // in every field of the records behind the last one
 
-struct Kv4Seq {  // one sequence of the batch (64 bytes)
+struct Kv4Seq {  // one sequence of the batch
     int32_t slot, length, rows, row0;  // length counts the new rows
     struct {
         int32_t unit0, splits, part0, pad;  // first (column tile, split) unit, splits of each tile, first partial slot
     } plan[kKv4Widths];
 };
-static_assert(sizeof(Kv4Seq) == 64, "descriptor");
+static_assert(sizeof(Kv4Seq) == 80, "descriptor");
 
 struct Kv4Range {  // rows to read back: positions pos .. pos + rows - 1 of a sequence, to output rows row0 ..
     int32_t slot, pos, rows, row0;

@@ -230,11 +230,12 @@ def test_a_probability_near_one_and_many_tiny_ones(A, ctx, where):
 
 
 @pytest.mark.parametrize("hd", [32, 64, 128, 256])
-def test_nothing_behind_a_row_reaches_it(A, ctx, hd):
+@pytest.mark.parametrize("nq", [2, 4, 32])
+def test_nothing_behind_a_row_reaches_it(A, ctx, hd, nq):
     """Freed pages full of NaN under the next sequence's last page, and later rows of the same batch whose
     keys and values are inf or NaN: a row's output is that of its own positions."""
     rng = np.random.default_rng(hd)
-    nq, nkv, rows, S = 4, 2, 24, 70
+    nkv, rows, S = 2, 24, 70
     kv = A.KV4Cache(ctx, 1, nq, nkv, hd, 128, 1, 64, 2)
     bad = np.full((128, nkv * hd), np.nan, np.float16)
     kv.begin([0], [128])
@@ -251,8 +252,8 @@ def test_nothing_behind_a_row_reaches_it(A, ctx, hd):
     got = attend(A, ctx, kv, 0, q).reshape(rows, nq, hd)
     K, V = kv4_values(k), kv4_values(v)
     want_nan = np.zeros((rows, nq, hd), bool)
-    want_nan[14:, :2] = True                # query heads 0, 1 read KV head 0
-    want_nan[18:, 2:, :32] = True
+    want_nan[14:, :nq // 2] = True          # the query heads of KV head 0
+    want_nan[18:, nq // 2:, :32] = True
     assert np.array_equal(np.isnan(got), want_nan), np.argwhere(np.isnan(got) != want_nan)[:5]
     Vc = V.copy()
     Vc[S - 6, hd:hd + 32] = 0               # for the dims that stay finite
@@ -262,6 +263,34 @@ def test_nothing_behind_a_row_reaches_it(A, ctx, hd):
         b = attention_bound(w, mass, top, n, hd, 8.0)
         ok = ~want_nan[r].reshape(-1)
         assert (np.abs(got[r].reshape(-1) - w[0])[ok] <= b[0][ok]).all(), r
+
+
+@pytest.mark.parametrize("hd,nq,nkv", [(32, 8, 2), (64, 8, 1), (128, 8, 2), (256, 4, 1), (128, 3, 3)])
+def test_batches_of_prompts_drafts_and_single_rows(A, ctx, hd, nq, nkv):
+    """Sequences of every column class in one batch, short and long, and a captured call of the same."""
+    rng = np.random.default_rng(hd + nq)
+    lens, new = [700, 300, 520, 900, 64, 2000, 33, 90], [1, 7, 40, 130, 64, 1, 2, 11]
+    ids = list(range(len(lens)))
+    kv = A.KV4Cache(ctx, 1, nq, nkv, hd, 2048, len(ids), 64, sum(-(-x // 64) for x in lens))
+    data = [(rand(rng, x, nkv * hd), rand(rng, x, nkv * hd)) for x in lens]
+    kv.begin(ids, [x - r for x, r in zip(lens, new)])
+    kv.append(0, *(ctx.from_numpy(np.concatenate([d[j][:x - r] for d, x, r in zip(data, lens, new)])) for j in (0, 1)))
+    kv.begin(ids, new)
+    kv.append(0, *(ctx.from_numpy(np.concatenate([d[j][x - r:] for d, x, r in zip(data, lens, new)])) for j in (0, 1)))
+    q = rand(rng, sum(new), nq * hd)
+    got = attend(A, ctx, kv, 0, q)
+    tq, out = ctx.from_numpy(q), ctx.from_numpy(np.zeros_like(q))
+    g = Graph(A, ctx, lambda: kv.attention(0, tq, out))
+    g.launch()
+    again = out.numpy().astype(np.float64)
+    g.close()
+    at = 0
+    for (k, v), x, r in zip(data, lens, new):
+        K, V = kv4_values(k), kv4_values(v)
+        for j in sorted({0, 1, r // 2, r - 1} & set(range(r))):
+            for o in (got, again):
+                check(o[at + j:at + j + 1], q[at + j:at + j + 1], K[:x - r + j + 1], V[:x - r + j + 1], nq, nkv, hd)
+        at += r
 
 
 def test_a_bad_query_row_is_its_own(A, ctx):
