@@ -503,23 +503,26 @@ struct Kv4Cols {
         }
     }
 
-    // Scores of keys k0 .. k0 + 7 (key 4 t + e in sc[t][.][e]) that a column does not see.
-    __device__ __forceinline__ void mask(f32x4 (&sc)[2][NC], int k0) const {
+    // Scores that a column does not see; sc[t][.][e] is that of key k0 + 32 (t / 2) + 4 (t % 2) + e.
+    template <int T>
+    __device__ __forceinline__ void mask(f32x4 (&sc)[T][NC], int k0) const {
 #pragma unroll
-        for (int t = 0; t < 2; t++)
+        for (int t = 0; t < T; t++)
 #pragma unroll
             for (int x = 0; x < NC; x++)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    if (k0 + 4 * t + e > limit[x]) sc[t][x][e] = -INFINITY;
+                    if (k0 + kKeys * (t / 2) + 4 * (t % 2) + e > limit[x]) sc[t][x][e] = -INFINITY;
     }
 
-    // The round's softmax step; the probabilities as P V's B operand.
-    __device__ __forceinline__ void softmax(const f32x4 (&sc)[2][NC], float scale, u32x4 (&pb)[NC]) {
+    // The softmax step of T / 2 rounds; the probabilities as P V's B operands.
+    template <int T>
+    __device__ __forceinline__ void softmax(const f32x4 (&sc)[T][NC], float scale, u32x4 (&pb)[T / 2][NC]) {
 #pragma unroll
         for (int x = 0; x < NC; x++) {
-            float mx = fmaxf(fmaxf(fmaxf(sc[0][x][0], sc[0][x][1]), fmaxf(sc[0][x][2], sc[0][x][3])),
-                             fmaxf(fmaxf(sc[1][x][0], sc[1][x][1]), fmaxf(sc[1][x][2], sc[1][x][3])));
+            float mx = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < T; t++) mx = fmaxf(mx, fmaxf(fmaxf(sc[t][x][0], sc[t][x][1]), fmaxf(sc[t][x][2], sc[t][x][3])));
             mx = swap_pair_max<32>(swap_pair_max<16>(mx));
             if (__any(mx > m[x])) {
                 const float up = fmaxf(m[x], mx), ref = up == -INFINITY ? 0.0f : up;
@@ -535,14 +538,17 @@ struct Kv4Cols {
                 m[x] = up;
             }
             const float ref = m[x] == -INFINITY ? 0.0f : m[x];
-            float pr[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                pr[e] = __builtin_amdgcn_exp2f(fmaf(sc[e / 4][x][e % 4] - ref, scale, 15.0f));
-                l[x] += pr[e];
+            for (int r = 0; r < T / 2; r++) {
+                float pr[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    pr[e] = __builtin_amdgcn_exp2f(fmaf(sc[2 * r + e / 4][x][e % 4] - ref, scale, 15.0f));
+                    l[x] += pr[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) pb[r][x][e] = h2_bits(h16x2{(h16)pr[2 * e], (h16)pr[2 * e + 1]});
             }
-#pragma unroll
-            for (int e = 0; e < 4; e++) pb[x][e] = h2_bits(h16x2{(h16)pr[2 * e], (h16)pr[2 * e + 1]});
         }
     }
 
@@ -644,13 +650,13 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
 #pragma unroll
                 for (int x = 0; x < NB; x++) bad[x] = d.hide(x, k0, keys);
             }
-            u32x4 pb[NC];
+            u32x4 pb[1][NC];
             own.softmax(sc, a.scale, pb);
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 d.value_operands(magic, b, i, [&](int p, int half, u32x4 va) {
 #pragma unroll
-                    for (int x = 0; x < NC; x++) own.acc[x][b][p][half] = mfma16x16x32(va, pb[x], own.acc[x][b][p][half]);
+                    for (int x = 0; x < NC; x++) own.acc[x][b][p][half] = mfma16x16x32(va, pb[0][x], own.acc[x][b][p][half]);
                 });
                 if (!whole && __any(bad[b] != 0)) own.spread_nan(b, ones_operand(bad[b]), k0);
             }
@@ -742,6 +748,7 @@ __global__ __launch_bounds__(8 * kWave) void kv4_prompt_kernel(Kv4Dev c, Kv4Attn
     constexpr int V = 3, W = kv4_width(V, HD), NC = W / 128, NJ = HD / 32, NP = NJ < 4 ? NJ : 4, NB = Kv4Round<HD>::NB;
     constexpr int RS = HD == 256 ? 2 : 4, PARTS = 8 / RS;  // rounds per stage; waves that unpack a round
     constexpr int NK = 2 * NJ;                             // key operands of a round, and value operands
+    constexpr int KR = 2;                                  // rounds per softmax step
     __shared__ __align__(16) u32x4 lds[2][RS][2 * NK][kWave];
     __shared__ __align__(16) u32x4 bad_at[2][RS][NB][kWave];
     __shared__ int any_bad[2][RS][NB];
@@ -833,38 +840,45 @@ __global__ __launch_bounds__(8 * kWave) void kv4_prompt_kernel(Kv4Dev c, Kv4Attn
         for (int st = 0; st < stages; st++) {
             if (st + 1 < stages) fetch(st + 1);
             __syncthreads();  // stage st is in LDS, and stage st - 1 is used up
-            for (int x = 0; x < RS; x++) {
+            for (int x = 0; x < RS; x += KR) {  // (rounds past the last are hidden keys)
                 const int r = r0 + st * RS + x;
                 if (r >= r1 || r * kKeys >= keys_w) break;
-                const u32x4(&from)[2 * NK][kWave] = lds[st & 1][x];
-                f32x4 sc[2][NC];
+                f32x4 sc[2 * KR][NC];
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
+                for (int t = 0; t < 2 * KR; t++) {
 #pragma unroll
                     for (int y = 0; y < NC; y++) sc[t][y] = f32x4{0, 0, 0, 0};
 #pragma unroll
                     for (int j = 0; j < NJ; j++) {
-                        const u32x4 ka = from[t * NJ + j][lane];
+                        const u32x4 ka = lds[st & 1][x + t / 2][t % 2 * NJ + j][lane];
 #pragma unroll
                         for (int y = 0; y < NC; y++) sc[t][y] = mfma16x16x32(ka, own.q[y][j], sc[t][y]);
                     }
                 }
-                const int k0 = r * kKeys + 8 * g;
-                if (r * kKeys + kKeys - 1 > low_w) own.mask(sc, k0);
-                u32x4 pb[NC];
+                const int k0 = r * kKeys + 8 * g, last = (r + KR) * kKeys - 1;
+                if (last > low_w) own.mask(sc, k0);
+                u32x4 pb[KR][NC];
                 own.softmax(sc, a.scale, pb);
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
+                for (int z = 0; z < KR; z++)
 #pragma unroll
-                    for (int p = 0; p < NP; p++)
+                    for (int b = 0; b < NB; b++) {
 #pragma unroll
-                        for (int half = 0; half < 2; half++) {
-                            const u32x4 va = from[NK + (b * NP + p) * 2 + half][lane];
+                        for (int p = 0; p < NP; p++)
 #pragma unroll
-                            for (int y = 0; y < NC; y++) own.acc[y][b][p][half] = mfma16x16x32(va, pb[y], own.acc[y][b][p][half]);
-                        }
-                    if (r * kKeys + kKeys - 1 > low && __builtin_amdgcn_readfirstlane(any_bad[st & 1][x][b]))
-                        own.spread_nan(b, bad_at[st & 1][x][b][lane], k0);
+                            for (int half = 0; half < 2; half++) {
+                                const u32x4 va = lds[st & 1][x + z][NK + (b * NP + p) * 2 + half][lane];
+#pragma unroll
+                                for (int y = 0; y < NC; y++) own.acc[y][b][p][half] = mfma16x16x32(va, pb[z][y], own.acc[y][b][p][half]);
+                            }
+                    }
+                if (last > low) {
+#pragma unroll
+                    for (int z = 0; z < KR; z++)
+#pragma unroll
+                        for (int b = 0; b < NB; b++)
+                            if ((r + z + 1) * kKeys - 1 > low && __builtin_amdgcn_readfirstlane(any_bad[st & 1][x + z][b]))
+                                own.spread_nan(b, bad_at[st & 1][x + z][b][lane], k0 + z * kKeys);
                 }
             }
             if (st + 1 < stages) unpack(st + 1);

@@ -293,6 +293,35 @@ def test_batches_of_prompts_drafts_and_single_rows(A, ctx, hd, nq, nkv):
         at += r
 
 
+@pytest.mark.parametrize("rows", [1, 3, 8, 80])
+@pytest.mark.parametrize("size", [30.0, 3000.0, 60000.0])
+def test_scores_of_any_size(A, ctx, rows, size):
+    """Scores from hundreds to the largest f16 rows give (10^10): no probability overflows, and a row whose best key
+    is alone gets its value. Keys are multiples of one row, so that products are exact: q = size, keys +-size times 0,
+    2^-6, .., values that tell them apart."""
+    nq, nkv, hd, S = 8, 2, 64, 300
+    rng = np.random.default_rng(rows)
+    steps = rng.permutation(np.concatenate([-np.arange(150), np.arange(150)])).astype(np.float64) / 150
+    k = np.repeat((steps * size)[:, None], nkv * hd, 1).astype(np.float16)
+    v = rand(rng, S, nkv * hd)
+    q = np.full((rows, nq * hd), size, np.float16)
+    q[:, hd:2 * hd] *= -1
+    kv = A.KV4Cache(ctx, 1, nq, nkv, hd, S, 1, 32, 10)
+    kv.begin([0], [S - rows])
+    kv.append(0, ctx.from_numpy(k[:S - rows]), ctx.from_numpy(v[:S - rows]))
+    kv.begin([0], [rows])
+    kv.append(0, ctx.from_numpy(k[S - rows:]), ctx.from_numpy(v[S - rows:]))
+    got = attend(A, ctx, kv, 0, q)
+    K, V = kv4_values(k), kv4_values(v).astype(np.float64).reshape(S, nkv, hd)
+    for r in range(rows):
+        n = S - rows + r + 1
+        for h in range(nq):
+            z = K[:n, 0].astype(np.float64) * q[r, h * hd].astype(np.float64) * hd / 8
+            if np.sort(z)[-1] - np.sort(z)[-2] > 60:  # e^-60 of the others is below every rounding
+                assert np.abs(got[r, h * hd:(h + 1) * hd] - V[z.argmax(), h // 4]).max() <= 2.0 ** -10 * np.abs(V).max(), (r, h)
+            assert np.isfinite(got[r, h * hd:(h + 1) * hd]).all()
+
+
 def test_a_bad_query_row_is_its_own(A, ctx):
     rng = np.random.default_rng(2)
     nq, nkv, hd, rows = 4, 1, 128, 6
