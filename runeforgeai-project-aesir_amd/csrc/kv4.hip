@@ -174,21 +174,21 @@ template <bool VEC>
 __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Dev c, Kv4AppendArgs a) {
     const int lane = threadIdx.x & 63;
     const Kv4Place q(c, blockIdx.x * kThreads + threadIdx.x);
-    const int per_row = c.hd / 8, row = q.row, head = q.head, chunk = q.chunk;
+    const int row = q.row, head = q.head, chunk = q.chunk;
     const i32x4 s = find_row(reinterpret_cast<const char *>(c.seqs), sizeof(Kv4Seq), row, lane);
     if (row < a.rows && s[2] > 0) {  // uniform over the quad
         const u32x4 kx = load8<VEC>(a.k + (int64_t)row * a.k_stride + head * c.hd + 8 * chunk);
         const u32x4 vx = load8<VEC>(a.v + (int64_t)row * a.v_stride + head * c.hd + 8 * chunk);
-        const int pos = s[1] - s[2] + (row - s[3]), slot = pos & (c.page_size() - 1);
-        char *b = c.block(c.table[(int64_t)s[0] * c.table_stride + (pos >> c.page_shift)], a.layer, head);
+        const int pos = s[1] - s[2] + (row - s[3]), at = pos % kKeys, grp = chunk / 4;
+        char *b = c.run(c.table[(int64_t)s[0] * c.table_stride + (pos >> c.page_shift)], a.layer, head, pos);
         const Kv4Code ck = kv4_encode(kx), cv = kv4_encode(vx);
-        reinterpret_cast<unsigned *>(b)[slot * per_row + chunk] = ck.word;
-        reinterpret_cast<unsigned *>(b + c.v_off())[(slot / 4 * per_row + chunk) * 4 + slot % 4] = cv.word;
+        *reinterpret_cast<unsigned *>(b + c.k_at(at, chunk)) = ck.word;
+        *reinterpret_cast<unsigned *>(b + c.v_at(at, chunk)) = cv.word;
         if (chunk % 4 == 0) {
-            const int grp = chunk / 4;
-            reinterpret_cast<h16x2 *>(b + c.k_scale_off())[slot * (c.hd / kKv4Group) + grp] = h16x2{ck.d, ck.m};
-            reinterpret_cast<h16 *>(b + c.v_d_off())[grp * c.page_size() + slot] = cv.d;
-            reinterpret_cast<h16 *>(b + c.v_m_off())[grp * c.page_size() + slot] = cv.m;
+            *reinterpret_cast<h16x2 *>(b + c.k_scale_at(at, grp)) = h16x2{ck.d, ck.m};
+            h16 *p = reinterpret_cast<h16 *>(b + c.v_scale_at(at, grp));
+            p[0] = cv.d;
+            p[8] = cv.m;
         }
     }
 }
@@ -226,20 +226,20 @@ __device__ __forceinline__ u32x4 kv4_decode(unsigned w, h16 d, h16 m) {
 
 template <bool VEC>
 __global__ __launch_bounds__(kThreads) void kv4_read_kernel(Kv4Dev c, Kv4ReadArgs a) {
-    const int lane = threadIdx.x & 63, per_row = c.hd / 8;
+    const int lane = threadIdx.x & 63;
     const Kv4Place q(c, blockIdx.x * kThreads + threadIdx.x);
     const int row = q.row, head = q.head, chunk = q.chunk;
     const i32x4 r = find_row(reinterpret_cast<const char *>(a.ranges), sizeof(Kv4Range), row, lane);
     if (r[2] == 0) return;
-    const int pos = r[1] + (row - r[3]), slot = pos & (c.page_size() - 1), grp = chunk / 4;
+    const int pos = r[1] + (row - r[3]), at = pos % kKeys, grp = chunk / 4;
     const int64_t page = c.table[(int64_t)r[0] * c.table_stride + (pos >> c.page_shift)];
     for (int64_t layer = blockIdx.y; layer < a.layers; layer += gridDim.y) {
-        const char *b = c.block(page, a.layer + layer, head);
-        const unsigned kw = reinterpret_cast<const unsigned *>(b)[slot * per_row + chunk];
-        const unsigned vw = reinterpret_cast<const unsigned *>(b + c.v_off())[(slot / 4 * per_row + chunk) * 4 + slot % 4];
-        const h16x2 ks = reinterpret_cast<const h16x2 *>(b + c.k_scale_off())[slot * (c.hd / kKv4Group) + grp];
-        const h16 vd = reinterpret_cast<const h16 *>(b + c.v_d_off())[grp * c.page_size() + slot];
-        const h16 vm = reinterpret_cast<const h16 *>(b + c.v_m_off())[grp * c.page_size() + slot];
+        const char *b = c.run(page, a.layer + layer, head, pos);
+        const unsigned kw = *reinterpret_cast<const unsigned *>(b + c.k_at(at, chunk));
+        const unsigned vw = *reinterpret_cast<const unsigned *>(b + c.v_at(at, chunk));
+        const h16x2 ks = *reinterpret_cast<const h16x2 *>(b + c.k_scale_at(at, grp));
+        const h16 *p = reinterpret_cast<const h16 *>(b + c.v_scale_at(at, grp));
+        const h16 vd = p[0], vm = p[8];
         const int64_t out = layer * a.all_rows + a.first_row + row;
         store8<VEC>(a.k + out * a.k_stride + head * c.hd + 8 * chunk, kv4_decode(kw, ks.x, ks.y));
         store8<VEC>(a.v + out * a.v_stride + head * c.hd + 8 * chunk, kv4_decode(vw, vd, vm));
@@ -295,13 +295,11 @@ struct Kv4AttnArgs {
     int64_t layer;
     int32_t rows;  // rows of q and out
     int32_t vec;   // q and out rows 16-byte aligned
-    int32_t only;  // leave out sequences of other column classes (they have launches of their own)
+    int32_t plan;  // of the batch's plans
     float scale;   // log2(e) / sqrt(hd)
 };
 
 constexpr int kMergeWaves = 4;
-constexpr int64_t kFewUnits = 512;  // workgroups up to which a unit takes eight waves
-constexpr int kKeys = 32;  // keys per round
 
 // Masks and exponents of the unpacking, one in a scalar and one in a vector register: as literals each pair would
 // take an AND and an OR, since one instruction takes no two literals here.
@@ -322,41 +320,45 @@ __device__ __forceinline__ h16x2 kv4_values(const Kv4Magic &c, unsigned x, h16x2
     return __builtin_elementwise_fma(n, d, m);
 }
 
-// A lane's place in the blocks of a cache: byte offsets of its share of a round behind the round's own.
+// A lane's byte offsets in a run.
 template <int HD>
 struct Kv4Lane {
     static constexpr int NJ = HD / 32, NB = NJ == 8 ? 2 : 1;
-    unsigned k, ks, v[NB], vs[NB];  // keys 8 (i / 4) + i % 4 (the second tile's four behind); 8-dim blocks and their scales
+    unsigned k, ks, v[NB], vs[NB];  // key 8 (i / 4) + i % 4 (the second tile's four behind); 8-dim blocks and their scales
 
     __device__ __forceinline__ Kv4Lane(const Kv4Dev &c, int i, int g) {
         const int key = 8 * (i / 4) + i % 4;
-        k = key * (HD / 2) + g * (HD / 8);
-        ks = c.k_scale_off() + (key * NJ + g * NJ / 4) * 4;
+        k = c.k_at(key, g * NJ);
+        ks = c.k_scale_at(key, g * NJ / 4);
 #pragma unroll
         for (int x = 0; x < NB; x++) {
             const int block = NJ < 4 ? i % (4 * NJ) : i + 16 * x;
-            v[x] = c.v_off() + (2 * g * (HD / 8) + block) * 16;
-            vs[x] = c.v_d_off() + (block / 4 * c.page_size() + 8 * g) * 2;
+            v[x] = c.v_at(8 * g, block);
+            vs[x] = c.v_scale_at(8 * g, block / 4);
         }
     }
 };
 
-template <int HD>
-struct Kv4Round {  // one lane's share of 32 keys
+// One lane's share of 32 keys. NT: loaded past the caches, for runs that one workgroup alone reads (64 sequences of about
+// 4096 positions: 74 -> 69 us); prompts' tiles share them (307 -> 322 us).
+template <int HD, bool NT>
+struct Kv4Round {
     static constexpr int NJ = HD / 32, NG = NJ == 8 ? 2 : 1, NB = NJ == 8 ? 2 : 1;
     unsigned k[2][NJ];
     h16x2 ks[2][NG];
     u32x4 v[NB][2], vd[NB], vm[NB];
 
-    // b: the block (uniform), s0: the round's first position in its page
-    __device__ __forceinline__ void load(const char *b, int s0, const Kv4Lane<HD> &o, int m_off) {
+    static __device__ __forceinline__ u32x4 ld(const char *p) { return NT ? ld16_stream(p) : ld16(p); }
+
+    __device__ __forceinline__ void load(const char *b, const Kv4Lane<HD> &o) {  // b: the run (uniform)
+        load_k(b, o, 0);
+        load_k(b, o, 1);
+        load_k_scales(b, o);
 #pragma unroll
-        for (int t = 0; t < 2; t++) load_k(b, s0, o, t);
-#pragma unroll
-        for (int x = 0; x < NB; x++) load_v(b, s0, o, m_off, x);
+        for (int x = 0; x < NB; x++) load_v(b, o, x);
     }
-    __device__ __forceinline__ void load_k(const char *b, int s0, const Kv4Lane<HD> &o, int t) {  // 16 keys
-        const char *p = b + s0 * (HD / 2) + (size_t)(o.k + t * 2 * HD);
+    __device__ __forceinline__ void load_k(const char *b, const Kv4Lane<HD> &o, int t) {  // 16 keys
+        const char *p = b + (size_t)(o.k + t * 2 * HD);
         if constexpr (NJ == 1) {
             k[t][0] = *reinterpret_cast<const unsigned *>(p);
         } else if constexpr (NJ == 2) {
@@ -366,21 +368,25 @@ struct Kv4Round {  // one lane's share of 32 keys
         } else {
 #pragma unroll
             for (int j = 0; j < NJ; j += 4) {
-                const u32x4 x = ld16(p + 4 * j);
+                const u32x4 x = ld(p + 4 * j);
 #pragma unroll
                 for (int e = 0; e < 4; e++) k[t][j + e] = x[e];
             }
         }
-        const h16x2 *ps = reinterpret_cast<const h16x2 *>(b + s0 * NJ * 4 + (size_t)(o.ks + t * 16 * NJ));
-#pragma unroll
-        for (int x = 0; x < NG; x++) ks[t][x] = ps[x];
     }
-    __device__ __forceinline__ void load_v(const char *b, int s0, const Kv4Lane<HD> &o, int m_off, int x) {  // 16 8-dim blocks
-        const char *rows = b + s0 * (HD / 2), *scales = b + s0 * 2;
+    __device__ __forceinline__ void load_k_scales(const char *b, const Kv4Lane<HD> &o) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) v[x][h] = ld16(rows + (size_t)(o.v[x] + h * 2 * HD));
-        vd[x] = ld16(scales + (size_t)o.vs[x]);
-        vm[x] = ld16(scales + m_off + (size_t)o.vs[x]);
+        for (int x = 0; x < NG; x++) {
+            const u32x2 s = *reinterpret_cast<const u32x2 *>(b + (size_t)(o.ks + 8 * x));
+            ks[0][x] = as_h2(s.x);
+            ks[1][x] = as_h2(s.y);
+        }
+    }
+    __device__ __forceinline__ void load_v(const char *b, const Kv4Lane<HD> &o, int x) {  // 16 8-dim blocks
+#pragma unroll
+        for (int h = 0; h < 2; h++) v[x][h] = ld(b + (size_t)(o.v[x] + h * 2 * HD));
+        vd[x] = ld(b + (size_t)o.vs[x]);
+        vm[x] = ld(b + (size_t)(o.vs[x] + 16));
     }
 
     // The A operand of key tile t's dims 8 j .. of the lane's share.
@@ -439,33 +445,45 @@ struct Kv4Round {  // one lane's share of 32 keys
     }
 };
 
-// What a unit of attention work needs of its sequence.
-struct Kv4Unit {
-    int slot, length, rows, row0;    // the sequence
-    int splits, part, local;         // splits of a tile, partial slot, (tile, split) index in the sequence
+// What attention needs of a sequence of the batch: its record and one of its plans.
+struct Kv4Found {
+    int slot, length, rows, row0;
+    int first, count, chunk, shift, own;
+    __device__ __forceinline__ int tile_steps() const { return (((length + kKeys - 1) / kKeys - 1) >> shift) + 1; }
 };
 
-// The sequence of a unit (a row with `by_row`) of column width V; rows 0 past the last. Lanes hold a record each; the
-// whole wave calls it.
-template <int V>
-__device__ __forceinline__ Kv4Unit find_unit(const Kv4Seq *seqs, int unit, bool by_row, int lane) {
-    Kv4Unit r{};
-    for (int base = 0;; base += kWave) {
-        const i32x4 *p = reinterpret_cast<const i32x4 *>(seqs + base + lane);
-        const i32x4 s = p[0], plan = p[1 + V];
-        const int at = __popcll(__ballot((by_row ? s[3] : plan[0]) <= unit)) - 1;
+// 64 records, one a lane.
+struct Kv4Records {
+    i32x4 s, plan;
+    __device__ __forceinline__ Kv4Records(const Kv4Seq *seqs, int p, int at) {
+        const i32x4 *r = reinterpret_cast<const i32x4 *>(seqs + at);
+        s = r[0];
+        plan = r[1 + p];
+    }
+};
+
+// The last sequence whose row0 (by_row) or plan's first is at or before x; rows and count 0 where there is none. Lanes
+// hold a record each (r: the first 64); the whole wave calls it.
+__device__ __forceinline__ Kv4Found find_seq(Kv4Records r, const Kv4Seq *seqs, int plan, int x, bool by_row, int lane) {
+    Kv4Found f{};
+    for (int base = kWave;; base += kWave) {
+        const int at = __popcll(__ballot((by_row ? r.s[3] : r.plan[0]) <= x)) - 1;
         if (at >= 0) {
-            r.slot = __builtin_amdgcn_readlane(s[0], at);
-            r.length = __builtin_amdgcn_readlane(s[1], at);
-            r.rows = __builtin_amdgcn_readlane(s[2], at);
-            r.row0 = __builtin_amdgcn_readlane(s[3], at);
-            r.local = unit - __builtin_amdgcn_readlane(plan[0], at);
-            r.splits = __builtin_amdgcn_readlane(plan[1], at);
-            r.part = __builtin_amdgcn_readlane(plan[2], at);
+            f.slot = __builtin_amdgcn_readlane(r.s[0], at);
+            f.length = __builtin_amdgcn_readlane(r.s[1], at);
+            f.rows = __builtin_amdgcn_readlane(r.s[2], at);
+            f.row0 = __builtin_amdgcn_readlane(r.s[3], at);
+            f.first = __builtin_amdgcn_readlane(r.plan[0], at);
+            f.count = __builtin_amdgcn_readlane(r.plan[1], at);
+            f.chunk = __builtin_amdgcn_readlane(r.plan[2], at);
+            const int z = __builtin_amdgcn_readlane(r.plan[3], at);
+            f.shift = z & 255;
+            f.own = z >> 8;
         }
         if (at < kWave - 1) break;
+        r = Kv4Records(seqs, plan, base + lane);
     }
-    return r;
+    return f;
 }
 
 // Two f16 per dword, 1 where bit 2 e (2 e + 1) of `bits` is set, as an operand of eight positions.
@@ -485,7 +503,7 @@ struct Kv4Cols {
     f32x4 acc[NC][NB][NP][2];
     float m[NC], l[NC];  // running maximum (the column's), sum (the lane's share, times 2^15 as acc)
 
-    __device__ __forceinline__ void start(const Kv4AttnArgs &a, const Kv4Unit &s, int first, int G, int kvh, int i, int g) {
+    __device__ __forceinline__ void start(const Kv4AttnArgs &a, const Kv4Found &s, int first, int G, int kvh, int i, int g) {
 #pragma unroll
         for (int t = 0; t < NC; t++) {
             const int col = first + 16 * t + i, row = col / G;
@@ -593,8 +611,8 @@ __device__ __forceinline__ int out_dim(int r, int x, int p, int half) {
 
 template <int HD, int NC, int NW>
 __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1) void kv4_attention_kernel(Kv4Dev c, Kv4AttnArgs a) {
-    constexpr int V = NC == 1 ? 0 : NC == 2 ? 1 : 2, W = 16 * NC;
-    constexpr int NJ = HD / 32, NP = NJ < 4 ? NJ : 4, NB = Kv4Round<HD>::NB;
+    constexpr int W = 16 * NC;
+    constexpr int NJ = HD / 32, NP = NJ < 4 ? NJ : 4, NB = Kv4Round<HD, true>::NB;
     constexpr int LD = HD + 4;  // LDS row of a column
     __shared__ float ml[NW][W][2];
     __shared__ __align__(16) float ox[NW][16][LD];
@@ -602,20 +620,30 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int G = c.nq / c.nkv;
     const Kv4Lane<HD> place(c, i, g);
-    const int m_off = c.v_m_off() - c.v_d_off();
     const Kv4Magic magic;
-    for (unsigned u = blockIdx.x;; u += gridDim.x) {
-        const int kvh = (int)(u % (unsigned)c.nkv), unit = (int)(u / (unsigned)c.nkv);
-        const Kv4Unit s = find_unit<V>(c.seqs, unit, false, lane);
-        const int splits = s.splits, cols = s.rows * G, tiles = (cols + W - 1) / W;
-        if (s.local >= tiles * splits) break;  // past the last unit (no batch: the first)
-        if (a.only && kv4_class(cols, HD) != V) continue;
-        const int tile = tiles - 1 - s.local / splits, split = s.local % splits;
+    Kv4Records records(c.seqs, a.plan, lane);
+    const int chunk = __builtin_amdgcn_readfirstlane(records.plan[2]);
+    if (chunk == kNone) return;  // no batch
+    // Workgroup b of a KV head takes steps b chunk .. (b + 1) chunk - 1 of the batch's tiles one behind the other, in
+    // pieces that end where a tile does. (A step is a round, or 2^shift of them in batches of billions of rounds.)
+    unsigned u = blockIdx.x;
+    int at = (int)(u / (unsigned)c.nkv) * chunk, end = at + chunk;
+    for (;;) {
+        const int kvh = (int)(u % (unsigned)c.nkv), b = (int)(u / (unsigned)c.nkv);
+        const Kv4Found s = find_seq(records, c.seqs, a.plan, at, false, lane);
+        const int local = at - s.first;
+        if (local >= s.count) break;  // past the last step
+        const int cols = s.rows * G, steps = s.tile_steps();
+        const int tile = local / steps, begin = local - tile * steps, stop = min(steps, begin + end - at);
+        const bool complete = begin == 0 && stop == steps;
+        const int partial = 2 * b + (at == b * chunk ? 0 : 1);  // a workgroup cuts two tiles at most
+        at += stop - begin;
+        const bool done = at >= end || (s.own && at - s.first >= s.count);  // (the next sequence starts in another)
         const int before = s.length - s.rows;
         const int low = before + tile * W / G;                                    // last position of the first column
         const int keys = before + min(s.rows - 1, (tile * W + W - 1) / G) + 1;     // positions the tile sees
-        const int rounds = (keys + kKeys - 1) / kKeys, per = (rounds + splits - 1) / splits;
-        const int r0 = split * per + wave, r1 = min(rounds, (split + 1) * per);
+        const int rounds = (keys + kKeys - 1) / kKeys;
+        const int r0 = (begin << s.shift) + wave, r1 = min(rounds, stop << s.shift);
 
         // pages of this wave's next 64 rounds, one a lane
         const int32_t *table = c.table + (int64_t)s.slot * c.table_stride;
@@ -624,12 +652,11 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
         Kv4Cols<HD, NC> own;
         own.start(a, s, tile * W, G, kvh, i, g);
 
-        const char *head_base = c.pool + a.layer * c.layer_bytes + kvh * c.head_bytes();
-        auto fetch = [&](int x, Kv4Round<HD> &d) {  // the wave's x-th round
+        auto fetch = [&](int x, Kv4Round<HD, true> &d) {  // the wave's x-th round
             const int page = __builtin_amdgcn_readlane(pages, x & (kWave - 1));
-            d.load(head_base + page * c.page_bytes, (r0 + x * NW) * kKeys & (c.page_size() - 1), place, m_off);
+            d.load(c.run(page, a.layer, kvh, (r0 + x * NW) * kKeys), place);
         };
-        auto round = [&](int r, Kv4Round<HD> &d) {
+        auto round = [&](int r, Kv4Round<HD, true> &d) {
             f32x4 sc[2][NC];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
@@ -665,7 +692,7 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
         // hit the cache): a load on one path only would make every wait behind it wait for all.
         const int mine = r0 < r1 ? (r1 - r0 + NW - 1) / NW : 0;
         if (mine > 0) {
-            Kv4Round<HD> cur, next;
+            Kv4Round<HD, true> cur, next;
             fetch(0, cur);
             for (int x = 0; x < mine; x++) {
                 const int y = min(x + 1, mine - 1);
@@ -717,7 +744,7 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
 #pragma unroll
                     for (int d = 0; d < D; d++) o[d] += ox[w][col][dim + d];
                 }
-                if (splits == 1) {
+                if (complete) {
                     h16 *p = a.out + (int64_t)(s.row0 + row) * a.out_stride + (kvh * G + gc % G) * HD + dim;
                     h16 r16[D];
 #pragma unroll
@@ -728,13 +755,20 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
                         for (int d = 0; d < D; d++) p[d] = r16[d];
                     }
                 } else {
-                    const int64_t at = ((int64_t)(s.part + s.local) * c.nkv + kvh) * W + 16 * t + col;
-                    if (threadIdx.x % T == 0) *reinterpret_cast<float2 *>(c.part_ml + 2 * at) = float2{M, L};
-                    __builtin_memcpy(__builtin_assume_aligned(c.part + at * HD + dim, 4 * D < 16 ? 4 * D : 16), o, sizeof o);
+                    const int64_t to = ((int64_t)partial * c.nkv + kvh) * W + 16 * t + col;
+                    if (threadIdx.x % T == 0) *reinterpret_cast<float2 *>(c.part_ml + 2 * to) = float2{M, L};
+                    __builtin_memcpy(__builtin_assume_aligned(c.part + to * HD + dim, 4 * D < 16 ? 4 * D : 16), o, sizeof o);
                 }
             }
-            __syncthreads();  // ox (and, before the next unit, ml) is rewritten
+            __syncthreads();  // ox (and, before the next piece, ml) is rewritten
         }
+        if (done) {
+            if (a.plan < kKv4Widths) break;  // the grid is the batch's own
+            u += gridDim.x;
+            at = (int)(u / (unsigned)c.nkv) * chunk;
+            end = at + chunk;
+        }
+        records = Kv4Records(c.seqs, a.plan, lane);
     }
 }
 
@@ -745,7 +779,8 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
 // during one and unpacked behind it.
 template <int HD>
 __global__ __launch_bounds__(8 * kWave) void kv4_prompt_kernel(Kv4Dev c, Kv4AttnArgs a) {
-    constexpr int V = 3, W = kv4_width(V, HD), NC = W / 128, NJ = HD / 32, NP = NJ < 4 ? NJ : 4, NB = Kv4Round<HD>::NB;
+    constexpr int V = 3, W = kv4_width(V, HD), NC = W / 128, NJ = HD / 32, NP = NJ < 4 ? NJ : 4;
+    constexpr int NB = Kv4Round<HD, false>::NB, NG = Kv4Round<HD, false>::NG;
     constexpr int RS = HD == 256 ? 2 : 4, PARTS = 8 / RS;  // rounds per stage; waves that unpack a round
     constexpr int NK = 2 * NJ;                             // key operands of a round, and value operands
     constexpr int KR = 2;                                  // rounds per softmax step
@@ -756,16 +791,14 @@ __global__ __launch_bounds__(8 * kWave) void kv4_prompt_kernel(Kv4Dev c, Kv4Attn
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int G = c.nq / c.nkv;
     const Kv4Lane<HD> place(c, i, g);
-    const int m_off = c.v_m_off() - c.v_d_off();
     const Kv4Magic magic;
     const int mr = wave / PARTS, part = wave % PARTS;  // the round of a stage this wave unpacks, and what of it
     for (unsigned u = blockIdx.x;; u += gridDim.x) {
         const int kvh = (int)(u % (unsigned)c.nkv), unit = (int)(u / (unsigned)c.nkv);
-        const Kv4Unit s = find_unit<V>(c.seqs, unit, false, lane);
-        const int splits = s.splits, cols = s.rows * G, tiles = (cols + W - 1) / W;
-        if (s.local >= tiles * splits) break;
-        if (a.only && kv4_class(cols, HD) != V) continue;
-        const int tile = tiles - 1 - s.local / splits, split = s.local % splits;
+        const Kv4Found s = find_seq(Kv4Records(c.seqs, a.plan, lane), c.seqs, a.plan, unit, false, lane);
+        const int splits = s.count, cols = s.rows * G, tiles = (cols + W - 1) / W, local = unit - s.first;
+        if (local >= tiles * splits) break;
+        const int tile = tiles - 1 - local / splits, split = local % splits;  // the longest first
         const int before = s.length - s.rows;
         const int low = before + tile * W / G, keys = before + min(s.rows - 1, (tile * W + W - 1) / G) + 1;
         const int rounds = (keys + kKeys - 1) / kKeys, per = ((rounds + splits - 1) / splits + RS - 1) / RS * RS;
@@ -780,56 +813,76 @@ __global__ __launch_bounds__(8 * kWave) void kv4_prompt_kernel(Kv4Dev c, Kv4Attn
         int pages = page_ids(0);
         Kv4Cols<HD, NC> own;
         own.start(a, s, first, G, kvh, i, g);
-        const char *head_base = c.pool + a.layer * c.layer_bytes + kvh * c.head_bytes();
-
-        Kv4Round<HD> d;
+        u32x4 raw[4];  // the next stage's share: keys and scales, or values and theirs
         auto fetch = [&](int st) {  // (rounds past the last one's page repeat it; their keys are hidden below)
             if ((st & (kWave - 1)) == 0 && st > 0) pages = page_ids(st);
             const int page = __builtin_amdgcn_readlane(pages, st & (kWave - 1));
-            const char *b = head_base + page * c.page_bytes;
-            const int s0 = min(r0 + st * RS + mr, rounds - 1) * kKeys & (c.page_size() - 1);
+            const char *b = c.run(page, a.layer, kvh, min(r0 + st * RS + mr, rounds - 1) * kKeys);
+            Kv4Round<HD, false> d;
             if constexpr (PARTS == 2) {
                 if (part == 0) {
-                    d.load_k(b, s0, place, 0);
-                    d.load_k(b, s0, place, 1);
+                    d.load_k(b, place, 0);
+                    d.load_k(b, place, 1);
+                    d.load_k_scales(b, place);
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) {
+                        raw[0][j] = d.k[0][j];
+                        raw[1][j] = d.k[1][j];
+                    }
+                    raw[2][0] = h2_bits(d.ks[0][0]);
+                    raw[2][1] = h2_bits(d.ks[1][0]);
                 } else {
-                    d.load_v(b, s0, place, m_off, 0);
+                    d.load_v(b, place, 0);
+                    raw[0] = d.v[0][0];
+                    raw[1] = d.v[0][1];
+                    raw[2] = d.vd[0];
+                    raw[3] = d.vm[0];
                 }
             } else {
-                if (part == 0) d.load_k(b, s0, place, 0);
-                if (part == 1) d.load_k(b, s0, place, 1);
-                if (part == 2) d.load_v(b, s0, place, m_off, 0);
-                if (part == 3) d.load_v(b, s0, place, m_off, NB - 1);
+                if (part < 2) {
+                    part == 0 ? d.load_k(b, place, 0) : d.load_k(b, place, 1);
+                    d.load_k_scales(b, place);
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) raw[j / 4][j % 4] = part == 0 ? d.k[0][j] : d.k[1][j];
+#pragma unroll
+                    for (int x = 0; x < NG; x++) raw[2][x] = h2_bits(part == 0 ? d.ks[0][x] : d.ks[1][x]);
+                } else {
+                    part == 2 ? d.load_v(b, place, 0) : d.load_v(b, place, NB - 1);
+                    raw[0] = part == 2 ? d.v[0][0] : d.v[NB - 1][0];
+                    raw[1] = part == 2 ? d.v[0][1] : d.v[NB - 1][1];
+                    raw[2] = part == 2 ? d.vd[0] : d.vd[NB - 1];
+                    raw[3] = part == 2 ? d.vm[0] : d.vm[NB - 1];
+                }
             }
         };
         auto unpack = [&](int st) {
             u32x4(&to)[2 * NK][kWave] = lds[st & 1][mr];
             const int r = r0 + st * RS + mr;
-            auto key = [&](int t) {
+            Kv4Round<HD, false> d;
+            if (part < PARTS / 2) {
+                constexpr int TILES = PARTS == 2 ? 2 : 1;  // key tiles of this wave
 #pragma unroll
-                for (int j = 0; j < NJ; j++) to[t * NJ + j][lane] = d.key_operand(magic, t, j);
-            };
-            auto value = [&](int x) {
+                for (int t = 0; t < TILES; t++) {
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) d.k[t][j] = TILES == 2 ? raw[t][j] : raw[j / 4][j % 4];
+#pragma unroll
+                    for (int x = 0; x < NG; x++) d.ks[t][x] = as_h2(raw[2][TILES == 2 ? t : x]);
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) to[(TILES == 2 ? t : part) * NJ + j][lane] = d.key_operand(magic, t, j);
+                }
+            } else {
+                const int x = part - PARTS / 2;  // the value block
+                d.v[0][0] = raw[0];
+                d.v[0][1] = raw[1];
+                d.vd[0] = raw[2];
+                d.vm[0] = raw[3];
                 if (r * kKeys + kKeys - 1 > low) {  // not seen whole by every column of the tile
-                    const unsigned bad = d.hide(x, r * kKeys + 8 * g, keys);
+                    const unsigned bad = d.hide(0, r * kKeys + 8 * g, keys);
                     const bool any = __any(bad != 0);
                     if (any) bad_at[st & 1][mr][x][lane] = ones_operand(bad);
                     if (lane == 0) any_bad[st & 1][mr][x] = any;
                 }
-                d.value_operands(magic, x, i, [&](int p, int half, u32x4 v) { to[NK + (x * NP + p) * 2 + half][lane] = v; });
-            };
-            if constexpr (PARTS == 2) {
-                if (part == 0) {
-                    key(0);
-                    key(1);
-                } else {
-                    value(0);
-                }
-            } else {
-                if (part == 0) key(0);
-                if (part == 1) key(1);
-                if (part == 2) value(0);
-                if (part == 3) value(NB - 1);
+                d.value_operands(magic, 0, i, [&](int p, int half, u32x4 v) { to[NK + (x * NP + p) * 2 + half][lane] = v; });
             }
         };
 
@@ -891,7 +944,7 @@ __global__ __launch_bounds__(8 * kWave) void kv4_prompt_kernel(Kv4Dev c, Kv4Attn
         for (int t = 0; t < NC; t++) {
             const int col = first + 16 * t + i, row = col / G;
             if (own.limit[t] < 0) continue;
-            const int64_t at = ((int64_t)(s.part + s.local) * c.nkv + kvh) * W + col % W;
+            const int64_t at = ((int64_t)(s.chunk + local) * c.nkv + kvh) * W + col % W;
             if (splits > 1 && g == 0) *reinterpret_cast<float2 *>(c.part_ml + 2 * at) = float2{own.m[t], own.l[t]};
 #pragma unroll
             for (int x = 0; x < NB; x++)
@@ -919,30 +972,44 @@ __global__ __launch_bounds__(8 * kWave) void kv4_prompt_kernel(Kv4Dev c, Kv4Attn
     }
 }
 
-// The splits of a column joined: o = sum_s 2^(scale (m_s - M)) acc_s / sum_s 2^(scale (m_s - M)) l_s. One workgroup
-// per (row, query head); its waves take the splits in turn, eight a step, all requested before their weights are known.
-template <int HD, int V>
+// The partials of a column joined: o = sum_s 2^(scale (m_s - M)) acc_s / sum_s 2^(scale (m_s - M)) l_s. MW waves per
+// (row, query head) take them in turn, eight a step, all requested before their weights are known.
+template <int HD, int V, int MW>
 __global__ __launch_bounds__(kMergeWaves *kWave) void kv4_merge_kernel(Kv4Dev c, Kv4AttnArgs a) {
     constexpr int D = HD >= kWave ? HD / kWave : 1, W = kv4_width(V, HD), B = 8;  // dims per lane
-    __shared__ float ox[kMergeWaves][HD];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ float ox[kMergeWaves][HD], mx[kMergeWaves], lx[kMergeWaves];
+    const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all % MW;
     const int G = c.nq / c.nkv;
-    const int row = (int)(blockIdx.x / (unsigned)c.nq), head = (int)(blockIdx.x % (unsigned)c.nq);
-    const Kv4Unit s = find_unit<V>(c.seqs, row, true, lane);
-    const int splits = s.splits;
-    if (row - s.row0 >= s.rows || splits <= 1) return;  // uniform over the workgroup
-    if (a.only && kv4_class(s.rows * G, HD) != V) return;
-    const int col = (row - s.row0) * G + head % G, tiles = (s.rows * G + W - 1) / W;
-    const int64_t first = ((int64_t)(s.part + (tiles - 1 - col / W) * splits) * c.nkv + head / G) * W + col % W;
-    const int64_t step = (int64_t)c.nkv * W;
+    const unsigned u = blockIdx.x * (kMergeWaves / MW) + all / MW;
+    const int row = (int)(u / (unsigned)c.nq), head = (int)(u % (unsigned)c.nq);
+    const Kv4Found s = find_seq(Kv4Records(c.seqs, a.plan, lane), c.seqs, a.plan, row, true, lane);
+    // (MW of 4: uniform over the workgroup; MW of 1: no barrier follows)
+    if (row >= a.rows || row - s.row0 >= s.rows || s.count == 0) return;
+    const int col = (row - s.row0) * G + head % G, tile = col / W;
+    int first, splits, start = 0;  // partial slots: first, then start + 2 x (width 3: first + x)
+    if constexpr (V < 3) {
+        const int steps = s.tile_steps(), from = s.first + tile * steps;
+        const int b0 = from / s.chunk;
+        splits = (from + steps - 1) / s.chunk - b0 + 1;
+        first = 2 * b0 + (from % s.chunk ? 1 : 0);
+        start = 2 * b0;
+    } else {
+        splits = s.count;
+        first = s.chunk + ((s.rows * G + W - 1) / W - 1 - tile) * splits;
+    }
+    if (splits <= 1) return;
+    auto slot = [&](int x) {
+        const int p = V == 3 ? first + x : x == 0 ? first : start + 2 * x;
+        return ((int64_t)p * c.nkv + head / G) * W + col % W;
+    };
     const int dim = HD >= kWave ? lane * D : lane % HD;
     float M = -INFINITY, L = 0.0f, o[D] = {};
-    for (int base = 0; base < splits; base += kMergeWaves * B) {
+    for (int base = 0; base < splits; base += MW * B) {
         float p[B][D];
         float2 e[B];
 #pragma unroll
         for (int j = 0; j < B; j++) {
-            const int64_t at = first + min(base + wave + kMergeWaves * j, splits - 1) * step;
+            const int64_t at = slot(min(base + wave + MW * j, splits - 1));
             e[j] = *reinterpret_cast<const float2 *>(c.part_ml + 2 * at);
             __builtin_memcpy(p[j], __builtin_assume_aligned(c.part + at * HD + dim, 4 * D < 16 ? 4 * D : 16), sizeof p[j]);
         }
@@ -955,7 +1022,7 @@ __global__ __launch_bounds__(kMergeWaves *kWave) void kv4_merge_kernel(Kv4Dev c,
         for (int d = 0; d < D; d++) o[d] *= al;
 #pragma unroll
         for (int j = 0; j < B; j++) {
-            if (base + wave + kMergeWaves * j >= splits) break;
+            if (base + wave + MW * j >= splits) break;
             const float w = __builtin_amdgcn_exp2f((e[j].x - ref) * a.scale);
             L += w * e[j].y;
 #pragma unroll
@@ -963,7 +1030,13 @@ __global__ __launch_bounds__(kMergeWaves *kWave) void kv4_merge_kernel(Kv4Dev c,
         }
         M = up;
     }
-    __shared__ float mx[kMergeWaves], lx[kMergeWaves];
+    if constexpr (MW == 1) {
+        if (HD >= kWave || lane < HD) {
+#pragma unroll
+            for (int d = 0; d < D; d++) a.out[(int64_t)row * a.out_stride + head * HD + dim + d] = (h16)(o[d] / L);
+        }
+        return;
+    }
     if (HD >= kWave || lane < HD) {
 #pragma unroll
         for (int d = 0; d < D; d++) ox[wave][dim + d] = o[d];
@@ -989,30 +1062,39 @@ __global__ __launch_bounds__(kMergeWaves *kWave) void kv4_merge_kernel(Kv4Dev c,
     }
 }
 
+// What begin() plans for one width: workgroups of a KV head, their waves, the most partials of a tile.
+struct Kv4Plan {
+    int64_t groups = 0, splits = 1;
+    int waves = 4;
+};
+
 template <int HD, int V>
-int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, int64_t units, bool merge) {
-    const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>(units * c.nkv, 1), 1 << 30));
-    // few units: eight waves each, so that a CU's one or two have enough loads in flight
+int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, const Kv4Plan &p, bool captured) {
+    const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>(p.groups * c.nkv, 1), 1 << 30));
     if constexpr (V == 3)
         hipLaunchKernelGGL(kv4_prompt_kernel<HD>, grid, dim3(8 * kWave), 0, st, c, a);
-    else if (V < 2 && units * c.nkv <= kFewUnits)
+    else if (p.waves == 8)
         hipLaunchKernelGGL((kv4_attention_kernel<HD, 1 << V, V < 2 ? 8 : 4>), grid, dim3((V < 2 ? 8 : 4) * kWave), 0, st, c, a);
     else
         hipLaunchKernelGGL((kv4_attention_kernel<HD, 1 << V, 4>), grid, dim3(4 * kWave), 0, st, c, a);
     AESIR_LAUNCH_CHECK("kv4_attention_kernel");
-    if (!merge) return AESIR_OK;
-    hipLaunchKernelGGL((kv4_merge_kernel<HD, V>), dim3((unsigned)(a.rows * c.nq)), dim3(kMergeWaves * kWave), 0, st, c, a);
+    const int64_t columns = (int64_t)a.rows * c.nq;
+    if (captured || p.splits > 8)  // a captured call may meet a batch that is split, whatever this one is
+        hipLaunchKernelGGL((kv4_merge_kernel<HD, V, kMergeWaves>), dim3((unsigned)columns), dim3(kMergeWaves * kWave), 0, st, c, a);
+    else if (p.splits > 1)
+        hipLaunchKernelGGL((kv4_merge_kernel<HD, V, 1>), dim3((unsigned)((columns + kMergeWaves - 1) / kMergeWaves)),
+                           dim3(kMergeWaves * kWave), 0, st, c, a);
     AESIR_LAUNCH_CHECK("kv4_merge_kernel");
     return AESIR_OK;
 }
 
 template <int HD>
-int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, int v, int64_t units, bool merge) {
+int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, int v, const Kv4Plan &p, bool captured) {
     switch (v) {
-        case 0: return launch_attention<HD, 0>(st, c, a, units, merge);
-        case 1: return launch_attention<HD, 1>(st, c, a, units, merge);
-        case 2: return launch_attention<HD, HD == 256 ? 1 : 2>(st, c, a, units, merge);  // (no class 2 at 256)
-        default: return launch_attention<HD, 3>(st, c, a, units, merge);
+        case 0: return launch_attention<HD, 0>(st, c, a, p, captured);
+        case 1: return launch_attention<HD, 1>(st, c, a, p, captured);
+        case 2: return launch_attention<HD, HD == 256 ? 1 : 2>(st, c, a, p, captured);  // (no class 2 at 256)
+        default: return launch_attention<HD, 3>(st, c, a, p, captured);
     }
 }
 
@@ -1036,8 +1118,7 @@ struct aesir_kv4 {
     bool batch = false;
     int64_t batch_rows = 0;
     bool in_class[kKv4Widths] = {};             // whether the batch has sequences of a column class
-    int64_t units[kKv4Widths] = {};             // attention's units of a KV head, per column width
-    bool split[kKv4Widths] = {};                // and whether any sequence is split
+    Kv4Plan plans[kKv4Plans];
 
     aesir_kv4(int64_t num_pages, int64_t page_size, int64_t max_seqs) : book(num_pages, page_size, max_seqs) {}
 };
@@ -1047,10 +1128,12 @@ namespace {
 constexpr int64_t kRingBytes = 1 << 20;
 constexpr int64_t kMaxPages = (int64_t)1 << 30;
 constexpr int64_t kPartCols = 32768;  // columns of split partials
-// Workgroups that a class is split for (nine of four waves or two of eight on each of 256 CUs), and the rounds of 32 keys
-// that a split has at least.
-constexpr int64_t kUnits[kKv4Widths] = {2304, 2304, 2304, 512};
-constexpr int64_t kMinRounds[kKv4Widths] = {32, 32, 32, 8};
+// Workgroups of attention that run at once on 256 CUs: four waves of 16, 32 and 64 columns (three, two and one to a CU by
+// their registers), or one of eight waves, which up to kFewRounds rounds in all take.
+constexpr int64_t kGroups[3] = {768, 512, 256};
+constexpr int64_t kFewRounds = 256 * 48;
+constexpr int64_t kMinRounds = 32;                       // of a workgroup, as long as CUs are left
+constexpr int64_t kPromptGroups = 512, kPromptRounds = 8;  // the same for prompts
 
 struct Kv4Sizes {
     int64_t page_bytes, pool, table, seqs, ranges, moves, part, part_ml;
@@ -1213,28 +1296,61 @@ bool aligned16(const void *p, int64_t cols) { return ((uintptr_t)p & 15) == 0 &&
 // Workgroups of the append and read kernels: a thread per 8 dims of a row, whole groups of four rows.
 int64_t threads_for(const aesir_kv4 *kv, int64_t rows) { return ((rows + 3) / 4 * kv->nkv * (kv->hd / 2) + kThreads - 1) / kThreads; }
 
-// Units of attention work for the column tiles of class v: every sequence's rounds cut into equal splits, so that the
-// class's own sequences give about kUnits workgroups with kMinRounds rounds or more, and the partials fit.
-int64_t plan_width(const aesir_kv4 *kv, int v, std::vector<Kv4Seq> &ds, bool *split) {
+// Plan p of the batch: width p for the sequences of that class, or width p - kKv4Widths for all sequences. Workgroups
+// of widths 0 - 2 get `chunk` rounds each. Where as many workgroups as run at once suffice for every tile to start one of
+// its own, tiles do (firsts rounded up to a chunk, no tile shorter than a chunk cut); else the tiles lie one behind the
+// other, so that all workgroups have equal work and none waits for a place.
+void make_plan(const aesir_kv4 *kv, int p, std::vector<Kv4Seq> &ds, Kv4Plan *out) {
+    const int v = p % kKv4Widths;
+    const bool all = p >= kKv4Widths;
     const int64_t W = kv4_width(v, (int)kv->hd), G = kv->nq / kv->nkv;
-    int64_t work = 0;
-    auto tiles = [&](const Kv4Seq &s) { return (s.rows * G + W - 1) / W; };
-    auto rounds = [&](const Kv4Seq &s) { return ((int64_t)s.length + kKeys - 1) / kKeys; };
-    for (const Kv4Seq &s : ds)
-        if (!kv->in_class[v] || kv4_class(s.rows * G, (int)kv->hd) == v) work += tiles(s) * rounds(s) * kv->nkv;
-    int64_t chunk = std::max<int64_t>(kMinRounds[v], (work + kUnits[v] - 1) / kUnits[v]);
-    for (;; chunk *= 2) {
-        int64_t items = 0, parts = 0;
-        for (Kv4Seq &s : ds) {
-            const int64_t n = std::max<int64_t>(1, (rounds(s) + chunk - 1) / chunk);
-            s.plan[v] = {(int32_t)items, (int32_t)n, (int32_t)parts, 0};
-            items += tiles(s) * n;
-            if (n > 1) parts += tiles(s) * n;
+    auto tiles = [&](const Kv4Seq &s) -> int64_t {
+        return all || kv4_class(s.rows * G, (int)kv->hd) == v ? (s.rows * G + W - 1) / W : 0;
+    };
+    int shift = 0;
+    auto rounds = [&](const Kv4Seq &s) { return (((int64_t)s.length + kKeys - 1) / kKeys + (1 << shift) - 1) >> shift; };
+    auto all_work = [&] {
+        int64_t w = 0;
+        for (const Kv4Seq &s : ds) w += tiles(s) * rounds(s);
+        return w;
+    };
+    int64_t work = all_work(), most = 1;
+    *out = Kv4Plan{};
+    if (v == 3) {  // equal splits of every tile
+        int64_t chunk = std::max<int64_t>(kPromptRounds, (work * kv->nkv + kPromptGroups - 1) / kPromptGroups);
+        for (;; chunk *= 2) {
+            int64_t units = 0, parts = 0;
+            most = 1;
+            for (Kv4Seq &s : ds) {
+                const int64_t n = tiles(s) ? std::max<int64_t>(1, (rounds(s) + chunk - 1) / chunk) : 0;
+                s.plan[p] = {(int32_t)units, (int32_t)n, (int32_t)parts, 0};
+                units += tiles(s) * n;
+                if (n > 1) parts += tiles(s) * n;
+                most = std::max(most, n);
+            }
+            if (parts * kv->nkv * W > kPartCols) continue;  // ends: one split needs no partials
+            out->groups = units;
+            out->splits = most;
+            return;
         }
-        if (parts * kv->nkv * W > kPartCols) continue;  // ends: one split needs no partials
-        *split = parts > 0;
-        return items;
     }
+    for (; work > INT32_MAX / 4; work = all_work()) shift++;  // ends: rows, and so tiles, are fewer
+    const bool few = v < 2 && work * kv->nkv <= kFewRounds;
+    const int64_t slots = std::max<int64_t>(1, (few ? 256 : kGroups[v]) / kv->nkv);  // of a KV head
+    int64_t chunk = std::max<int64_t>(std::max<int64_t>(kMinRounds >> shift, 1), (work + slots - 1) / slots), groups = 0;
+    for (const Kv4Seq &s : ds) groups += (tiles(s) * rounds(s) + chunk - 1) / chunk;
+    const bool own = groups <= slots;
+    int64_t at = 0;
+    for (Kv4Seq &s : ds) {
+        const int64_t n = tiles(s) * rounds(s);
+        if (own) at = (at + chunk - 1) / chunk * chunk;
+        s.plan[p] = {(int32_t)at, (int32_t)n, (int32_t)chunk, shift + (own ? 256 : 0)};
+        if (n) most = std::max(most, std::min((rounds(s) - 1) / chunk + 2, (at + n - 1) / chunk - at / chunk + 1));
+        at += n;
+    }
+    out->groups = (at + chunk - 1) / chunk;
+    out->splits = most;
+    out->waves = few ? 8 : 4;
 }
 
 int32_t kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64_t n) {
@@ -1263,22 +1379,25 @@ int32_t kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64
     for (int64_t i = 0; i < n; i++) kv->book.reserve(seqs[i], kv->book.seq(seqs[i]).length + rows[i]);
     int64_t at = 0;
     for (int64_t i = 0; i < n; i++) {
-        kv->book.grow(seqs[i], rows[i], copies);
         Kv4Seq &s = ds[(size_t)i];
         s = Kv4Seq{};
         s.slot = (int32_t)seqs[i];
-        s.length = (int32_t)kv->book.seq(seqs[i]).length;
+        s.length = (int32_t)(kv->book.seq(seqs[i]).length + rows[i]);
         s.rows = (int32_t)rows[i];
         s.row0 = (int32_t)at;
         at += rows[i];
     }
+    Kv4Plan plans[kKv4Plans];
+    if (kv->ctx)
+        for (int p = 0; p < kKv4Plans; p++) make_plan(kv, p, ds, &plans[p]);
+    for (int64_t i = 0; i < n; i++) kv->book.grow(seqs[i], rows[i], copies);
+    std::copy(plans, plans + kKv4Plans, kv->plans);
     kv->batch = true;
     kv->batch_rows = total;
     for (bool &b : kv->in_class) b = false;
     for (int64_t i = 0; i < n; i++)
         if (rows[i] > 0) kv->in_class[kv4_class(rows[i] * (kv->nq / kv->nkv), (int)kv->hd)] = true;
     if (!kv->ctx) return AESIR_OK;
-    for (int v = 0; v < kKv4Widths; v++) kv->units[v] = plan_width(kv, v, ds, &kv->split[v]);
     AESIR_TRY(upload(kv, seqs, n, records(kv->seqs, ds.data(), n)));
     return copy_pages(kv, copies);
 }
@@ -1431,26 +1550,26 @@ int32_t aesir_kv4_attention(aesir_kv4 *kv, int64_t layer, const void *query, int
         return fail(AESIR_ERR_SHAPE, "KV4Cache.attention: query/output rows narrower than heads * head_dim");
     if (!query || !output) return fail(AESIR_ERR_INVALID, "KV4Cache.attention: null tensor pointer");
     Kv4AttnArgs a{(const h16 *)query, (h16 *)output, query_cols, output_cols, layer, (int32_t)query_rows,
-                  aligned16(query, query_cols) && aligned16(output, output_cols), 1,
+                  aligned16(query, query_cols) && aligned16(output, output_cols), 0,
                   (float)(1.4426950408889634 / std::sqrt((double)kv->hd))};
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     AESIR_HIP_TRY(hipStreamIsCapturing(kv->ctx->stream, &st));
     const bool captured = st != hipStreamCaptureStatusNone;
     // A launch for the sequences of each class there is. A captured call may meet any batch later: one launch for all
-    // sequences, by its own batch's widest class, and the merge.
-    a.only = !captured;
+    // sequences, as wide as its own batch's widest.
     int widest = 0;
     for (int v = 0; v < kKv4Widths; v++)
         if (kv->in_class[v]) widest = v;
     for (int v = captured ? widest : 0; v <= widest; v++) {
         if (!kv->in_class[v]) continue;
-        const bool merge = kv->split[v] || captured;
+        a.plan = captured ? v + kKv4Widths : v;
+        const Kv4Plan &p = kv->plans[a.plan];
         int32_t rc;
         switch (kv->hd) {
-            case 32: rc = launch_attention<32>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge); break;
-            case 64: rc = launch_attention<64>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge); break;
-            case 128: rc = launch_attention<128>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge); break;
-            default: rc = launch_attention<256>(kv->ctx->stream, kv->dev, a, v, kv->units[v], merge); break;
+            case 32: rc = launch_attention<32>(kv->ctx->stream, kv->dev, a, v, p, captured); break;
+            case 64: rc = launch_attention<64>(kv->ctx->stream, kv->dev, a, v, p, captured); break;
+            case 128: rc = launch_attention<128>(kv->ctx->stream, kv->dev, a, v, p, captured); break;
+            default: rc = launch_attention<256>(kv->ctx->stream, kv->dev, a, v, p, captured); break;
         }
         AESIR_TRY(rc);
     }
