@@ -40,30 +40,34 @@ __global__ __launch_bounds__(kThreads) void kv4_upload_kernel(Kv4Upload u) {
 }
 
 // The record {slot, length or position, rows, first row} that a lane's row belongs to, of records in row order ended by
-// ones of kNone; rows 0 past the last. Lanes hold a record each and answer the wave's distinct rows (few: the rows of a wave
-// are neighbours) one after another, so that the only memory latency is the one load of the records.
+// ones of kNone; rows 0 past the last. Rows do not fall from lane to lane. Lanes hold a record each and answer the wave's rows
+// (few, neighbours, mostly of one record) sequence by sequence: the only memory latency is the load of the records.
 __device__ __forceinline__ i32x4 find_row(const char *records, int stride, int row, int lane) {
     i32x4 mine = {0, 0, 0, 0};
-    uint64_t open = __ballot(true);
-    for (int base = 0; open; base += kWave) {
+    int x = __builtin_amdgcn_readlane(row, 0);  // the least row that is left
+    for (int base = 0;; base += kWave) {
         const i32x4 r = *reinterpret_cast<const i32x4 *>(records + (int64_t)(base + lane) * stride);
-        const bool last = __builtin_amdgcn_readlane(r[3], kWave - 1) == kNone;  // no further records
-        uint64_t todo = open;
-        while (todo) {
-            const int x = __builtin_amdgcn_readlane(row, __builtin_ctzll(todo));
+        for (;;) {
             const int at = __popcll(__ballot(r[3] <= x)) - 1;  // the last record that starts at or before row x
-            const uint64_t same = __ballot(row == x);
+            if (at == kWave - 1) break;                        // or one of the next 64
             if (at >= 0) {
                 const i32x4 f = {__builtin_amdgcn_readlane(r[0], at), __builtin_amdgcn_readlane(r[1], at),
                                  __builtin_amdgcn_readlane(r[2], at), __builtin_amdgcn_readlane(r[3], at)};
-                if (row == x) mine = f;
+                if (row >= x) mine = f;
             }
-            if (last || at < kWave - 1) open &= ~same;
-            todo &= ~same;
+            const int next = __builtin_amdgcn_readlane(r[3], at + 1);  // of the record behind it
+            const uint64_t left = __ballot(row >= next);
+            if (!left) {
+                if (row - mine[3] >= mine[2]) mine[2] = 0;
+                return mine;
+            }
+            x = __builtin_amdgcn_readlane(row, __builtin_ctzll(left));
         }
+        // record 63 is row x's unless the next 64 say otherwise
+        const i32x4 f = {__builtin_amdgcn_readlane(r[0], kWave - 1), __builtin_amdgcn_readlane(r[1], kWave - 1),
+                         __builtin_amdgcn_readlane(r[2], kWave - 1), __builtin_amdgcn_readlane(r[3], kWave - 1)};
+        if (row >= x) mine = f;
     }
-    if (row - mine[3] >= mine[2]) mine[2] = 0;
-    return mine;
 }
 
 constexpr int kMaxSeqs = 4096;
@@ -118,21 +122,35 @@ __device__ __forceinline__ Kv4Code kv4_encode(u32x4 x) {
         c.m = bits_to_h(0x7E00);
         return c;
     }
-    h16 d = nearest_half(((double)mx - (double)mn) / 15.0);
-    if ((double)mn + 15.0 * (double)(float)d > 65504.0) d = bits_to_h((uint16_t)(h_to_bits(d) - 1));
-    const float df = (float)d, inv = df > 0.0f ? 1.0f / df : 0.0f;
+    // d from f32, which is within 2^-21 of the quotient: exact but where f16 is subnormal or the quotient lies by a
+    // border between two f16 values
+    const float step = (mx - mn) * (1.0f / 15.0f);
+    h16 d = (h16)step;
+    const unsigned tail = __builtin_bit_cast(unsigned, step) & 0x1FFFu;
+    if (step < 0x1p-14f || tail - 0xFF0u <= 0x20u) d = nearest_half(((double)mx - (double)mn) / 15.0);
+    if (mx > 60000.0f && (double)mn + 15.0 * (double)(float)d > 65504.0) d = bits_to_h((uint16_t)(h_to_bits(d) - 1));
+    const float df = (float)d, inv = df > 0.0f ? __builtin_amdgcn_rcpf(df) : 0.0f;
     unsigned w = 0;
+    bool near = false;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        // t is within 2^-18 of (v - mn) / d; where that could cross a border between levels, the border itself
-        // is compared in 64 bits (every term is exact there)
-        const float t = (v[i] - mn) * inv, low = floorf(t);
-        float q = rintf(t);
-        if (fabsf(t - low - 0.5f) < 0x1p-15f) {
-            const double u = (double)v[i] - (double)mn, border = ((double)low + 0.5) * (double)df;
-            q = u > border || (u == border && ((int)low & 1)) ? low + 1.0f : low;
+        // t is within 2^-17 of (v - mn) / d
+        const float t = (v[i] - mn) * inv;
+        near |= fabsf(__builtin_amdgcn_fractf(t) - 0.5f) < 0x1p-15f;
+        w |= (unsigned)fminf(rintf(t), 15.0f) << (4 * (i / 2) + 16 * (i % 2));
+    }
+    if (near) {  // where that could cross a border between levels, the border is compared in 64 bits (every term is exact there)
+        w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float t = (v[i] - mn) * inv, low = floorf(t);
+            float q = rintf(t);
+            if (fabsf(t - low - 0.5f) < 0x1p-15f) {
+                const double u = (double)v[i] - (double)mn, border = ((double)low + 0.5) * (double)df;
+                q = u > border || (u == border && ((int)low & 1)) ? low + 1.0f : low;
+            }
+            w |= (unsigned)fminf(q, 15.0f) << (4 * (i / 2) + 16 * (i % 2));
         }
-        w |= (unsigned)fminf(q, 15.0f) << (4 * (i / 2) + 16 * (i % 2));
     }
     c.word = w;
     c.d = d;
@@ -140,14 +158,14 @@ __device__ __forceinline__ Kv4Code kv4_encode(u32x4 x) {
     return c;
 }
 
-// What a thread of the append and read kernels works on: four rows of one head are 4 hd / 8 neighbouring threads.
+// What a thread of the append and read kernels works on (grid y: heads): four rows of a head are HD / 2 neighbouring threads.
+template <int HD>
 struct Kv4Place {
-    int row, head, chunk;
-    __device__ __forceinline__ Kv4Place(const Kv4Dev &c, unsigned u) {
-        const unsigned per_row = c.hd / 8, g = u / per_row, g4 = g / 4;
-        chunk = (int)(u % per_row);
-        head = (int)(g4 % c.nkv);
-        row = (int)(g4 / c.nkv * 4 + g % 4);
+    int row, chunk;
+    __device__ __forceinline__ Kv4Place() {
+        const unsigned u = blockIdx.x * kThreads + threadIdx.x;
+        chunk = (int)(u % (HD / 8));
+        row = (int)(u / (HD / 8));
     }
 };
 
@@ -170,15 +188,17 @@ __device__ __forceinline__ u32x4 load8(const h16 *p) {
     }
 }
 
-template <bool VEC>
+template <int HD, bool VEC>
 __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Dev c, Kv4AppendArgs a) {
-    const int lane = threadIdx.x & 63;
-    const Kv4Place q(c, blockIdx.x * kThreads + threadIdx.x);
-    const int row = q.row, head = q.head, chunk = q.chunk;
+    c.hd = HD;
+    const int lane = threadIdx.x & 63, head = blockIdx.y;
+    const Kv4Place<HD> q;
+    const int row = q.row, chunk = q.chunk;
+    // requested before the row's place is known; rows past the last repeat it
+    const int64_t from = min(row, a.rows - 1), col = head * HD + 8 * chunk;
+    const u32x4 kx = load8<VEC>(a.k + from * a.k_stride + col), vx = load8<VEC>(a.v + from * a.v_stride + col);
     const i32x4 s = find_row(reinterpret_cast<const char *>(c.seqs), sizeof(Kv4Seq), row, lane);
     if (row < a.rows && s[2] > 0) {  // uniform over the quad
-        const u32x4 kx = load8<VEC>(a.k + (int64_t)row * a.k_stride + head * c.hd + 8 * chunk);
-        const u32x4 vx = load8<VEC>(a.v + (int64_t)row * a.v_stride + head * c.hd + 8 * chunk);
         const int pos = s[1] - s[2] + (row - s[3]), at = pos % kKeys, grp = chunk / 4;
         char *b = c.run(c.table[(int64_t)s[0] * c.table_stride + (pos >> c.page_shift)], a.layer, head, pos);
         const Kv4Code ck = kv4_encode(kx), cv = kv4_encode(vx);
@@ -224,16 +244,17 @@ __device__ __forceinline__ u32x4 kv4_decode(unsigned w, h16 d, h16 m) {
     return r;
 }
 
-template <bool VEC>
+template <int HD, bool VEC>
 __global__ __launch_bounds__(kThreads) void kv4_read_kernel(Kv4Dev c, Kv4ReadArgs a) {
-    const int lane = threadIdx.x & 63;
-    const Kv4Place q(c, blockIdx.x * kThreads + threadIdx.x);
-    const int row = q.row, head = q.head, chunk = q.chunk;
+    c.hd = HD;
+    const int lane = threadIdx.x & 63, head = blockIdx.y;
+    const Kv4Place<HD> q;
+    const int row = q.row, chunk = q.chunk;
     const i32x4 r = find_row(reinterpret_cast<const char *>(a.ranges), sizeof(Kv4Range), row, lane);
     if (r[2] == 0) return;
     const int pos = r[1] + (row - r[3]), at = pos % kKeys, grp = chunk / 4;
     const int64_t page = c.table[(int64_t)r[0] * c.table_stride + (pos >> c.page_shift)];
-    for (int64_t layer = blockIdx.y; layer < a.layers; layer += gridDim.y) {
+    for (int64_t layer = blockIdx.z; layer < a.layers; layer += gridDim.z) {
         const char *b = c.run(page, a.layer + layer, head, pos);
         const unsigned kw = *reinterpret_cast<const unsigned *>(b + c.k_at(at, chunk));
         const unsigned vw = *reinterpret_cast<const unsigned *>(b + c.v_at(at, chunk));
@@ -241,8 +262,8 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(Kv4Dev c, Kv4ReadArg
         const h16 *p = reinterpret_cast<const h16 *>(b + c.v_scale_at(at, grp));
         const h16 vd = p[0], vm = p[8];
         const int64_t out = layer * a.all_rows + a.first_row + row;
-        store8<VEC>(a.k + out * a.k_stride + head * c.hd + 8 * chunk, kv4_decode(kw, ks.x, ks.y));
-        store8<VEC>(a.v + out * a.v_stride + head * c.hd + 8 * chunk, kv4_decode(vw, vd, vm));
+        store8<VEC>(a.k + out * a.k_stride + head * HD + 8 * chunk, kv4_decode(kw, ks.x, ks.y));
+        store8<VEC>(a.v + out * a.v_stride + head * HD + 8 * chunk, kv4_decode(vw, vd, vm));
     }
 }
 
@@ -1293,8 +1314,23 @@ int32_t guarded(const char *what, F f) {
 
 bool aligned16(const void *p, int64_t cols) { return ((uintptr_t)p & 15) == 0 && cols % 8 == 0; }
 
-// Workgroups of the append and read kernels: a thread per 8 dims of a row, whole groups of four rows.
-int64_t threads_for(const aesir_kv4 *kv, int64_t rows) { return ((rows + 3) / 4 * kv->nkv * (kv->hd / 2) + kThreads - 1) / kThreads; }
+// Grid of the append and read kernels: a thread per 8 dims of a row and head.
+dim3 rows_grid(const aesir_kv4 *kv, int64_t rows, int64_t layers) {
+    return dim3((unsigned)((rows * (kv->hd / 8) + kThreads - 1) / kThreads), (unsigned)kv->nkv,
+                (unsigned)std::min<int64_t>(layers, 65535));
+}
+
+#define AESIR_KV4_ROWS(kernel, vec, grid, st, dev, args)                                                          \
+    switch (kv->hd * 2 + (vec)) {                                                                                 \
+        case 64: hipLaunchKernelGGL((kernel<32, false>), grid, dim3(kThreads), 0, st, dev, args); break;          \
+        case 65: hipLaunchKernelGGL((kernel<32, true>), grid, dim3(kThreads), 0, st, dev, args); break;           \
+        case 128: hipLaunchKernelGGL((kernel<64, false>), grid, dim3(kThreads), 0, st, dev, args); break;         \
+        case 129: hipLaunchKernelGGL((kernel<64, true>), grid, dim3(kThreads), 0, st, dev, args); break;          \
+        case 256: hipLaunchKernelGGL((kernel<128, false>), grid, dim3(kThreads), 0, st, dev, args); break;        \
+        case 257: hipLaunchKernelGGL((kernel<128, true>), grid, dim3(kThreads), 0, st, dev, args); break;         \
+        case 512: hipLaunchKernelGGL((kernel<256, false>), grid, dim3(kThreads), 0, st, dev, args); break;        \
+        default: hipLaunchKernelGGL((kernel<256, true>), grid, dim3(kThreads), 0, st, dev, args); break;          \
+    }
 
 // Plan p of the batch: width p for the sequences of that class, or width p - kKv4Widths for all sequences. Workgroups
 // of widths 0 - 2 get `chunk` rounds each. Where as many workgroups as run at once suffice for every tile to start one of
@@ -1529,11 +1565,8 @@ int32_t aesir_kv4_append(aesir_kv4 *kv, int64_t layer, const void *key, int64_t 
         return fail(AESIR_ERR_SHAPE, "KV4Cache.append: key/val rows narrower than kv_heads * head_dim");
     if (!key || !val) return fail(AESIR_ERR_INVALID, "KV4Cache.append: null tensor pointer");
     const Kv4AppendArgs a{(const h16 *)key, (const h16 *)val, key_cols, val_cols, layer, (int32_t)key_rows};
-    const dim3 grid((unsigned)threads_for(kv, key_rows));
-    if (aligned16(key, key_cols) && aligned16(val, val_cols))
-        hipLaunchKernelGGL(kv4_append_kernel<true>, grid, dim3(kThreads), 0, kv->ctx->stream, kv->dev, a);
-    else
-        hipLaunchKernelGGL(kv4_append_kernel<false>, grid, dim3(kThreads), 0, kv->ctx->stream, kv->dev, a);
+    const bool vec = aligned16(key, key_cols) && aligned16(val, val_cols);
+    AESIR_KV4_ROWS(kv4_append_kernel, vec, rows_grid(kv, key_rows, 1), kv->ctx->stream, kv->dev, a)
     AESIR_LAUNCH_CHECK("kv4_append_kernel");
     return AESIR_OK;
 }
@@ -1614,11 +1647,7 @@ int32_t aesir_kv4_read(aesir_kv4 *kv, int64_t layer, int64_t layers, const int64
             AESIR_TRY(upload(kv, seqs + at, m, records(kv->ranges, r.data(), m)));
             const Kv4ReadArgs a{(h16 *)key, (h16 *)val, key_cols,     val_cols,       layer,         layers,
                                 kv->ranges, (int32_t)total, (int32_t)first};
-            const dim3 grid((unsigned)threads_for(kv, count), (unsigned)std::min<int64_t>(layers, 65535));
-            if (vec)
-                hipLaunchKernelGGL(kv4_read_kernel<true>, grid, dim3(kThreads), 0, kv->ctx->stream, kv->dev, a);
-            else
-                hipLaunchKernelGGL(kv4_read_kernel<false>, grid, dim3(kThreads), 0, kv->ctx->stream, kv->dev, a);
+            AESIR_KV4_ROWS(kv4_read_kernel, vec, rows_grid(kv, count, layers), kv->ctx->stream, kv->dev, a)
             AESIR_LAUNCH_CHECK("kv4_read_kernel");
             first += count;
         }
