@@ -130,28 +130,30 @@ __device__ __forceinline__ Kv4Code kv4_encode(u32x4 x) {
     if (step < 0x1p-14f || tail - 0xFF0u <= 0x20u) d = nearest_half(((double)mx - (double)mn) / 15.0);
     if (mx > 60000.0f && (double)mn + 15.0 * (double)(float)d > 65504.0) d = bits_to_h((uint16_t)(h_to_bits(d) - 1));
     const float df = (float)d, inv = df > 0.0f ? __builtin_amdgcn_rcpf(df) : 0.0f;
-    unsigned w = 0;
-    bool near = false;
+    // t is within 2^-17 of (v - mn) / d. Levels are joined as floats: 16 bits of them are exact
+    float q[8], far = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        // t is within 2^-17 of (v - mn) / d
         const float t = (v[i] - mn) * inv;
-        near |= fabsf(__builtin_amdgcn_fractf(t) - 0.5f) < 0x1p-15f;
-        w |= (unsigned)fminf(rintf(t), 15.0f) << (4 * (i / 2) + 16 * (i % 2));
+        q[i] = rintf(t);
+        far = fmaxf(far, fabsf(t - q[i]));
     }
-    if (near) {  // where that could cross a border between levels, the border is compared in 64 bits (every term is exact there)
-        w = 0;
+    // Where a t could be on the other side of a border between levels, the border is compared in 64 bits (every term is
+    // exact there); steps that are subnormal in f16 can leave levels past 15
+    if (far > 0.5f - 0x1p-15f || (mx - mn) * inv > 15.5f) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const float t = (v[i] - mn) * inv, low = floorf(t);
-            float q = rintf(t);
-            if (fabsf(t - low - 0.5f) < 0x1p-15f) {
+            if (fabsf(t - low - 0.5f) < 0x1p-14f) {
                 const double u = (double)v[i] - (double)mn, border = ((double)low + 0.5) * (double)df;
-                q = u > border || (u == border && ((int)low & 1)) ? low + 1.0f : low;
+                q[i] = u > border || (u == border && ((int)low & 1)) ? low + 1.0f : low;
             }
-            w |= (unsigned)fminf(q, 15.0f) << (4 * (i / 2) + 16 * (i % 2));
+            q[i] = fminf(q[i], 15.0f);
         }
     }
+    const unsigned even = (unsigned)fmaf(fmaf(fmaf(q[6], 16.0f, q[4]), 16.0f, q[2]), 16.0f, q[0]);
+    const unsigned odd = (unsigned)fmaf(fmaf(fmaf(q[7], 16.0f, q[5]), 16.0f, q[3]), 16.0f, q[1]);
+    const unsigned w = even | odd << 16;
     c.word = w;
     c.d = d;
     c.m = (h16)mn;
