@@ -222,8 +222,9 @@ struct Kv4ReadArgs {
     h16 *k, *v;
     int64_t k_stride, v_stride;
     int64_t layer, layers;
-    const Kv4Range *ranges;
+    const Kv4Range *ranges;  // null: `one`
     int32_t all_rows, first_row;  // output rows of a layer, first output row
+    Kv4Range one;                 // the only range, without a launch that brings it to the device
 };
 
 template <bool VEC>
@@ -252,7 +253,8 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(Kv4Dev c, Kv4ReadArg
     const int lane = threadIdx.x & 63, head = blockIdx.y;
     const Kv4Place<HD> q;
     const int row = q.row, chunk = q.chunk;
-    const i32x4 r = find_row(reinterpret_cast<const char *>(a.ranges), sizeof(Kv4Range), row, lane);
+    i32x4 r = {a.one.slot, a.one.pos, row < a.one.rows ? a.one.rows : 0, 0};
+    if (a.ranges) r = find_row(reinterpret_cast<const char *>(a.ranges), sizeof(Kv4Range), row, lane);
     if (r[2] == 0) return;
     const int pos = r[1] + (row - r[3]), at = pos % kKeys, grp = chunk / 4;
     const int64_t page = c.table[(int64_t)r[0] * c.table_stride + (pos >> c.page_shift)];
@@ -1613,7 +1615,7 @@ int32_t aesir_kv4_attention(aesir_kv4 *kv, int64_t layer, const void *query, int
 
 int32_t aesir_kv4_read(aesir_kv4 *kv, int64_t layer, int64_t layers, const int64_t *seqs, const int64_t *pos, const int64_t *rows,
                        int64_t n, void *key, int64_t key_rows, int64_t key_cols, void *val, int64_t val_rows, int64_t val_cols) {
-    AESIR_TRY(need_device(kv, "read"));
+    if (kv && !kv->ctx) return need_device(kv, "read");
     AESIR_TRY(can_change(kv, "read"));
     if (layer < 0 || layers < 0 || layer > kv->layers - layers) return fail(AESIR_ERR_INVALID, "KV4Cache.read: layer out of bounds");
     if (n < 0 || (n > 0 && (!seqs || !pos || !rows))) return fail(AESIR_ERR_INVALID, "KV4Cache.read: null argument");
@@ -1646,9 +1648,9 @@ int32_t aesir_kv4_read(aesir_kv4 *kv, int64_t layer, int64_t layers, const int64
                 count += rows[i];
             }
             if (count == 0) continue;
-            AESIR_TRY(upload(kv, seqs + at, m, records(kv->ranges, r.data(), m)));
+            AESIR_TRY(upload(kv, seqs + at, m, m == 1 ? Run{} : records(kv->ranges, r.data(), m)));
             const Kv4ReadArgs a{(h16 *)key, (h16 *)val, key_cols,     val_cols,       layer,         layers,
-                                kv->ranges, (int32_t)total, (int32_t)first};
+                                m == 1 ? nullptr : kv->ranges, (int32_t)total, (int32_t)first, r[0]};
             AESIR_KV4_ROWS(kv4_read_kernel, vec, rows_grid(kv, count, layers), kv->ctx->stream, kv->dev, a)
             AESIR_LAUNCH_CHECK("kv4_read_kernel");
             first += count;
