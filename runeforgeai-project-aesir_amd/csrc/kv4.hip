@@ -618,13 +618,9 @@ struct Kv4Cols {
     }
 };
 
-// The column tile width of a launch for sequences of many or few columns ((row, query head of a group) pairs), and which
-// one a sequence takes: the narrowest that holds its columns, up to 64; more go to the kernel that shares unpacked keys
-// among eight waves of columns (256 wide, 128 at head_dim 256, where 64 would not fit the registers).
+// The column tile widths of the launches: 16, 32 or 64 ((row, query head of a group) pairs), and for prompts 256; at head_dim
+// 256 16 and 128.
 __host__ __device__ constexpr int kv4_width(int v, int hd) { return v < 3 ? 16 << v : hd == 256 ? 128 : 256; }
-__host__ __device__ constexpr int kv4_class(int64_t cols, int hd) {
-    return cols <= 16 ? 0 : cols <= 32 ? 1 : cols <= 64 && hd < 256 ? 2 : 3;
-}
 
 // The dim of accumulator (x, p, half) in matrix row r.
 template <int HD>
@@ -1104,7 +1100,9 @@ int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, 
         hipLaunchKernelGGL((kv4_attention_kernel<HD, 1 << V, 4>), grid, dim3(4 * kWave), 0, st, c, a);
     AESIR_LAUNCH_CHECK("kv4_attention_kernel");
     const int64_t columns = (int64_t)a.rows * c.nq;
-    if (captured || p.splits > 8)  // a captured call may meet a batch that is split, whatever this one is
+    // a wave for a row and head with few partials, four with many (47: 16.5 -> 14.4 us in all; 12 of 40 rows: 16.3, 19.1 with four);
+    // a captured call may meet a batch that is split, whatever this one is
+    if (captured || p.splits > 16)
         hipLaunchKernelGGL((kv4_merge_kernel<HD, V, kMergeWaves>), dim3((unsigned)columns), dim3(kMergeWaves * kWave), 0, st, c, a);
     else if (p.splits > 1)
         hipLaunchKernelGGL((kv4_merge_kernel<HD, V, 1>), dim3((unsigned)((columns + kMergeWaves - 1) / kMergeWaves)),
@@ -1115,12 +1113,12 @@ int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, 
 
 template <int HD>
 int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, int v, const Kv4Plan &p, bool captured) {
-    switch (v) {
-        case 0: return launch_attention<HD, 0>(st, c, a, p, captured);
-        case 1: return launch_attention<HD, 1>(st, c, a, p, captured);
-        case 2: return launch_attention<HD, HD == 256 ? 1 : 2>(st, c, a, p, captured);  // (no class 2 at 256)
-        default: return launch_attention<HD, 3>(st, c, a, p, captured);
+    if (v == 3) return launch_attention<HD, 3>(st, c, a, p, captured);
+    if constexpr (HD < 256) {
+        if (v == 1) return launch_attention<HD, 1>(st, c, a, p, captured);
+        if (v == 2) return launch_attention<HD, 2>(st, c, a, p, captured);
     }
+    return launch_attention<HD, 0>(st, c, a, p, captured);
 }
 
 }  // namespace aesir
@@ -1153,12 +1151,31 @@ namespace {
 constexpr int64_t kRingBytes = 1 << 20;
 constexpr int64_t kMaxPages = (int64_t)1 << 30;
 constexpr int64_t kPartCols = 32768;  // columns of split partials
-// Workgroups of attention that run at once on 256 CUs: four waves of 16, 32 and 64 columns (three, two and one to a CU by
-// their registers), or one of eight waves, which up to kFewRounds rounds in all take.
-constexpr int64_t kGroups[3] = {768, 512, 256};
-constexpr int64_t kFewRounds = 256 * 48;
-constexpr int64_t kMinRounds = 32;                       // of a workgroup, as long as CUs are left
-constexpr int64_t kPromptGroups = 512, kPromptRounds = 8;  // the same for prompts
+// How attention's work is cut, with us per call of 32 query heads of 128 over 8 KV heads, one row a sequence, unless
+// said otherwise:
+// - a workgroup to a tile where that fills the CUs and no tile is long (merges saved: 64 sequences of about 1000
+//   positions 25.5 -> 21.5, of 2000 at 4 KV heads of 64 20.5 -> 17.1; 32 of 2000 25.3 / 25.9), or where all are short (4 of
+//   500, 4 KV heads of 64: 6.7, in two pieces 8.3);
+// - little work that one workgroup a CU can take in pieces of their own: kFewLeast rounds or more each (8 / 12 / 16 / 32
+//   rounds: one sequence of 1024 positions 8.8 / 9.5 / 10.2 / 10.5, of 4096 10.4 / 10.6 / 10.9 / 13.2), of eight
+//   waves where pieces are over 16 rounds (one of 65536 positions 25.4 with four, 22.9; of 100 4.7 with four, 5.0);
+// - else as many workgroups of four waves as run at once (three, two and one to a CU by the registers of 16, 32 and 64
+//   columns), kLeast rounds each or more (32 / 48 / 64: 24 sequences of 3000 26.0 / 25.6 / 31.0, 40 of 4000 43.1 / 43.4 /
+//   47.3), half of that with little work (12 / 24 / 48: 8 of 2048 12.7 / 12.3 / 17.6); equal shares of all tiles where
+//   starts of their own don't fit (64 of 4096: 66.5 against 75.8).
+constexpr int64_t kWholeRounds = 96, kShortRounds = 24;
+constexpr int64_t kFewRounds = 256 * 64, kFewLeast = 8;
+constexpr int64_t kGroups[3] = {768, 512, 256}, kLeast = 48;
+// Workgroups of prompts, and rounds of each at least (8 / 16 / 32: 128 rows over 2048 positions 28.1 / 34.2 / 51.7).
+constexpr int64_t kPromptGroups = 512, kPromptRounds = 8;
+// Rounds of all tiles up to which 16-column tiles, which work side by side, beat the tile that holds all columns of a
+// sequence and reads its keys once (one sequence of 2048 positions, 16 rows: 10.0 against 15.7 with 64 columns, 4.0 K
+// rounds of 8000 positions 16.5 / 15.0 with 32), and up to which 32-column tiles beat the prompts' (128 rows of 2048
+// positions 20.0 / 28.1, 48 of 8 sequences of 2048, 24.5 K rounds, 51 / 99; 1000 of 1000, 32 K, 58 / 48). At head_dim 256
+// there are 16-column tiles (for up to 32 columns: 64 sequences of 8 rows 94 / 126) and the prompts' only: 32 columns
+// would leave the registers one wave to a SIMD and spill (4 KV heads, 128 rows of 2048 positions, 8.2 K rounds, 23 / 30; 300
+// of 1000, 9.6 K, 39 / 31; 16 rows of 8 sequences of 2048, 8.2 K, 41 / 32).
+constexpr int64_t kNarrowRounds = 2560, kNarrowRounds256 = 6144, kPromptLeast = 28672;
 
 struct Kv4Sizes {
     int64_t page_bytes, pool, table, seqs, ranges, moves, part, part_ml;
@@ -1336,16 +1353,37 @@ dim3 rows_grid(const aesir_kv4 *kv, int64_t rows, int64_t layers) {
         default: hipLaunchKernelGGL((kernel<256, true>), grid, dim3(kThreads), 0, st, dev, args); break;          \
     }
 
+// The width every sequence of the batch takes: the narrowest that holds its columns, or a narrower one with little work.
+std::vector<int> column_classes(const aesir_kv4 *kv, const std::vector<Kv4Seq> &ds) {
+    const int64_t G = kv->nq / kv->nkv;
+    auto work = [&](int64_t W) {
+        int64_t w = 0;
+        for (const Kv4Seq &s : ds) w += (s.rows * G + W - 1) / W * (((int64_t)s.length + kKeys - 1) / kKeys) * kv->nkv;
+        return w;
+    };
+    const bool large = kv->hd == 256;
+    const bool narrow = work(16) <= (large ? kNarrowRounds256 : kNarrowRounds), prompts = work(32) > kPromptLeast;
+    std::vector<int> c;
+    for (const Kv4Seq &s : ds) {
+        const int64_t cols = s.rows * G;
+        if (large)
+            c.push_back(narrow || cols <= 32 ? 0 : 3);
+        else
+            c.push_back(narrow || cols <= 16 ? 0 : cols <= 32 ? 1 : cols <= 64 ? 2 : prompts ? 3 : 1);
+    }
+    return c;
+}
+
 // Plan p of the batch: width p for the sequences of that class, or width p - kKv4Widths for all sequences. Workgroups
-// of widths 0 - 2 get `chunk` rounds each. Where as many workgroups as run at once suffice for every tile to start one of
-// its own, tiles do (firsts rounded up to a chunk, no tile shorter than a chunk cut); else the tiles lie one behind the
-// other, so that all workgroups have equal work and none waits for a place.
-void make_plan(const aesir_kv4 *kv, int p, std::vector<Kv4Seq> &ds, Kv4Plan *out) {
+// of widths 0 - 2 get `chunk` rounds each. With `own`, sequences start workgroups of their own (firsts rounded up to a
+// chunk); else they lie one behind the other, so that all workgroups have equal work and none waits for a place. Partials
+// fit: only tiles that are cut have them, two at most a workgroup, and there are no more workgroups than kGroups then.
+void make_plan(const aesir_kv4 *kv, int p, std::vector<Kv4Seq> &ds, const std::vector<int> &classes, Kv4Plan *out) {
     const int v = p % kKv4Widths;
     const bool all = p >= kKv4Widths;
     const int64_t W = kv4_width(v, (int)kv->hd), G = kv->nq / kv->nkv;
     auto tiles = [&](const Kv4Seq &s) -> int64_t {
-        return all || kv4_class(s.rows * G, (int)kv->hd) == v ? (s.rows * G + W - 1) / W : 0;
+        return all || classes[(size_t)(&s - ds.data())] == v ? (s.rows * G + W - 1) / W : 0;
     };
     int shift = 0;
     auto rounds = [&](const Kv4Seq &s) { return (((int64_t)s.length + kKeys - 1) / kKeys + (1 << shift) - 1) >> shift; };
@@ -1375,11 +1413,31 @@ void make_plan(const aesir_kv4 *kv, int p, std::vector<Kv4Seq> &ds, Kv4Plan *out
         }
     }
     for (; work > INT32_MAX / 4; work = all_work()) shift++;  // ends: rows, and so tiles, are fewer
-    const bool few = v < 2 && work * kv->nkv <= kFewRounds;
-    const int64_t slots = std::max<int64_t>(1, (few ? 256 : kGroups[v]) / kv->nkv);  // of a KV head
-    int64_t chunk = std::max<int64_t>(std::max<int64_t>(kMinRounds >> shift, 1), (work + slots - 1) / slots), groups = 0;
-    for (const Kv4Seq &s : ds) groups += (tiles(s) * rounds(s) + chunk - 1) / chunk;
-    const bool own = groups <= slots;
+    int64_t longest = 0, count = 0;
+    bool single = true;  // no sequence of several tiles
+    for (const Kv4Seq &s : ds) {
+        if (tiles(s)) longest = std::max(longest, rounds(s));
+        count += tiles(s);
+        single &= tiles(s) <= 1;
+    }
+    int64_t slots = 1, chunk = 1, groups = 0;
+    auto cut = [&](int64_t at_once, int64_t least) {
+        slots = std::max<int64_t>(1, at_once / kv->nkv);  // of a KV head
+        chunk = std::max<int64_t>(std::max<int64_t>(least >> shift, 1), (work + slots - 1) / slots);
+        groups = 0;
+        for (const Kv4Seq &s : ds) groups += (tiles(s) * rounds(s) + chunk - 1) / chunk;
+        return groups <= slots;
+    };
+    bool eight = false, own = true;
+    const bool few = work * kv->nkv <= kFewRounds;
+    if (single && shift == 0 && longest <= (count * kv->nkv >= 256 ? kWholeRounds : kShortRounds)) {
+        chunk = std::max<int64_t>(longest, 1);
+        eight = v < 2 && count * kv->nkv <= 256 && longest > 16;
+    } else if (few && cut(256, kFewLeast)) {
+        eight = v < 2 && std::min(longest, chunk) > 16;
+    } else {
+        own = cut(kv->hd == 256 ? kGroups[1] : kGroups[v], few ? kLeast / 2 : kLeast);
+    }
     int64_t at = 0;
     for (Kv4Seq &s : ds) {
         const int64_t n = tiles(s) * rounds(s);
@@ -1390,7 +1448,7 @@ void make_plan(const aesir_kv4 *kv, int p, std::vector<Kv4Seq> &ds, Kv4Plan *out
     }
     out->groups = (at + chunk - 1) / chunk;
     out->splits = most;
-    out->waves = few ? 8 : 4;
+    out->waves = eight ? 8 : 4;
 }
 
 int32_t kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64_t n) {
@@ -1428,15 +1486,16 @@ int32_t kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64
         at += rows[i];
     }
     Kv4Plan plans[kKv4Plans];
+    const std::vector<int> classes = kv->ctx ? column_classes(kv, ds) : std::vector<int>();
     if (kv->ctx)
-        for (int p = 0; p < kKv4Plans; p++) make_plan(kv, p, ds, &plans[p]);
+        for (int p = 0; p < kKv4Plans; p++) make_plan(kv, p, ds, classes, &plans[p]);
     for (int64_t i = 0; i < n; i++) kv->book.grow(seqs[i], rows[i], copies);
     std::copy(plans, plans + kKv4Plans, kv->plans);
     kv->batch = true;
     kv->batch_rows = total;
     for (bool &b : kv->in_class) b = false;
     for (int64_t i = 0; i < n; i++)
-        if (rows[i] > 0) kv->in_class[kv4_class(rows[i] * (kv->nq / kv->nkv), (int)kv->hd)] = true;
+        if (rows[i] > 0 && kv->ctx) kv->in_class[classes[(size_t)i]] = true;
     if (!kv->ctx) return AESIR_OK;
     AESIR_TRY(upload(kv, seqs, n, records(kv->seqs, ds.data(), n)));
     return copy_pages(kv, copies);
