@@ -281,7 +281,8 @@ int32_t aesir_kv_v_slice(const aesir_kv *kv, int64_t layer_idx, int64_t seq_len,
  * in batch order, each sequence's in position order, row r of a sequence seeing the positions up to its
  * own. Tensors are f16 rows of `cols` elements from row to row, of which the first heads * head_dim count
  * (so K, V and Q may be parts of one fused matrix); any 2-byte alignment, 16 bytes with cols a multiple of
- * 8 being the fast one. Outputs must not overlap inputs.
+ * 8 being the fast one. Outputs must not overlap inputs. Sums run in an order that the batch and the sizes fix: the
+ * same call gives the same bits, other batches around a row may give others.
  *
  * append() and attention() may be captured into a HIP graph on the context's stream. A replay there serves
  * the batch of its time: it stores or attends for the first rows of it, as many as the captured call had,

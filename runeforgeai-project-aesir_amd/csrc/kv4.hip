@@ -77,7 +77,8 @@ constexpr int kMaxSeqs = 4096;
 // One thread per 8 dims of a K and of a V row (16-byte loads); the four lanes of a quad hold a group of 32, whose
 // minimum and maximum they exchange by DPP. Four consecutive rows of one head are neighbouring lane groups, so a
 // V tile of four positions leaves as one contiguous store. The quantization is exact: scales and levels are the
-// nearest ones of the real quotients, ties to even, as their definition says.
+// nearest ones of the real quotients, ties to even, as their definition says. Bound by instructions (some 20 an element of
+// scales, levels and packing): 8192 rows of 8 heads of 128, 13.8 us for 44 MB; one row by the launch and two reads, 2.7 us.
 
 // The f16 nearest a double (ties to even): through f32 rounded to odd, so the second rounding decides alone.
 __device__ __forceinline__ h16 nearest_half(double x) {
@@ -217,7 +218,8 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Dev c, Kv4Appen
 
 // ------------------------------------------------------------------ read
 //
-// The f16 values of position ranges, one thread per 8 dims of K and V.
+// The f16 values of position ranges, one thread per 8 dims of K and V. Bound by memory: 2000 positions of 32 layers and 8
+// heads of 128 (344 MB with what it writes) 70 us, 4.9 TB/s.
 struct Kv4ReadArgs {
     h16 *k, *v;
     int64_t k_stride, v_stride;
@@ -274,7 +276,7 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(Kv4Dev c, Kv4ReadArg
 // ------------------------------------------------------------------ page copies
 //
 // 16 KB of a page per workgroup step, four 16-byte loads in flight per thread. Sources and destinations of one
-// launch are disjoint.
+// launch are disjoint. Bound by memory: 32 pages of 2.6 MB 25 us, 6.7 TB/s read and written.
 constexpr int kCopyChunk = kThreads * 16 * 4;
 
 __global__ __launch_bounds__(kThreads) void kv4_copy_kernel(char *pool, int64_t page_bytes, const PageMove *moves, int n) {
@@ -297,9 +299,12 @@ __global__ __launch_bounds__(kThreads) void kv4_copy_kernel(char *pool, int64_t 
 // ------------------------------------------------------------------ attention
 //
 // o = softmax(q k^T / sqrt(hd)) v of the batch's new rows over the positions up to their own, on the matrix
-// cores. A column is one (row, query head of the KV head's group) pair; a unit of work is a tile of 16 NC columns
-// of one sequence and KV head and a split of its rounds of 32 keys. Four waves take the unit's rounds in turn, each
-// for all columns (a key is unpacked by one wave, once a unit), and meet in LDS at the end.
+// cores. A column is one (row, query head of the KV head's group) pair. A workgroup takes a tile of 16 NC columns of one
+// sequence and KV head, or a piece of its rounds of 32 keys, or pieces of several; its four or eight waves take the rounds in
+// turn, each for all columns (a key is unpacked by one wave, once a tile), and meet in LDS at the end; a tile's
+// pieces meet in kv4_merge_kernel. Bound by memory where there is much to read: 64 sequences of about 4096 positions, 8 KV
+// heads of 128 (335 MB), 62 us and 5 for the merge, 5.4 TB/s; else by the chain of reads that a workgroup starts
+// with (records, page ids, the first round) and the launches: 4.2 us for 100 positions.
 //
 //   scores   S^T = K q^T: a 16-key tile's A operand is unpacked nibbles; lane (i, g) holds key 8 (i / 4) + 4 t + i % 4
 //            of the round (t = 0, 1) and the hd / 4 dims from g hd / 4, so one load brings its part of the row
@@ -797,7 +802,9 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
 // and values between them, each operand once, into LDS in the order in which the matrix instructions take them (1 KB an
 // operand, 16 bytes a lane, no bank conflicts); every wave then runs those rounds over its own columns, so unpacking costs
 // an eighth a column and the waves never meet but at the barrier between stages. Two stages of LDS: the next is loaded
-// during one and unpacked behind it.
+// during one and unpacked behind it. 2048 rows of 8192 positions (32 query heads of 128, 8 KV heads): 296 us, 813 TFLOP/s;
+// two waves to a SIMD issue vector instructions half of the time and matrix instructions a third, mostly not at once
+// (raising the priority of either phase, or sums as a product with ones, changed nothing: 296 - 310 us).
 template <int HD>
 __global__ __launch_bounds__(8 * kWave) void kv4_prompt_kernel(Kv4Dev c, Kv4AttnArgs a) {
     constexpr int V = 3, W = kv4_width(V, HD), NC = W / 128, NJ = HD / 32, NP = NJ < 4 ? NJ : 4;
@@ -1149,7 +1156,7 @@ struct aesir_kv4 {
 namespace {
 
 constexpr int64_t kRingBytes = 1 << 20;
-constexpr int64_t kMaxPages = (int64_t)1 << 30;
+constexpr int64_t kMaxPages = (int64_t)1 << 27;
 constexpr int64_t kPartCols = 32768;  // columns of split partials
 // How attention's work is cut, with us per call of 32 query heads of 128 over 8 KV heads, one row a sequence, unless
 // said otherwise:
@@ -1219,18 +1226,19 @@ int32_t need_device(aesir_kv4 *kv, const char *what) {
 }
 
 // Calls that change the tables send host data to the device, which a replay would not send again.
-int32_t can_change(aesir_kv4 *kv, const char *what) {
-    if (!kv) return fail(AESIR_ERR_INVALID, "KV4Cache.%s: null cache", what);
-    if (!kv->ctx) {
-        clear_error();
-        return AESIR_OK;
-    }
-    AESIR_TRY(bind(kv->ctx));
+int32_t not_captured(aesir_ctx *ctx, const char *what) {
+    AESIR_TRY(bind(ctx));
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    AESIR_HIP_TRY(hipStreamIsCapturing(kv->ctx->stream, &st));
+    AESIR_HIP_TRY(hipStreamIsCapturing(ctx->stream, &st));
     if (st != hipStreamCaptureStatusNone)
         return fail(AESIR_ERR_INVALID, "KV4Cache.%s: not while the context's stream is being captured", what);
     return AESIR_OK;
+}
+
+int32_t can_change(aesir_kv4 *kv, const char *what) {
+    clear_error();
+    if (!kv) return fail(AESIR_ERR_INVALID, "KV4Cache.%s: null cache", what);
+    return kv->ctx ? not_captured(kv->ctx, what) : AESIR_OK;
 }
 
 int32_t seq_ok(aesir_kv4 *kv, const char *what, int64_t s) {
@@ -1331,6 +1339,13 @@ int32_t guarded(const char *what, F f) {
     } catch (const std::exception &) {
         return fail(AESIR_ERR_EXHAUSTED, "KV4Cache.%s: out of host memory", what);
     }
+}
+
+// f16 rows start on f16 boundaries.
+int32_t pointers_ok(const char *what, const void *a, const void *b) {
+    if (!a || !b) return fail(AESIR_ERR_INVALID, "KV4Cache.%s: null tensor pointer", what);
+    if (((uintptr_t)a | (uintptr_t)b) & 1) return fail(AESIR_ERR_INVALID, "KV4Cache.%s: tensor pointer not 2-byte aligned", what);
+    return AESIR_OK;
 }
 
 bool aligned16(const void *p, int64_t cols) { return ((uintptr_t)p & 15) == 0 && cols % 8 == 0; }
@@ -1525,7 +1540,7 @@ int32_t aesir_kv4_create(aesir_ctx *ctx, int64_t num_layers, int64_t n_heads, in
     *out = nullptr;
     Kv4Sizes z;
     AESIR_TRY(kv4_sizes(num_layers, n_heads, n_kv_heads, head_dim, max_seq_len, max_seqs, page_size, num_pages, &z));
-    if (ctx) AESIR_TRY(bind(ctx));
+    if (ctx) AESIR_TRY(not_captured(ctx, "create"));
     return guarded("create", [&]() -> int32_t {
         auto *kv = new aesir_kv4(num_pages, page_size, max_seqs);
         kv->layers = num_layers;
@@ -1626,7 +1641,7 @@ int32_t aesir_kv4_append(aesir_kv4 *kv, int64_t layer, const void *key, int64_t 
     if (kv->batch_rows == 0) return AESIR_OK;
     if (key_cols < kv->nkv * kv->hd || val_cols < kv->nkv * kv->hd)
         return fail(AESIR_ERR_SHAPE, "KV4Cache.append: key/val rows narrower than kv_heads * head_dim");
-    if (!key || !val) return fail(AESIR_ERR_INVALID, "KV4Cache.append: null tensor pointer");
+    AESIR_TRY(pointers_ok("append", key, val));
     const Kv4AppendArgs a{(const h16 *)key, (const h16 *)val, key_cols, val_cols, layer, (int32_t)key_rows};
     const bool vec = aligned16(key, key_cols) && aligned16(val, val_cols);
     AESIR_KV4_ROWS(kv4_append_kernel, vec, rows_grid(kv, key_rows, 1), kv->ctx->stream, kv->dev, a)
@@ -1644,7 +1659,7 @@ int32_t aesir_kv4_attention(aesir_kv4 *kv, int64_t layer, const void *query, int
     if (kv->batch_rows == 0) return AESIR_OK;
     if (query_cols < kv->nq * kv->hd || output_cols < kv->nq * kv->hd)
         return fail(AESIR_ERR_SHAPE, "KV4Cache.attention: query/output rows narrower than heads * head_dim");
-    if (!query || !output) return fail(AESIR_ERR_INVALID, "KV4Cache.attention: null tensor pointer");
+    AESIR_TRY(pointers_ok("attention", query, output));
     Kv4AttnArgs a{(const h16 *)query, (h16 *)output, query_cols, output_cols, layer, (int32_t)query_rows,
                   aligned16(query, query_cols) && aligned16(output, output_cols), 0,
                   (float)(1.4426950408889634 / std::sqrt((double)kv->hd))};
@@ -1693,7 +1708,7 @@ int32_t aesir_kv4_read(aesir_kv4 *kv, int64_t layer, int64_t layers, const int64
     if (total * layers == 0) return AESIR_OK;
     if (key_cols < kv->nkv * kv->hd || val_cols < kv->nkv * kv->hd)
         return fail(AESIR_ERR_SHAPE, "KV4Cache.read: key/val rows narrower than kv_heads * head_dim");
-    if (!key || !val) return fail(AESIR_ERR_INVALID, "KV4Cache.read: null tensor pointer");
+    AESIR_TRY(pointers_ok("read", key, val));
     return guarded("read", [&]() -> int32_t {
         const bool vec = aligned16(key, key_cols) && aligned16(val, val_cols);
         std::vector<Kv4Range> r;

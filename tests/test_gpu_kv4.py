@@ -19,7 +19,7 @@ def A():
 
 @pytest.fixture(scope="module")
 def ctx(A):
-    with A.Context(1 << 30) as c:
+    with A.Context(2 << 30) as c:
         yield c
 
 
@@ -209,6 +209,35 @@ def test_attention_of_long_and_wide_batches(A, ctx, hd, nq, nkv, length, rows):
         check(got[r:r + 1], q[r:r + 1], kv4_values(k[:n]), kv4_values(v[:n]), nq, nkv, hd)
     again = attend(A, ctx, kv, 0, q)
     assert np.array_equal(got, again)  # the order of every sum is fixed
+
+
+@pytest.mark.parametrize("hd,nq,nkv,lens,new", [
+    (32, 128, 128, [3500, 1200, 3300, 700, 2600], [1, 1, 1, 1, 1]),      # equal shares that cut and join tiles of 16
+    (64, 96, 96, [3200, 3100, 1900], [1, 3, 1]),                         # a workgroup to a piece
+    (32, 256, 64, [3300, 3150, 700, 1800], [6, 5, 8, 7]),                # shares of 32-column tiles
+    (64, 128, 16, [4000, 3300, 900, 2500, 3900, 3600, 1300], [6] * 7),   # of 64-column tiles
+    (256, 16, 16, [3900, 2500, 3700, 1300, 3300, 100], [1] * 6)])
+def test_attention_cut_into_equal_shares(A, ctx, hd, nq, nkv, lens, new):
+    """More work than the workgroups that run at once take as pieces of their own: a few heads of every row."""
+    rng = np.random.default_rng(nkv)
+    ids = list(range(len(lens)))
+    kv = A.KV4Cache(ctx, 1, nq, nkv, hd, 4096, len(ids), 128, sum(-(-x // 128) for x in lens))
+    data = [rng.standard_normal((2, x, nkv * hd), dtype=np.float32).astype(np.float16) for x in lens]
+    kv.begin(ids, [x - r for x, r in zip(lens, new)])
+    mark = ctx.offset
+    kv.append(0, *(ctx.from_numpy(np.concatenate([d[j, :x - r] for d, x, r in zip(data, lens, new)])) for j in (0, 1)))
+    ctx.reset(mark)
+    kv.begin(ids, new)
+    kv.append(0, *(ctx.from_numpy(np.concatenate([d[j, x - r:] for d, x, r in zip(data, lens, new)])) for j in (0, 1)))
+    q = rand(rng, sum(new), nq * hd)
+    got = attend(A, ctx, kv, 0, q).reshape(sum(new), nkv, -1)
+    at = 0
+    for d, r in zip(data, new):
+        for h in (0, nkv // 2 + 1, nkv - 1):
+            K, V = (kv4_values(x[:, h * hd:(h + 1) * hd]) for x in d)
+            w = nq // nkv * hd
+            check(got[at:at + r, h], q[at:at + r, h * w:(h + 1) * w], K, V, nq // nkv, 1, hd)
+        at += r
 
 
 @pytest.mark.parametrize("where", ["first", "last", "middle"])
@@ -454,6 +483,41 @@ def test_pages_past_four_gigabytes(A):
             same_bits(g, kv4_values(np.concatenate([x, x])))
 
 
+def test_a_sequence_of_a_million_positions(A):
+    """More table entries and page moves than one upload holds, and attention over 1.2 million positions: zeros (a
+    fresh well) but for rows near the start, in the middle and at the end."""
+    rng = np.random.default_rng(11)
+    nq, nkv, hd, page, n = 4, 1, 32, 32, 1200000
+    pages = -(-(n + 40) // page)
+    with A.Context(A.KV4Cache.well_bytes(1, nq, nkv, hd, 2 * n, 3, page, 2 * pages) + (64 << 20)) as ctx:
+        kv = A.KV4Cache(ctx, 1, nq, nkv, hd, 2 * n, 3, page, 2 * pages)
+        K, V = np.zeros((2, n + 40, hd), np.float16)
+        for start, rows in ((0, 50), (600000, 70), (n, 40)):
+            if start > kv.length(0):
+                kv.begin([0], [start - kv.length(0)])
+            K[start:start + rows], V[start:start + rows] = rand(rng, rows, hd), rand(rng, rows, hd)
+            K[start:start + rows] *= np.float16(3)
+            kv.begin([0], [rows])
+            kv.append(0, ctx.from_numpy(K[start:start + rows]), ctx.from_numpy(V[start:start + rows]))
+        q = rand(rng, 40, nq * hd) * np.float16(2)
+        got = attend(A, ctx, kv, 0, q)
+        K, V = kv4_values(K), kv4_values(V)
+        for r in (0, 39):
+            check(got[r:r + 1], q[r:r + 1], K[:n + r + 1], V[:n + r + 1], nq, nkv, hd)
+        kv.copy(0, 1)
+        kv.truncate(0, 0)
+        assert kv.compact() == pages and max(kv.pages(1)) == pages - 1
+        kv.begin([1], [1])
+        k, v = rand(rng, 1, hd), rand(rng, 1, hd)
+        kv.append(0, ctx.from_numpy(k), ctx.from_numpy(v))
+        got = attend(A, ctx, kv, 0, q[:1])
+        check(got, q[:1], np.concatenate([K, kv4_values(k)]), np.concatenate([V, kv4_values(v)]), nq, nkv, hd)
+        at, rows = [599990, n - 5, 0], [90, 46, 60]
+        want = [np.concatenate([np.concatenate([x, kv4_values(y)])[a:a + b] for a, b in zip(at, rows)]) for x, y in ((K, k), (V, v))]
+        for g, w in zip(read(ctx, kv, 0, 1, [1] * 3, at, rows), want):
+            same_bits(g, w)
+
+
 # ------------------------------------------------------------------ capture, lifetimes, refusals
 
 class Graph:
@@ -541,6 +605,7 @@ def test_changes_are_refused_while_capturing(A, ctx):
     kv.begin([0], [1])
     calls = [lambda: kv.begin([1], [1]), lambda: kv.fork(0, 1), lambda: kv.copy(0, 1), lambda: kv.truncate(0, 0), kv.compact,
              lambda: kv.read(0, 1, [0], [0], [1], t, t)]
+    calls.append(lambda: A.KV4Cache(ctx, 1, 2, 1, 64, 64, 3, 32, 4))
     refused = []
 
     def run():
@@ -565,11 +630,14 @@ def test_refusals(A, ctx):
             call()
     kv.begin([0, 1], [2, 1])
     thin, short = ctx.tensor(3, 100), ctx.tensor(2, 256)
+    odd = A.Tensor(ctx, k.ptr + 1, 3, 128)
     for call, text in [(lambda: kv.append(2, k, k), "layer"), (lambda: kv.append(-1, k, k), "layer"), (lambda: kv.attention(2, q, q), "layer"),
                        (lambda: kv.append(0, short, k), "3 new rows"), (lambda: kv.append(0, k, short), "3 new rows"),
                        (lambda: kv.append(0, thin, k), "narrower"), (lambda: kv.append(0, k, thin), "narrower"), (lambda: kv.append(0, none, k), "null"),
                        (lambda: kv.attention(0, short, q), "3 new rows"), (lambda: kv.attention(0, q, short), "3 new rows"),
                        (lambda: kv.attention(0, k, q), "narrower"), (lambda: kv.attention(0, q, k), "narrower"), (lambda: kv.attention(0, q, none), "null"),
+                       (lambda: kv.append(0, odd, k), "2-byte"), (lambda: kv.attention(0, q, A.Tensor(ctx, q.ptr + 1, 3, 256)), "2-byte"),
+                       (lambda: kv.read(0, 1, [0, 1], [0, 0], [2, 1], k, odd), "2-byte"),
                        (lambda: kv.read(0, 3, [0], [0], [1], k, k), "layer"), (lambda: kv.read(1, 2, [0], [0], [1], k, k), "layer"),
                        (lambda: kv.read(0, 1, [3], [0], [1], k, k), "not in"), (lambda: kv.read(0, 1, [0], [1], [2], k, k), "outside"),
                        (lambda: kv.read(0, 1, [0], [-1], [1], k, k), "outside"), (lambda: kv.read(0, 1, [0], [0], [2], k, k), "2 rows"),
