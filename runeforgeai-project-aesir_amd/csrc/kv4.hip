@@ -1,5 +1,6 @@
 // The paged 4-bit KV cache: appending (quantizing) rows, attention over the pages, reading values back, page
 // copies, and the C entry points with the bookkeeping of pages and sequences.
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -1157,7 +1158,7 @@ namespace {
 
 constexpr int64_t kRingBytes = 1 << 20;
 constexpr int64_t kMaxPages = (int64_t)1 << 27;
-constexpr int64_t kPartCols = 32768;  // columns of split partials
+constexpr int64_t kPartCols = 65536;  // columns of split partials: 256 of every CU
 // How attention's work is cut, with us per call of 32 query heads of 128 over 8 KV heads, one row a sequence, unless
 // said otherwise:
 // - a workgroup to a tile where that fills the CUs and no tile is long (merges saved: 64 sequences of about 1000
@@ -1173,8 +1174,9 @@ constexpr int64_t kPartCols = 32768;  // columns of split partials
 constexpr int64_t kWholeRounds = 96, kShortRounds = 24;
 constexpr int64_t kFewRounds = 256 * 64, kFewLeast = 8;
 constexpr int64_t kGroups[3] = {768, 512, 256}, kLeast = 48;
-// Workgroups of prompts, and rounds of each at least (8 / 16 / 32: 128 rows over 2048 positions 28.1 / 34.2 / 51.7).
-constexpr int64_t kPromptGroups = 512, kPromptRounds = 8;
+// Rounds of a prompt's split at least (8 / 16 / 32: 128 rows over 2048 positions 28.1 / 34.2 / 51.7), and what a workgroup's
+// start and the merge cost, in rounds (of 1.2 us).
+constexpr int64_t kPromptRounds = 8, kPromptStart = 3, kPromptMerge = 5;
 // Rounds of all tiles up to which 16-column tiles, which work side by side, beat the tile that holds all columns of a
 // sequence and reads its keys once (one sequence of 2048 positions, 16 rows: 10.0 against 15.7 with 64 columns, 4.0 K
 // rounds of 8000 positions 16.5 / 15.0 with 32), and up to which 32-column tiles beat the prompts' (128 rows of 2048
@@ -1400,6 +1402,11 @@ void make_plan(const aesir_kv4 *kv, int p, std::vector<Kv4Seq> &ds, const std::v
     auto tiles = [&](const Kv4Seq &s) -> int64_t {
         return all || classes[(size_t)(&s - ds.data())] == v ? (s.rows * G + W - 1) / W : 0;
     };
+    *out = Kv4Plan{};
+    if (!all && !std::count(classes.begin(), classes.end(), v)) {
+        for (Kv4Seq &s : ds) s.plan[p] = {0, 0, 1, 0};
+        return;
+    }
     int shift = 0;
     auto rounds = [&](const Kv4Seq &s) { return (((int64_t)s.length + kKeys - 1) / kKeys + (1 << shift) - 1) >> shift; };
     auto all_work = [&] {
@@ -1408,24 +1415,36 @@ void make_plan(const aesir_kv4 *kv, int p, std::vector<Kv4Seq> &ds, const std::v
         return w;
     };
     int64_t work = all_work(), most = 1;
-    *out = Kv4Plan{};
-    if (v == 3) {  // equal splits of every tile
-        int64_t chunk = std::max<int64_t>(kPromptRounds, (work * kv->nkv + kPromptGroups - 1) / kPromptGroups);
-        for (;; chunk *= 2) {
+    if (v == 3) {  // equal splits of every tile: as many as make the workgroups that run one after the other on a CU shortest
+        int64_t longest = 1, chunk = 0, best = INT64_MAX;
+        for (const Kv4Seq &s : ds)
+            if (tiles(s)) longest = std::max(longest, rounds(s));
+        auto splits = [&](const Kv4Seq &s, int64_t c) { return tiles(s) ? (rounds(s) + c - 1) / c : 0; };
+        for (int64_t n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+            if (n > 1 && longest / n < kPromptRounds) break;
+            const int64_t c = (longest + n - 1) / n;
             int64_t units = 0, parts = 0;
-            most = 1;
-            for (Kv4Seq &s : ds) {
-                const int64_t n = tiles(s) ? std::max<int64_t>(1, (rounds(s) + chunk - 1) / chunk) : 0;
-                s.plan[p] = {(int32_t)units, (int32_t)n, (int32_t)parts, 0};
-                units += tiles(s) * n;
-                if (n > 1) parts += tiles(s) * n;
-                most = std::max(most, n);
+            for (const Kv4Seq &s : ds) {
+                units += tiles(s) * splits(s, c);
+                if (splits(s, c) > 1) parts += tiles(s) * splits(s, c);
             }
-            if (parts * kv->nkv * W > kPartCols) continue;  // ends: one split needs no partials
-            out->groups = units;
-            out->splits = most;
-            return;
+            const int64_t cost = (units * kv->nkv + 255) / 256 * (c + kPromptStart) + (parts ? kPromptMerge : 0);
+            if (parts * kv->nkv * W <= kPartCols && cost < best) {  // (n of 1 has none)
+                best = cost;
+                chunk = c;
+            }
         }
+        int64_t units = 0, parts = 0;
+        for (Kv4Seq &s : ds) {
+            const int64_t n = splits(s, chunk);
+            s.plan[p] = {(int32_t)units, (int32_t)n, (int32_t)parts, 0};
+            units += tiles(s) * n;
+            if (n > 1) parts += tiles(s) * n;
+            most = std::max(most, n);
+        }
+        out->groups = units;
+        out->splits = most;
+        return;
     }
     for (; work > INT32_MAX / 4; work = all_work()) shift++;  // ends: rows, and so tiles, are fewer
     int64_t longest = 0, count = 0;
