@@ -79,7 +79,7 @@ constexpr int kMaxSeqs = 4096;
 // minimum and maximum they exchange by DPP. Four consecutive rows of one head are neighbouring lane groups, so a
 // V tile of four positions leaves as one contiguous store. The quantization is exact: scales and levels are the
 // nearest ones of the real quotients, ties to even, as their definition says. Bound by instructions (some 20 an element of
-// scales, levels and packing): 8192 rows of 8 heads of 128, 13.8 us for 44 MB; one row by the launch and two reads, 2.7 us.
+// scales, levels and packing): 8192 rows of 8 heads of 128, 13.4 us for 44 MB; one row by the launch and two reads, 3.4 us.
 
 // The f16 nearest a double (ties to even): through f32 rounded to odd, so the second rounding decides alone.
 __device__ __forceinline__ h16 nearest_half(double x) {
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(Kv4Dev c, Kv4Appen
 // ------------------------------------------------------------------ read
 //
 // The f16 values of position ranges, one thread per 8 dims of K and V. Bound by memory: 2000 positions of 32 layers and 8
-// heads of 128 (344 MB with what it writes) 70 us, 4.9 TB/s.
+// heads of 128 (344 MB with what it writes) 63 us, 5.5 TB/s.
 struct Kv4ReadArgs {
     h16 *k, *v;
     int64_t k_stride, v_stride;
@@ -304,8 +304,8 @@ __global__ __launch_bounds__(kThreads) void kv4_copy_kernel(char *pool, int64_t 
 // sequence and KV head, or a piece of its rounds of 32 keys, or pieces of several; its four or eight waves take the rounds in
 // turn, each for all columns (a key is unpacked by one wave, once a tile), and meet in LDS at the end; a tile's
 // pieces meet in kv4_merge_kernel. Bound by memory where there is much to read: 64 sequences of about 4096 positions, 8 KV
-// heads of 128 (335 MB), 62 us and 5 for the merge, 5.4 TB/s; else by the chain of reads that a workgroup starts
-// with (records, page ids, the first round) and the launches: 4.2 us for 100 positions.
+// heads of 128 (335 MB), 63 us and 5 for the merge, 5.3 TB/s; else by the chain of reads that a workgroup starts
+// with (records, page ids, the first round) and the launches: 4.5 us for 100 positions.
 //
 //   scores   S^T = K q^T: a 16-key tile's A operand is unpacked nibbles; lane (i, g) holds key 8 (i / 4) + 4 t + i % 4
 //            of the round (t = 0, 1) and the hd / 4 dims from g hd / 4, so one load brings its part of the row
@@ -803,7 +803,7 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
 // and values between them, each operand once, into LDS in the order in which the matrix instructions take them (1 KB an
 // operand, 16 bytes a lane, no bank conflicts); every wave then runs those rounds over its own columns, so unpacking costs
 // an eighth a column and the waves never meet but at the barrier between stages. Two stages of LDS: the next is loaded
-// during one and unpacked behind it. 2048 rows of 8192 positions (32 query heads of 128, 8 KV heads): 296 us, 813 TFLOP/s;
+// during one and unpacked behind it. 2048 rows of 8192 positions (32 query heads of 128, 8 KV heads): 300 us, 800 TFLOP/s;
 // two waves to a SIMD issue vector instructions half of the time and matrix instructions a third, mostly not at once
 // (raising the priority of either phase, or sums as a product with ones, changed nothing: 296 - 310 us).
 template <int HD>
