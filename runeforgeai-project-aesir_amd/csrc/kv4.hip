@@ -653,8 +653,10 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
     if (chunk == kNone) return;  // no batch
     // Workgroup b of a KV head takes steps b chunk .. (b + 1) chunk - 1 of the batch's tiles one behind the other, in
     // pieces that end where a tile does. (A step is a round, or 2^shift of them in batches of billions of rounds.)
+    // A captured grid may be larger than a later batch's: its starts can pass 32 bits. 2^30 is behind every last step.
+    auto start = [&](unsigned x) { return (int)min((int64_t)(x / (unsigned)c.nkv) * chunk, (int64_t)1 << 30); };
     unsigned u = blockIdx.x;
-    int at = (int)(u / (unsigned)c.nkv) * chunk, end = at + chunk;
+    int at = start(u), end = at + chunk;
     for (;;) {
         const int kvh = (int)(u % (unsigned)c.nkv), b = (int)(u / (unsigned)c.nkv);
         const Kv4Found s = find_seq(records, c.seqs, a.plan, at, false, lane);
@@ -792,7 +794,7 @@ __global__ __launch_bounds__(NW *kWave, NC == 1 && HD <= 128 && NW == 4 ? 3 : 1)
         if (done) {
             if (a.plan < kKv4Widths) break;  // the grid is the batch's own
             u += gridDim.x;
-            at = (int)(u / (unsigned)c.nkv) * chunk;
+            at = start(u);
             end = at + chunk;
         }
         records = Kv4Records(c.seqs, a.plan, lane);

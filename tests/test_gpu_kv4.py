@@ -599,6 +599,43 @@ def test_a_captured_step_serves_later_batches(A, ctx, rows):
     g.close()
 
 
+def test_a_capture_of_many_sequences_serves_long_ones(A):
+    """A grid of 4096 workgroups a KV head, replayed for 4096 forks of a long sequence: 700 K rounds to a workgroup, so the
+    starts of those that have no work lie past 32 bits."""
+    rng = np.random.default_rng(12)
+    nkv, hd, page, seqs, n = 256, 32, 32, 4096, 16384
+    sizes = (1, nkv, nkv, hd, n + page, seqs, page, n // page + seqs)
+    with A.Context(A.KV4Cache.well_bytes(*sizes) + (512 << 20)) as ctx:
+        kv = A.KV4Cache(ctx, *sizes)
+        ids, new = list(range(seqs)), [1] * seqs
+        k, v, q, out = (ctx.tensor(seqs, nkv * hd) for _ in range(4))
+        kv.begin(ids, new)
+        g = Graph(A, ctx, lambda: (kv.append(0, k, v), kv.attention(0, q, out)))
+        for i in ids:
+            kv.truncate(i, 0)
+        K, V = np.zeros((2, n, nkv * hd), np.float16)  # a fresh well
+        kv.begin([0], [n - 64])
+        K[-64:], V[-64:] = rand(rng, 64, nkv * hd) * np.float16(3), rand(rng, 64, nkv * hd)
+        kv.begin([0], [64])
+        kv.append(0, ctx.from_numpy(K[-64:]), ctx.from_numpy(V[-64:]))
+        for i in ids[1:]:
+            kv.fork(0, i)
+        x = [rand(rng, seqs, nkv * hd) for _ in range(3)]
+        for t, y in zip((k, v, q), x):
+            t.upload(y)
+        kv.begin(ids, new)
+        for _ in range(2):
+            out.upload(np.full((seqs, nkv * hd), 9.0, np.float16))
+            g.launch()
+            got = out.numpy().astype(np.float64)
+            for r in (0, 1365, 1366, 4095):
+                for h in (0, 100, 255):
+                    c = slice(h * hd, (h + 1) * hd)
+                    have = [kv4_values(np.concatenate([a[:, c], b[r:r + 1, c]])) for a, b in zip((K, V), x)]
+                    check(got[r:r + 1, c], x[2][r:r + 1, c], *have, 1, 1, hd)
+        g.close()
+
+
 def test_changes_are_refused_while_capturing(A, ctx):
     kv = A.KV4Cache(ctx, 1, 2, 1, 64, 64, 3, 32, 4)
     t = ctx.tensor(1, 128)
