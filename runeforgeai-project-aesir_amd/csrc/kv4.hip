@@ -331,6 +331,7 @@ struct Kv4AttnArgs {
 };
 
 constexpr int kMergeWaves = 4;
+constexpr int64_t kMergeGrid = 1 << 22;  // workgroups at most: a launch holds under 2^32 threads
 
 // Masks and exponents of the unpacking, one in a scalar and one in a vector register: as literals each pair would
 // take an AND and an OR, since one instruction takes no two literals here.
@@ -1011,85 +1012,88 @@ __global__ __launch_bounds__(kMergeWaves *kWave) void kv4_merge_kernel(Kv4Dev c,
     __shared__ float ox[kMergeWaves][HD], mx[kMergeWaves], lx[kMergeWaves];
     const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all % MW;
     const int G = c.nq / c.nkv;
-    const unsigned u = blockIdx.x * (kMergeWaves / MW) + all / MW;
-    const int row = (int)(u / (unsigned)c.nq), head = (int)(u % (unsigned)c.nq);
-    const Kv4Found s = find_seq(Kv4Records(c.seqs, a.plan, lane), c.seqs, a.plan, row, true, lane);
-    // (MW of 4: uniform over the workgroup; MW of 1: no barrier follows)
-    if (row >= a.rows || row - s.row0 >= s.rows || s.count == 0) return;
-    const int col = (row - s.row0) * G + head % G, tile = col / W;
-    int first, splits, start = 0;  // partial slots: first, then start + 2 x (width 3: first + x)
-    if constexpr (V < 3) {
-        const int steps = s.tile_steps(), from = s.first + tile * steps;
-        const int b0 = from / s.chunk;
-        splits = (from + steps - 1) / s.chunk - b0 + 1;
-        first = 2 * b0 + (from % s.chunk ? 1 : 0);
-        start = 2 * b0;
-    } else {
-        splits = s.count;
-        first = s.chunk + ((s.rows * G + W - 1) / W - 1 - tile) * splits;
-    }
-    if (splits <= 1) return;
-    auto slot = [&](int x) {
-        const int p = V == 3 ? first + x : x == 0 ? first : start + 2 * x;
-        return ((int64_t)p * c.nkv + head / G) * W + col % W;
-    };
-    const int dim = HD >= kWave ? lane * D : lane % HD;
-    float M = -INFINITY, L = 0.0f, o[D] = {};
-    for (int base = 0; base < splits; base += MW * B) {
-        float p[B][D];
-        float2 e[B];
-#pragma unroll
-        for (int j = 0; j < B; j++) {
-            const int64_t at = slot(min(base + wave + MW * j, splits - 1));
-            e[j] = *reinterpret_cast<const float2 *>(c.part_ml + 2 * at);
-            __builtin_memcpy(p[j], __builtin_assume_aligned(c.part + at * HD + dim, 4 * D < 16 ? 4 * D : 16), sizeof p[j]);
+    const unsigned columns = (unsigned)a.rows * (unsigned)c.nq;
+    for (unsigned u = blockIdx.x * (kMergeWaves / MW) + all / MW; u < columns; u += gridDim.x * (kMergeWaves / MW)) {
+        const int row = (int)(u / (unsigned)c.nq), head = (int)(u % (unsigned)c.nq);
+        const Kv4Found s = find_seq(Kv4Records(c.seqs, a.plan, lane), c.seqs, a.plan, row, true, lane);
+        // (MW of 4: uniform over the workgroup; MW of 1: no barrier follows)
+        if (row - s.row0 >= s.rows || s.count == 0) continue;
+        const int col = (row - s.row0) * G + head % G, tile = col / W;
+        int first, splits, start = 0;  // partial slots: first, then start + 2 x (width 3: first + x)
+        if constexpr (V < 3) {
+            const int steps = s.tile_steps(), from = s.first + tile * steps;
+            const int b0 = from / s.chunk;
+            splits = (from + steps - 1) / s.chunk - b0 + 1;
+            first = 2 * b0 + (from % s.chunk ? 1 : 0);
+            start = 2 * b0;
+        } else {
+            splits = s.count;
+            first = s.chunk + ((s.rows * G + W - 1) / W - 1 - tile) * splits;
         }
-        float up = M;
+        if (splits <= 1) continue;
+        auto slot = [&](int x) {
+            const int p = V == 3 ? first + x : x == 0 ? first : start + 2 * x;
+            return ((int64_t)p * c.nkv + head / G) * W + col % W;
+        };
+        const int dim = HD >= kWave ? lane * D : lane % HD;
+        float M = -INFINITY, L = 0.0f, o[D] = {};
+        for (int base = 0; base < splits; base += MW * B) {
+            float p[B][D];
+            float2 e[B];
 #pragma unroll
-        for (int j = 0; j < B; j++) up = fmaxf(up, e[j].x);  // (the last one again where there are fewer)
-        const float ref = up == -INFINITY ? 0.0f : up, al = __builtin_amdgcn_exp2f((M - ref) * a.scale);
-        L *= al;
+            for (int j = 0; j < B; j++) {
+                const int64_t at = slot(min(base + wave + MW * j, splits - 1));
+                e[j] = *reinterpret_cast<const float2 *>(c.part_ml + 2 * at);
+                __builtin_memcpy(p[j], __builtin_assume_aligned(c.part + at * HD + dim, 4 * D < 16 ? 4 * D : 16), sizeof p[j]);
+            }
+            float up = M;
 #pragma unroll
-        for (int d = 0; d < D; d++) o[d] *= al;
+            for (int j = 0; j < B; j++) up = fmaxf(up, e[j].x);  // (the last one again where there are fewer)
+            const float ref = up == -INFINITY ? 0.0f : up, al = __builtin_amdgcn_exp2f((M - ref) * a.scale);
+            L *= al;
 #pragma unroll
-        for (int j = 0; j < B; j++) {
-            if (base + wave + MW * j >= splits) break;
-            const float w = __builtin_amdgcn_exp2f((e[j].x - ref) * a.scale);
-            L += w * e[j].y;
+            for (int d = 0; d < D; d++) o[d] *= al;
 #pragma unroll
-            for (int d = 0; d < D; d++) o[d] += w * p[j][d];
+            for (int j = 0; j < B; j++) {
+                if (base + wave + MW * j >= splits) break;
+                const float w = __builtin_amdgcn_exp2f((e[j].x - ref) * a.scale);
+                L += w * e[j].y;
+#pragma unroll
+                for (int d = 0; d < D; d++) o[d] += w * p[j][d];
+            }
+            M = up;
         }
-        M = up;
-    }
-    if constexpr (MW == 1) {
+        if constexpr (MW == 1) {
+            if (HD >= kWave || lane < HD) {
+#pragma unroll
+                for (int d = 0; d < D; d++) a.out[(int64_t)row * a.out_stride + head * HD + dim + d] = (h16)(o[d] / L);
+            }
+            continue;
+        }
         if (HD >= kWave || lane < HD) {
 #pragma unroll
-            for (int d = 0; d < D; d++) a.out[(int64_t)row * a.out_stride + head * HD + dim + d] = (h16)(o[d] / L);
+            for (int d = 0; d < D; d++) ox[wave][dim + d] = o[d];
         }
-        return;
-    }
-    if (HD >= kWave || lane < HD) {
-#pragma unroll
-        for (int d = 0; d < D; d++) ox[wave][dim + d] = o[d];
-    }
-    if (lane == 0) {
-        mx[wave] = M;
-        lx[wave] = L;
-    }
-    __syncthreads();
-    float up = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kMergeWaves; w++) up = fmaxf(up, mx[w]);
-    const float ref = up == -INFINITY ? 0.0f : up;
-    for (int d = threadIdx.x; d < HD; d += kMergeWaves * kWave) {
-        float x = 0.0f, l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kMergeWaves; w++) {
-            const float z = __builtin_amdgcn_exp2f((mx[w] - ref) * a.scale);
-            x += z * ox[w][d];
-            l += z * lx[w];
+        if (lane == 0) {
+            mx[wave] = M;
+            lx[wave] = L;
         }
-        a.out[(int64_t)row * a.out_stride + head * HD + d] = (h16)(x / l);
+        __syncthreads();
+        float up = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kMergeWaves; w++) up = fmaxf(up, mx[w]);
+        const float ref = up == -INFINITY ? 0.0f : up;
+        for (int d = threadIdx.x; d < HD; d += kMergeWaves * kWave) {
+            float x = 0.0f, l = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kMergeWaves; w++) {
+                const float z = __builtin_amdgcn_exp2f((mx[w] - ref) * a.scale);
+                x += z * ox[w][d];
+                l += z * lx[w];
+            }
+            a.out[(int64_t)row * a.out_stride + head * HD + d] = (h16)(x / l);
+        }
+        __syncthreads();  // ox, mx and lx are rewritten
     }
 }
 
@@ -1113,9 +1117,9 @@ int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, 
     // a wave for a row and head with few partials, four with many (47: 16.5 -> 14.4 us in all; 12 of 40 rows: 16.3, 19.1 with four);
     // a captured call may meet a batch that is split, whatever this one is
     if (captured || p.splits > 16)
-        hipLaunchKernelGGL((kv4_merge_kernel<HD, V, kMergeWaves>), dim3((unsigned)columns), dim3(kMergeWaves * kWave), 0, st, c, a);
+        hipLaunchKernelGGL((kv4_merge_kernel<HD, V, kMergeWaves>), dim3((unsigned)std::min(columns, kMergeGrid)), dim3(kMergeWaves * kWave), 0, st, c, a);
     else if (p.splits > 1)
-        hipLaunchKernelGGL((kv4_merge_kernel<HD, V, 1>), dim3((unsigned)((columns + kMergeWaves - 1) / kMergeWaves)),
+        hipLaunchKernelGGL((kv4_merge_kernel<HD, V, 1>), dim3((unsigned)std::min((columns + kMergeWaves - 1) / kMergeWaves, kMergeGrid)),
                            dim3(kMergeWaves * kWave), 0, st, c, a);
     AESIR_LAUNCH_CHECK("kv4_merge_kernel");
     return AESIR_OK;

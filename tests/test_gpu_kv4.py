@@ -518,6 +518,34 @@ def test_a_sequence_of_a_million_positions(A):
             same_bits(g, w)
 
 
+def test_a_merge_of_more_heads_and_rows_than_a_launch_holds(A):
+    """A split row among prompts of 17 M rows and query heads in all."""
+    rng = np.random.default_rng(13)
+    nq, nkv, hd, page, prompts, rows, n = 64, 8, 32, 32, 4095, 65, 32768
+    sizes = (1, nq, nkv, hd, n + page, prompts + 1, page, n // page + 1 + 3 * prompts)
+    total = prompts * rows + 1
+    assert total * nq > 1 << 24
+    with A.Context(A.KV4Cache.well_bytes(*sizes) + 2 * total * (nq + nkv) * hd * 2 + (64 << 20)) as ctx:
+        kv = A.KV4Cache(ctx, *sizes)
+        K, V = np.zeros((2, n, nkv * hd), np.float16)  # a fresh well
+        kv.begin([0], [n - 64])
+        K[-64:], V[-64:] = rand(rng, 64, nkv * hd) * np.float16(3), rand(rng, 64, nkv * hd)
+        kv.begin([0], [64])
+        kv.append(0, ctx.from_numpy(K[-64:]), ctx.from_numpy(V[-64:]))
+        # prompts repeat every 16 sequences
+        k, v, q = (np.resize(rand(rng, 16 * rows, w * hd), (total, w * hd)) for w in (nkv, nkv, nq))
+        kv.begin([*range(1, prompts + 1), 0], [rows] * prompts + [1])
+        out = ctx.tensor(total, nq * hd)
+        kv.append(0, ctx.from_numpy(k), ctx.from_numpy(v))
+        kv.attention(0, ctx.from_numpy(q), out)
+        got = out.numpy()
+        have = [kv4_values(np.concatenate([a, b[-1:]])) for a, b in ((K, k), (V, v))]
+        check(got[-1:].astype(np.float64), q[-1:], *have, nq, nkv, hd)
+        for i in (0, 1000, prompts - 1):
+            c = slice(i * rows, (i + 1) * rows)
+            check(got[c].astype(np.float64), q[c], kv4_values(k[c]), kv4_values(v[c]), nq, nkv, hd)
+
+
 # ------------------------------------------------------------------ capture, lifetimes, refusals
 
 class Graph:
