@@ -293,8 +293,8 @@ int32_t aesir_kv_v_slice(const aesir_kv *kv, int64_t layer_idx, int64_t seq_len,
 int64_t aesir_kv4_well_bytes(int64_t num_layers, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
                              int64_t max_seq_len, int64_t max_seqs, int64_t page_size, int64_t num_pages);
 /* A cache of num_pages pages of page_size positions (a power of two, 32 to 1024), for sequences 0 ..
- * max_seqs - 1 (at most 4096) of up to max_seq_len positions; head_dim 32, 64, 128 or 256, n_heads query
- * heads a multiple of n_kv_heads. Its memory is taken from the context's well. ctx may be NULL: such a cache keeps the
+ * max_seqs - 1 (at most 4096, and 2^22 with the KV heads counted) of up to max_seq_len positions; head_dim 32, 64, 128
+ * or 256, n_heads query heads a multiple of n_kv_heads. Its memory is taken from the context's well. ctx may be NULL: such a cache keeps the
  * tables only (begin, fork, copy, truncate, compact and the queries work, for planning without a GPU). */
 int32_t aesir_kv4_create(aesir_ctx *ctx, int64_t num_layers, int64_t n_heads, int64_t n_kv_heads,
                          int64_t head_dim, int64_t max_seq_len, int64_t max_seqs, int64_t page_size,

@@ -1105,7 +1105,7 @@ struct Kv4Plan {
 
 template <int HD, int V>
 int32_t launch_attention(hipStream_t st, const Kv4Dev &c, const Kv4AttnArgs &a, const Kv4Plan &p, bool captured) {
-    const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>(p.groups * c.nkv, 1), 1 << 30));
+    const dim3 grid((unsigned)std::max<int64_t>(p.groups * c.nkv, 1));
     if constexpr (V == 3)
         hipLaunchKernelGGL(kv4_prompt_kernel<HD>, grid, dim3(8 * kWave), 0, st, c, a);
     else if (p.waves == 8)
@@ -1213,6 +1213,8 @@ int32_t kv4_sizes(int64_t layers, int64_t nq, int64_t nkv, int64_t hd, int64_t m
     if (max_seqs > kMaxSeqs) return fail(AESIR_ERR_UNSUPPORTED, "KV4Cache: more than %d sequences", kMaxSeqs);
     if (max_seq_len > INT32_MAX / 2 || pages > kMaxPages || nq > 65535 || layers > 65535)
         return fail(AESIR_ERR_UNSUPPORTED, "KV4Cache: a dimension is too large");
+    // a workgroup or more of 512 threads to a sequence and KV head; a launch holds under 2^32 threads
+    if (max_seqs * nkv > 1 << 22) return fail(AESIR_ERR_UNSUPPORTED, "KV4Cache: a dimension is too large");
     const int64_t stride = (max_seq_len + page - 1) / page;
     if (mul_checked(stride, max_seqs) > INT32_MAX) return fail(AESIR_ERR_UNSUPPORTED, "KV4Cache: a dimension is too large");
     z->page_bytes = mul_checked(mul_checked(layers, nkv, page), hd / 4 * 5);

@@ -128,6 +128,12 @@ def test_sizes_are_checked(A):
         A.KV4Cache.well_bytes(3, 8, 4, 100, 300, 6, 64, 12)
 
 
+def test_sequences_times_heads_have_a_limit(A):
+    with pytest.raises(A.AesirError, match="too large"):
+        cache(A, seqs=4096, n_heads=1025, n_kv_heads=1025)
+    assert cache(A, seqs=4096, n_heads=1024, n_kv_heads=1024).free_pages > 0
+
+
 def test_without_a_context_there_is_no_data(A):
     kv = cache(A)
     kv.begin([0], [1])
