@@ -410,6 +410,8 @@ class KV4Cache:
     def __init__(self, ctx, num_layers: int, n_heads: int, n_kv_heads: int, head_dim: int, max_seq_len: int, max_seqs: int,
                  page_size: int, num_pages: int):
         self.h = None
+        if ctx is not None and not ctx.h:
+            raise AesirError(-1, "KV4Cache: the context is closed")
         h = P()
         _check(_L.aesir_kv4_create(ctx.h if ctx is not None else None, num_layers, n_heads, n_kv_heads, head_dim, max_seq_len,
                                    max_seqs, page_size, num_pages, C.byref(h)))

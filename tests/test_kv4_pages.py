@@ -143,6 +143,14 @@ def test_without_a_context_there_is_no_data(A):
             call()
 
 
+def test_a_closed_context_is_not_no_context(A):
+    class Closed:
+        h = None
+
+    with pytest.raises(A.AesirError, match="closed"):
+        A.KV4Cache(Closed(), 1, 2, 1, 64, 64, 3, 32, 4)
+
+
 def test_null_handles_are_refused(A):
     L = A._L
     assert L.aesir_kv4_begin(None, None, None, 0) == -1
