@@ -299,7 +299,7 @@ int64_t aesir_kv4_well_bytes(int64_t num_layers, int64_t n_heads, int64_t n_kv_h
 int32_t aesir_kv4_create(aesir_ctx *ctx, int64_t num_layers, int64_t n_heads, int64_t n_kv_heads,
                          int64_t head_dim, int64_t max_seq_len, int64_t max_seqs, int64_t page_size,
                          int64_t num_pages, aesir_kv4 **out);
-/* Frees the descriptor (waiting for the stream); the pages' memory belongs to the well. */
+/* Frees the descriptor (waiting for the stream, so not while it is captured); the pages' memory belongs to the well. */
 int32_t aesir_kv4_destroy(aesir_kv4 *kv);
 /* Bytes of one page (all layers), free pages, and positions of a sequence; -1 for a bad argument. */
 int64_t aesir_kv4_page_bytes(const aesir_kv4 *kv);

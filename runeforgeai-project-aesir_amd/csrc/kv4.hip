@@ -1628,7 +1628,7 @@ int32_t aesir_kv4_create(aesir_ctx *ctx, int64_t num_layers, int64_t n_heads, in
 int32_t aesir_kv4_destroy(aesir_kv4 *kv) {
     if (!kv) return AESIR_OK;
     if (kv->ctx) {
-        AESIR_TRY(bind(kv->ctx));
+        AESIR_TRY(not_captured(kv->ctx, "destroy"));
         (void)hipStreamSynchronize(kv->ctx->stream);  // launches may still read the staging memory
         (void)hipHostFree(kv->ring);
         kv->ctx->live_caches--;

@@ -686,6 +686,21 @@ def test_changes_are_refused_while_capturing(A, ctx):
     g.close()
 
 
+def test_destroy_waits_for_the_end_of_a_capture(A, ctx):
+    kv, other = (A.KV4Cache(ctx, 1, 2, 1, 64, 64, 3, 32, 4) for _ in range(2))
+    t = ctx.tensor(1, 128)
+    kv.begin([0], [1])
+
+    def run():
+        with pytest.raises(A.AesirError, match="captured"):
+            other.close()
+        kv.append(0, t, t)
+
+    Graph(A, ctx, run).close()
+    other.close()
+    assert other.h is None
+
+
 def test_refusals(A, ctx):
     kv = A.KV4Cache(ctx, 2, 4, 2, 64, 64, 3, 32, 6)
     k, q = ctx.tensor(3, 128), ctx.tensor(3, 256)
