@@ -762,3 +762,38 @@ def test_lifetimes(A):
         same_bits(g, kv4_values(x))
     ctx.close()  # closes b first
     assert b.h is None
+
+
+# ------------------------------------------------------------------ weights
+
+def half_weights(hd, q_rows, heads):
+    """Query rows whose score against a key of ones is d above that of a key of zeros, e^-d = (1 + 2^-11 + 2^-13) / 2: a weight
+    that f16 rounds up by 2^-11 - 2^-13 of itself."""
+    total = -np.log(0.5 * (1 + 2.0 ** -11 + 2.0 ** -13)) * np.sqrt(hd)
+    q = np.full(hd, total / hd).astype(np.float16)
+    q[0] = np.float16(float(q[0]) + total - q.astype(np.float64).sum())
+    got = 2 * np.exp(-q.astype(np.float64).sum() / np.sqrt(hd)) - 1
+    assert 2.0 ** -11 + 2.0 ** -14 < got < 2.0 ** -10
+    return np.tile(q, (q_rows, heads))
+
+
+@pytest.mark.parametrize("hd,nq,nkv,length,rows", [(128, 4, 1, 4096, 1), (64, 32, 8, 8192, 8), (64, 32, 8, 8192, 16), (32, 32, 8, 8192, 128),
+                                                   (64, 32, 8, 8192, 128), (128, 32, 8, 8192, 128), (256, 4, 4, 2000, 1), (256, 16, 4, 4096, 64)])
+@pytest.mark.parametrize("value", [65504.0, -65504.0, 1.5])
+def test_weights_sum_to_one(A, ctx, hd, nq, nkv, length, rows, value):
+    """Equal values come out as they are, the largest f16 among them, where 31 of 32 weights round the same way (each wave
+    meets a key of weight one in each round of 32, so that its maximum is that key's). A lane's
+    chain of sums is at most 8192 / 4 / 2 dot products of 3 * 2^-24 (and 256 matrix instructions of 2^-23): 2.2e-4 of the
+    weights' sum, under half an f16 step (2.4e-4)."""
+    kv = A.KV4Cache(ctx, 1, nq, nkv, hd, length, 1, 64, -(-length // 64))
+    k, v = np.zeros((length, nkv * hd), np.float16), np.full((length, nkv * hd), value, np.float16)
+    k[::32] = 1
+    mark = ctx.offset
+    if length > rows:
+        kv.begin([0], [length - rows])
+        kv.append(0, ctx.from_numpy(k[:-rows]), ctx.from_numpy(v[:-rows]))
+        ctx.reset(mark)
+    kv.begin([0], [rows])
+    kv.append(0, ctx.from_numpy(k[-rows:]), ctx.from_numpy(v[-rows:]))
+    got = attend(A, ctx, kv, 0, half_weights(hd, rows, nq))
+    assert (got == value).all(), (got[got != value][:5], (got != value).sum())
