@@ -319,6 +319,10 @@ int32_t aesir_kv4_append(aesir_kv4 *kv, int64_t layer, const void *key, int64_t 
  * query and output have as many rows as begin() added. The positions must have been appended. */
 int32_t aesir_kv4_attention(aesir_kv4 *kv, int64_t layer, const void *query, int64_t query_rows,
                             int64_t query_cols, void *output, int64_t output_rows, int64_t output_cols);
+/* How attention of the batch is cut, narrowest first: *n launches (0 without a batch or new rows; the first cap in
+ * the arrays), each over tiles of widths[i] (row, query head) columns, which pieces[i] workgroups share at most.
+ * captured: as a call that is being captured would launch it. */
+int32_t aesir_kv4_plan(const aesir_kv4 *kv, int32_t captured, int64_t *widths, int64_t *pieces, int64_t cap, int64_t *n);
 /* The f16 values that positions pos[i] .. pos[i] + rows[i] - 1 of sequences seqs[i] stand for, of layers
  * layer .. layer + layers - 1: row (l * sum(rows) + r) of key and val is the r-th of the ranges' rows. */
 int32_t aesir_kv4_read(aesir_kv4 *kv, int64_t layer, int64_t layers, const int64_t *seqs, const int64_t *pos,

@@ -97,6 +97,7 @@ _sig("aesir_kv4_free_pages", [P], I64)
 _sig("aesir_kv4_length", [P, I64], I64)
 _sig("aesir_kv4_pages", [P, I64, P, I64, C.POINTER(I64)])
 _sig("aesir_kv4_begin", [P, P, P, I64])
+_sig("aesir_kv4_plan", [P, I32, P, P, I64, C.POINTER(I64)])
 _sig("aesir_kv4_append", [P, I64, P, I64, I64, P, I64, I64])
 _sig("aesir_kv4_attention", [P, I64, P, I64, I64, P, I64, I64])
 _sig("aesir_kv4_read", [P, I64, I64, P, P, P, I64, P, I64, I64, P, I64, I64])
@@ -466,6 +467,13 @@ class KV4Cache:
             raise ValueError("begin: as many row counts as sequences")
         s, r = _i64s(seqs), _i64s(rows)
         _check(_L.aesir_kv4_begin(self.h, s.buffer_info()[0], r.buffer_info()[0], len(s)))
+
+    def plan(self, captured: bool = False) -> dict:
+        """How attention of the batch is cut: {columns of a tile: workgroups that share one at most}, a launch each."""
+        n = I64()
+        widths, pieces = (I64 * 4)(), (I64 * 4)()
+        _check(_L.aesir_kv4_plan(self.h, int(captured), widths, pieces, 4, C.byref(n)))
+        return dict(zip(widths[: n.value], pieces[: n.value]))
 
     def append(self, layer: int, key: Tensor, val: Tensor):
         """Stores the batch's new rows of one layer."""

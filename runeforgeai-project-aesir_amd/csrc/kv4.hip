@@ -1533,19 +1533,30 @@ int32_t kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64
         at += rows[i];
     }
     Kv4Plan plans[kKv4Plans];
-    const std::vector<int> classes = kv->ctx ? column_classes(kv, ds) : std::vector<int>();
-    if (kv->ctx)
-        for (int p = 0; p < kKv4Plans; p++) make_plan(kv, p, ds, classes, &plans[p]);
+    const std::vector<int> classes = column_classes(kv, ds);
+    for (int p = 0; p < kKv4Plans; p++) make_plan(kv, p, ds, classes, &plans[p]);
     for (int64_t i = 0; i < n; i++) kv->book.grow(seqs[i], rows[i], copies);
     std::copy(plans, plans + kKv4Plans, kv->plans);
     kv->batch = true;
     kv->batch_rows = total;
     for (bool &b : kv->in_class) b = false;
     for (int64_t i = 0; i < n; i++)
-        if (rows[i] > 0 && kv->ctx) kv->in_class[classes[(size_t)i]] = true;
+        if (rows[i] > 0) kv->in_class[classes[(size_t)i]] = true;
     if (!kv->ctx) return AESIR_OK;
     AESIR_TRY(upload(kv, seqs, n, records(kv->seqs, ds.data(), n)));
     return copy_pages(kv, copies);
+}
+
+// The plans that attention of the batch launches, n of them: one for the sequences of each class there is. A captured call
+// may meet any batch later: one launch for all sequences, as wide as its own batch's widest.
+int launched(const aesir_kv4 *kv, bool captured, int (&plans)[kKv4Widths]) {
+    int n = 0;
+    for (int v = 0; v < kKv4Widths; v++) {
+        if (!kv->batch || !kv->in_class[v]) continue;
+        if (captured) n = 0;
+        plans[n++] = captured ? v + kKv4Widths : v;
+    }
+    return n;
 }
 
 int32_t layer_ok(aesir_kv4 *kv, const char *what, int64_t layer) {
@@ -1663,6 +1674,18 @@ int32_t aesir_kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows,
     return guarded("begin", [&] { return kv4_begin(kv, seqs, rows, n); });
 }
 
+int32_t aesir_kv4_plan(const aesir_kv4 *kv, int32_t captured, int64_t *widths, int64_t *pieces, int64_t cap, int64_t *n) {
+    clear_error();
+    if (!kv || !n || cap < 0 || (cap > 0 && (!widths || !pieces))) return fail(AESIR_ERR_INVALID, "KV4Cache.plan: null argument");
+    int plans[kKv4Widths];
+    *n = launched(kv, captured != 0, plans);
+    for (int64_t i = 0; i < *n && i < cap; i++) {
+        widths[i] = kv4_width(plans[i] % kKv4Widths, (int)kv->hd);
+        pieces[i] = kv->plans[plans[i]].splits;
+    }
+    return AESIR_OK;
+}
+
 int32_t aesir_kv4_append(aesir_kv4 *kv, int64_t layer, const void *key, int64_t key_rows, int64_t key_cols, const void *val,
                          int64_t val_rows, int64_t val_cols) {
     AESIR_TRY(need_device(kv, "append"));
@@ -1698,14 +1721,11 @@ int32_t aesir_kv4_attention(aesir_kv4 *kv, int64_t layer, const void *query, int
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     AESIR_HIP_TRY(hipStreamIsCapturing(kv->ctx->stream, &st));
     const bool captured = st != hipStreamCaptureStatusNone;
-    // A launch for the sequences of each class there is. A captured call may meet any batch later: one launch for all
-    // sequences, as wide as its own batch's widest.
-    int widest = 0;
-    for (int v = 0; v < kKv4Widths; v++)
-        if (kv->in_class[v]) widest = v;
-    for (int v = captured ? widest : 0; v <= widest; v++) {
-        if (!kv->in_class[v]) continue;
-        a.plan = captured ? v + kKv4Widths : v;
+    int plans[kKv4Widths];
+    const int n = launched(kv, captured, plans);
+    for (int i = 0; i < n; i++) {
+        a.plan = plans[i];
+        const int v = a.plan % kKv4Widths;
         const Kv4Plan &p = kv->plans[a.plan];
         int32_t rc;
         switch (kv->hd) {
