@@ -310,7 +310,8 @@ int32_t aesir_kv4_pages(const aesir_kv4 *kv, int64_t seq, int64_t *pages, int64_
 
 /* Adds rows[i] >= 0 positions to sequence seqs[i] (each listed once) and makes the n sequences the batch.
  * A last page that is shared and would be written to is copied first. The lowest free pages are taken;
- * without enough of them AESIR_ERR_EXHAUSTED, and nothing has changed. */
+ * without enough of them (or of host memory) AESIR_ERR_EXHAUSTED, and nothing has changed; after AESIR_ERR_HIP the
+ * sequences are as they were and there is no batch. */
 int32_t aesir_kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64_t n);
 /* Stores the batch's new rows of one layer: key and val have as many rows as begin() added. */
 int32_t aesir_kv4_append(aesir_kv4 *kv, int64_t layer, const void *key, int64_t key_rows, int64_t key_cols,

@@ -1296,23 +1296,39 @@ int32_t launch_upload(aesir_kv4 *kv, const Run &run, const uint32_t *updates, in
     return AESIR_OK;
 }
 
-// Brings the device's table rows of the listed sequences up to date, with `run` in the last launch.
-int32_t upload(aesir_kv4 *kv, const int64_t *seqs, int64_t n, const Run &run) {
-    const int64_t most = kRingBytes / 4 / 8;
-    std::vector<uint32_t> e;
+// Table entries that go to the device with one launch at most.
+constexpr int64_t kUpdates = kRingBytes / 4 / 8;
+
+// Entries of the listed sequences that the device lacks.
+int64_t unsynced(const aesir_kv4 *kv, const int64_t *seqs, int64_t n) {
+    int64_t count = 0;
+    for (int64_t i = 0; i < n; i++) count += (int64_t)kv->book.seq(seqs[i]).pages.size() - kv->book.seq(seqs[i]).synced;
+    return count;
+}
+
+int32_t send(aesir_kv4 *kv, const int64_t *seqs, int64_t n, const Run &run, std::vector<uint32_t> &e) {
     for (int64_t i = 0; i < n; i++) {
         const PageBook::Seq &s = kv->book.seq(seqs[i]);
         for (int64_t j = s.synced; j < (int64_t)s.pages.size(); j++) {
             e.push_back((uint32_t)(seqs[i] * kv->dev.table_stride + j));
             e.push_back((uint32_t)s.pages[(size_t)j]);
-            if ((int64_t)e.size() == 2 * most) {
-                AESIR_TRY(launch_upload(kv, Run{}, e.data(), most));
+            if ((int64_t)e.size() == 2 * kUpdates) {
+                AESIR_TRY(launch_upload(kv, Run{}, e.data(), kUpdates));
                 e.clear();
             }
         }
-        kv->book.mark_synced(seqs[i]);
+        kv->book.mark_synced(seqs[i]);  // (a sequence may be listed again)
     }
     return launch_upload(kv, run, e.data(), (int64_t)e.size() / 2);
+}
+
+// Brings the device's table rows of the listed sequences up to date, with `run` in the last launch; after a failure all of
+// them are sent again. e: empty, with room for the entries (or for kUpdates).
+int32_t upload(aesir_kv4 *kv, const int64_t *seqs, int64_t n, const Run &run, std::vector<uint32_t> &e) {
+    const int32_t rc = send(kv, seqs, n, run, e);
+    if (rc != AESIR_OK)
+        for (int64_t i = 0; i < n; i++) kv->book.mark_unsynced(seqs[i]);
+    return rc;
 }
 
 // n records and, behind them, at least one and up to a multiple of 64 of kNone.
@@ -1518,10 +1534,18 @@ int32_t kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64
     if (need > kv->book.free_pages())
         return fail(AESIR_ERR_EXHAUSTED, "KV4Cache.begin: %lld pages needed, %lld free", (long long)need,
                     (long long)kv->book.free_pages());
+    // All memory first: nothing fails between the tables' change and the launches.
     std::vector<PageMove> copies;
     std::vector<Kv4Seq> ds((size_t)n);
+    std::vector<uint32_t> entries;
     copies.reserve((size_t)n);
-    for (int64_t i = 0; i < n; i++) kv->book.reserve(seqs[i], kv->book.seq(seqs[i]).length + rows[i]);
+    int64_t most = 0;
+    for (int64_t i = 0; i < n; i++) {
+        const PageBook::Seq &s = kv->book.seq(seqs[i]);
+        kv->book.reserve(seqs[i], s.length + rows[i]);
+        most += kv->book.pages_for(s.length + rows[i]) - s.synced + 1;  // one more: a last page that is copied
+    }
+    entries.reserve((size_t)(2 * std::min(most, kUpdates)));
     int64_t at = 0;
     for (int64_t i = 0; i < n; i++) {
         Kv4Seq &s = ds[(size_t)i];
@@ -1535,16 +1559,28 @@ int32_t kv4_begin(aesir_kv4 *kv, const int64_t *seqs, const int64_t *rows, int64
     Kv4Plan plans[kKv4Plans];
     const std::vector<int> classes = column_classes(kv, ds);
     for (int p = 0; p < kKv4Plans; p++) make_plan(kv, p, ds, classes, &plans[p]);
+    kv->batch = false;
     for (int64_t i = 0; i < n; i++) kv->book.grow(seqs[i], rows[i], copies);
+    if (kv->ctx) {
+        int32_t rc = copy_pages(kv, copies);
+        if (rc == AESIR_OK) rc = upload(kv, seqs, n, records(kv->seqs, ds.data(), n), entries);
+        if (rc != AESIR_OK) {
+            for (int64_t i = n - 1; i >= 0; i--) kv->book.shrink(seqs[i], rows[i], copies);
+            return rc;
+        }
+    }
     std::copy(plans, plans + kKv4Plans, kv->plans);
     kv->batch = true;
     kv->batch_rows = total;
     for (bool &b : kv->in_class) b = false;
     for (int64_t i = 0; i < n; i++)
         if (rows[i] > 0) kv->in_class[classes[(size_t)i]] = true;
-    if (!kv->ctx) return AESIR_OK;
-    AESIR_TRY(upload(kv, seqs, n, records(kv->seqs, ds.data(), n)));
-    return copy_pages(kv, copies);
+    return AESIR_OK;
+}
+
+int32_t layer_ok(aesir_kv4 *kv, const char *what, int64_t layer) {
+    if (layer < 0 || layer >= kv->layers) return fail(AESIR_ERR_INVALID, "KV4Cache.%s: layer out of bounds", what);
+    return AESIR_OK;
 }
 
 // The plans that attention of the batch launches, n of them: one for the sequences of each class there is. A captured call
@@ -1557,11 +1593,6 @@ int launched(const aesir_kv4 *kv, bool captured, int (&plans)[kKv4Widths]) {
         plans[n++] = captured ? v + kKv4Widths : v;
     }
     return n;
-}
-
-int32_t layer_ok(aesir_kv4 *kv, const char *what, int64_t layer) {
-    if (layer < 0 || layer >= kv->layers) return fail(AESIR_ERR_INVALID, "KV4Cache.%s: layer out of bounds", what);
-    return AESIR_OK;
 }
 
 }  // namespace
@@ -1774,7 +1805,9 @@ int32_t aesir_kv4_read(aesir_kv4 *kv, int64_t layer, int64_t layers, const int64
                 count += rows[i];
             }
             if (count == 0) continue;
-            AESIR_TRY(upload(kv, seqs + at, m, m == 1 ? Run{} : records(kv->ranges, r.data(), m)));
+            std::vector<uint32_t> entries;
+            entries.reserve((size_t)(2 * std::min(unsynced(kv, seqs + at, m), kUpdates)));
+            AESIR_TRY(upload(kv, seqs + at, m, m == 1 ? Run{} : records(kv->ranges, r.data(), m), entries));
             const Kv4ReadArgs a{(h16 *)key, (h16 *)val, key_cols,     val_cols,       layer,         layers,
                                 m == 1 ? nullptr : kv->ranges, (int32_t)total, (int32_t)first, r[0]};
             AESIR_KV4_ROWS(kv4_read_kernel, vec, rows_grid(kv, count, layers), kv->ctx->stream, kv->dev, a)

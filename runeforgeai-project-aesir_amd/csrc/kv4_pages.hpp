@@ -31,6 +31,7 @@ class PageBook {
     int64_t free_pages() const { return (int64_t)free_.size(); }
     int64_t pages_for(int64_t positions) const { return (positions + page_size_ - 1) / page_size_; }
     void mark_synced(int64_t s) { seqs_[(size_t)s].synced = (int64_t)seqs_[(size_t)s].pages.size(); }
+    void mark_unsynced(int64_t s) { seqs_[(size_t)s].synced = 0; }
 
     // Pages that `rows` new positions of every listed sequence take: new ones, and one per shared last page
     // that would be written to (of k sequences on one page the last keeps it, if no other sequence has it).
@@ -67,6 +68,20 @@ class PageBook {
         }
         s.length += rows;
         while ((int64_t)s.pages.size() < pages_for(s.length)) s.pages.push_back(take());
+    }
+
+    // Takes back what grow(id, rows, copies) did, in reverse order of several; copies loses the sequence's own.
+    void shrink(int64_t id, int64_t rows, std::vector<PageMove> &copies) {
+        Seq &s = seqs_[(size_t)id];
+        truncate(id, s.length - rows);
+        if (!copies.empty() && !s.pages.empty() && s.pages.back() == copies.back().dst) {
+            s.pages.back() = copies.back().src;
+            refs_[(size_t)copies.back().src]++;
+            refs_[(size_t)copies.back().dst] = 0;
+            free_.push(copies.back().dst);
+            touch(s, (int64_t)s.pages.size() - 1);
+            copies.pop_back();
+        }
     }
 
     void fork(int64_t src, int64_t dst) {

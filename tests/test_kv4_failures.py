@@ -1,0 +1,126 @@
+"""The paged 4-bit KV cache's host side when a launch or an allocation fails: run in a child process over a stand-in for the
+HIP runtime (fake_hip.cpp), so without a GPU."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+PKG = os.path.join(os.path.dirname(HERE), "runeforgeai-project-aesir_amd")
+
+START = f"""
+import ctypes as C, sys
+F = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)
+F.fake_table.restype = C.POINTER(C.c_int32)
+sys.path.insert(0, {PKG!r})
+import aesir_hip as A
+
+ctx = A.Context(64 << 20)
+
+def cache(pages=12, seqs=4, longest=320):
+    return A.KV4Cache(ctx, 1, 2, 1, 64, longest, seqs, 32, pages)
+
+def state(kv):
+    return [(kv.length(i), kv.pages(i)) for i in range(kv.max_seqs)], kv.free_pages, kv.plan()
+
+def on_device(kv, seqs):
+    stride = -(-kv.max_seq_len // 32)
+    for i in seqs:
+        got = F.fake_table()[i * stride: i * stride + len(kv.pages(i))]
+        assert got == kv.pages(i), (i, got, kv.pages(i))
+
+def failing(fail, call):
+    '''Calls with the n-th launch or allocation failing, for n from 1, until none does: the error codes.'''
+    codes = []
+    while True:
+        fail(len(codes) + 1)
+        try:
+            call()
+            fail(0)
+            return codes
+        except A.AesirError as e:
+            codes.append(e.code)
+"""
+
+
+@pytest.fixture(scope="module")
+def child(tmp_path_factory):
+    lib = str(tmp_path_factory.mktemp("fake") / "fake_hip.so")
+    subprocess.run(["g++", "-shared", "-fPIC", "-O1", "-w", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", os.path.join(HERE, "fake_hip.cpp"), "-o", lib],
+                   check=True)
+
+    def run(script):
+        r = subprocess.run([sys.executable, "-c", START + script, lib], capture_output=True, text=True, timeout=100)
+        assert r.returncode == 0, r.stdout + r.stderr
+
+    return run
+
+
+def test_the_stand_in_runs_the_tables(child):
+    child("""
+kv = cache()
+kv.begin([0], [40])
+kv.fork(0, 1)
+kv.begin([1, 0], [1, 1])
+assert kv.pages(1) == [0, 2] and kv.pages(0) == [0, 1]
+on_device(kv, [0, 1])
+""")
+
+
+@pytest.mark.parametrize("what", ["launch", "new"])
+def test_begin_that_fails_changes_nothing(child, what):
+    """Growth, new table entries and a shared page's copy, with every launch and every host allocation of it failing in turn."""
+    child(f"""
+fail, expect = (F.fake_fail_launch, -4) if {what!r} == "launch" else (F.fake_fail_new, -3)
+kv = cache()
+kv.begin([0], [40])
+kv.fork(0, 1)
+kv.fork(0, 3)          # both writers below copy the last page
+kv.begin([2], [1])
+before = state(kv)
+
+def step():
+    try:
+        kv.begin([1, 0], [1, 100])
+    except A.AesirError:
+        now = state(kv)
+        if expect == -3:  # not even the batch
+            assert now == before, (now, before)
+        else:             # there is none
+            assert now[:2] == before[:2] and now[2] == {{}}, (now, before)
+        raise
+
+codes = failing(fail, step)
+assert len(codes) >= 2 and set(codes) == {{expect}}, codes
+assert kv.length(0) == 140 and kv.length(1) == 41
+on_device(kv, [0, 1])
+""")
+
+
+def test_table_entries_of_a_failed_launch_are_sent_again(child):
+    """By begin, and by a read of sequences that no batch has sent."""
+    child("""
+kv = cache()
+kv.begin([0], [40])
+kv.copy(0, 1)          # its entries are not on the device
+k = ctx.tensor(40, 64)
+codes = failing(F.fake_fail_launch, lambda: kv.read(0, 1, [1], [0], [40], k, k))
+assert len(codes) == 2 and set(codes) == {-4}  # the entries, the read
+on_device(kv, [1])
+kv.compact()
+kv.truncate(0, 0)
+kv.compact()           # sequence 1 moves to pages 0 and 1
+assert kv.pages(1) == [0, 1]
+codes = failing(F.fake_fail_launch, lambda: kv.read(0, 1, [1, 1], [0, 20], [20, 20], k, k))
+assert len(codes) == 2
+on_device(kv, [1])
+F.fake_fail_launch(1)
+try:
+    kv.begin([1], [30])
+    assert False
+except A.AesirError:
+    pass
+kv.begin([1], [1])
+on_device(kv, [1])
+""")
