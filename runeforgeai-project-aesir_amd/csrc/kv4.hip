@@ -1843,7 +1843,9 @@ int32_t aesir_kv4_copy(aesir_kv4 *kv, int64_t src, int64_t dst) {
         AESIR_TRY(end_batch(kv));
         std::vector<PageMove> copies;
         if (src != dst) kv->book.copy(src, dst, copies);
-        return copy_pages(kv, copies);
+        const int32_t rc = copy_pages(kv, copies);
+        if (rc != AESIR_OK) kv->book.truncate(dst, 0);
+        return rc;
     });
 }
 

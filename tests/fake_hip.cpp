@@ -109,7 +109,7 @@ hipError_t hipGetDevicePropertiesR0600(hipDeviceProp_tR0600 *p, int) {
 }
 #undef hipMalloc
 #undef hipHostMalloc
-hipError_t hipMalloc(void **p, size_t n) { return (*p = std::malloc(n)) ? hipSuccess : hipErrorOutOfMemory; }
+hipError_t hipMalloc(void **p, size_t n) { return (*p = std::aligned_alloc(4096, (n + 4095) / 4096 * 4096)) ? hipSuccess : hipErrorOutOfMemory; }
 hipError_t hipFree(void *p) { return std::free(p), hipSuccess; }
 hipError_t hipHostMalloc(void **p, size_t n, unsigned) { return hipMalloc(p, n); }
 hipError_t hipHostFree(void *p) { return hipFree(p); }

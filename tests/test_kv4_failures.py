@@ -124,3 +124,49 @@ except A.AesirError:
 kv.begin([1], [1])
 on_device(kv, [1])
 """)
+
+
+@pytest.mark.parametrize("what", ["launch", "new"])
+@pytest.mark.parametrize("op", ["copy(0, 3)", "truncate(0, 33)", "fork(0, 3)"])
+def test_page_operations_that_fail_change_nothing(child, what, op):
+    """Every launch and host allocation of an operation failing in turn: lengths, pages and what the pages hold stay; then it
+    succeeds."""
+    child(f"""
+fail, expect = (F.fake_fail_launch, -4) if {what!r} == "launch" else (F.fake_fail_new, -3)
+import numpy as np
+pool = ctx.allocate(1)     # where the cache's pages will start
+ctx.reset(0)
+kv = cache()
+kv.begin([2], [60])
+kv.begin([0, 1], [70, 33])
+kv.truncate(2, 0)          # pages 0 and 1 are free: compact has moves
+kv.begin([], [])           # a batch, which the operation ends
+
+def held(i):
+    raw = (C.c_char * (kv.num_pages * kv.page_bytes)).from_address(pool)
+    return [raw[p * kv.page_bytes:(p + 1) * kv.page_bytes] for p in kv.pages(i)]
+
+raw = (C.c_char * (kv.num_pages * kv.page_bytes)).from_address(pool)
+raw[:] = np.random.default_rng(0).bytes(len(raw))
+before, data = state(kv)[:2], [held(i) for i in range(2)]
+want = {{"copy(0, 3)": data[0], "compact()": [], "truncate(0, 33)": [], "fork(0, 3)": data[0]}}[{op!r}]
+
+def step():
+    try:
+        return kv.{op}
+    except A.AesirError:
+        assert state(kv)[:2] == before and [held(i) for i in range(2)] == data
+        raise
+
+codes = failing(fail, step)
+assert set(codes) <= {{expect}}, codes
+assert held(1) == data[1] and held(0) == data[0][:len(kv.pages(0))] and held(3) == want
+free = kv.free_pages
+for i in range(4):         # nothing was lost: all pages come back
+    fail(1 if {what!r} == "new" else 0)  # (cutting a sequence needs no memory)
+    kv.truncate(i, 0)
+    fail(0)
+assert kv.free_pages == kv.num_pages
+kv.begin([0], [320])
+assert kv.pages(0) == list(range(10))
+""")
