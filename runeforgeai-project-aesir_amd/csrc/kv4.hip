@@ -1867,9 +1867,11 @@ int32_t aesir_kv4_compact(aesir_kv4 *kv, int64_t *used_pages) {
     return guarded("compact", [&]() -> int32_t {
         AESIR_TRY(end_batch(kv));
         std::vector<PageMove> moves;
-        const int64_t used = kv->book.compact(moves);
+        const int64_t used = kv->book.compaction(moves);
+        AESIR_TRY(copy_pages(kv, moves));  // to free pages: nothing has changed if it fails
+        kv->book.compact(moves);
         if (used_pages) *used_pages = used;
-        return copy_pages(kv, moves);
+        return AESIR_OK;
     });
 }
 

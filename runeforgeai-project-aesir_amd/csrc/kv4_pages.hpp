@@ -118,32 +118,38 @@ class PageBook {
         touch(s, keep);
     }
 
-    // Moves every used page above the used count into a free one below it; afterwards pages [0, used) are the
-    // used ones. No move's destination is another's source.
-    int64_t compact(std::vector<PageMove> &moves) {
+    // The moves of every used page above the used count into a free one below it, both in ascending order: no move's
+    // destination is another's source. Returns the used count.
+    int64_t compaction(std::vector<PageMove> &moves) const {
         const int64_t total = (int64_t)refs_.size(), used = total - free_pages();
-        std::vector<int32_t> to((size_t)total, -1);
-        moves.reserve((size_t)free_pages());
-        for (int64_t p = used; p < total; p++)
-            if (refs_[(size_t)p] > 0) {
-                const int32_t dst = free_.top();  // the lowest free page: below `used` while sources are left
-                free_.pop();
-                to[(size_t)p] = dst;
-                moves.push_back({(int32_t)p, dst});
-                refs_[(size_t)dst] = refs_[(size_t)p];
-                refs_[(size_t)p] = 0;
-            }
-        if (!moves.empty()) {
-            for (Seq &s : seqs_)
-                for (size_t i = 0; i < s.pages.size(); i++)
-                    if (const int32_t dst = to[(size_t)s.pages[i]]; dst >= 0) {
-                        s.pages[i] = dst;
-                        touch(s, (int64_t)i);
-                    }
-            free_ = Free();
-            for (int64_t p = used; p < total; p++) free_.push((int32_t)p);
+        int64_t dst = 0;
+        for (int64_t p = used; p < total; p++) {
+            if (refs_[(size_t)p] == 0) continue;
+            while (refs_[(size_t)dst] > 0) dst++;  // below `used` while sources are left
+            moves.push_back({(int32_t)p, (int32_t)dst++});
         }
         return used;
+    }
+
+    // Makes these moves; afterwards pages [0, used) are the used ones.
+    void compact(const std::vector<PageMove> &moves) {
+        if (moves.empty()) return;
+        const int64_t total = (int64_t)refs_.size(), used = total - free_pages();
+        std::vector<int32_t> to((size_t)total, -1), rest;  // (what can throw comes before what changes)
+        rest.reserve((size_t)total);
+        for (int64_t p = used; p < total; p++) rest.push_back((int32_t)p);
+        for (const PageMove &m : moves) {
+            to[(size_t)m.src] = m.dst;
+            refs_[(size_t)m.dst] = refs_[(size_t)m.src];
+            refs_[(size_t)m.src] = 0;
+        }
+        for (Seq &s : seqs_)
+            for (size_t i = 0; i < s.pages.size(); i++)
+                if (const int32_t dst = to[(size_t)s.pages[i]]; dst >= 0) {
+                    s.pages[i] = dst;
+                    touch(s, (int64_t)i);
+                }
+        free_ = Free(std::greater<int32_t>(), std::move(rest));
     }
 
   private:
@@ -165,7 +171,7 @@ class PageBook {
     int64_t page_size_;
     std::vector<Seq> seqs_;
     std::vector<int32_t> refs_;  // sequences that hold each page
-    Free free_;
+    Free free_;  // (holds all pages at first, and compact() gives it as much room again: pushes take no memory)
 };
 
 }  // namespace aesir

@@ -127,7 +127,7 @@ on_device(kv, [1])
 
 
 @pytest.mark.parametrize("what", ["launch", "new"])
-@pytest.mark.parametrize("op", ["copy(0, 3)", "truncate(0, 33)", "fork(0, 3)"])
+@pytest.mark.parametrize("op", ["copy(0, 3)", "compact()", "truncate(0, 33)", "fork(0, 3)"])
 def test_page_operations_that_fail_change_nothing(child, what, op):
     """Every launch and host allocation of an operation failing in turn: lengths, pages and what the pages hold stay; then it
     succeeds."""
