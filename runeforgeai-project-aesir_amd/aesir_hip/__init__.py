@@ -209,11 +209,18 @@ class Context:
         self.h = h.value
         self._models = weakref.WeakSet()  # models hold pointers into the context: closed first
         self._caches = weakref.WeakSet()  # and so do paged 4-bit caches
+        self._dropped = []  # handles of caches whose last reference went while the stream was captured
+
+    def _destroy_dropped(self):
+        while self._dropped:
+            _check(_L.aesir_kv4_destroy(self._dropped[-1]))
+            self._dropped.pop()
 
     def close(self):
         if self.h:
             for m in list(self._models) + list(self._caches):
                 m.close()
+            self._destroy_dropped()
             _check(_L.aesir_ctx_destroy(self.h))
             self.h = None
 
@@ -421,6 +428,7 @@ class KV4Cache:
         self.max_seq_len, self.max_seqs, self.page_size, self.num_pages = max_seq_len, max_seqs, page_size, num_pages
         if ctx is not None:
             ctx._caches.add(self)
+            ctx._destroy_dropped()
 
     @staticmethod
     def well_bytes(num_layers: int, n_heads: int, n_kv_heads: int, head_dim: int, max_seq_len: int, max_seqs: int,
@@ -439,8 +447,9 @@ class KV4Cache:
     def __del__(self):
         try:
             self.close()
-        except Exception:
-            pass
+        except Exception:  # refused while the stream is captured: the context destroys it later
+            if self.ctx is not None:
+                self.ctx._dropped.append(self.h)
 
     @property
     def page_bytes(self) -> int:

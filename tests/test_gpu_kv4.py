@@ -797,3 +797,18 @@ def test_weights_sum_to_one(A, ctx, hd, nq, nkv, length, rows, value):
     kv.append(0, ctx.from_numpy(k[-rows:]), ctx.from_numpy(v[-rows:]))
     got = attend(A, ctx, kv, 0, half_weights(hd, rows, nq))
     assert (got == value).all(), (got[got != value][:5], (got != value).sum())
+
+
+def test_a_cache_dropped_during_a_capture_does_not_outlive_its_context(A):
+    ctx = A.Context(64 << 20)
+    caches = [A.KV4Cache(ctx, 1, 2, 1, 64, 64, 3, 32, 4) for _ in range(2)]
+    t = ctx.tensor(1, 128)
+    caches[0].begin([0], [1])
+
+    def run():
+        caches.pop()
+        caches[0].append(0, t, t)
+
+    Graph(A, ctx, run).close()
+    ctx.close()
+    assert not ctx.h and not caches[0].h

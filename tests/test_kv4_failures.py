@@ -170,3 +170,27 @@ assert kv.free_pages == kv.num_pages
 kv.begin([0], [320])
 assert kv.pages(0) == list(range(10))
 """)
+
+
+@pytest.mark.parametrize("later", ["", "other = cache()", "other = cache(); other.close()", "ctx.synchronize()"])
+def test_a_cache_dropped_during_a_capture_is_destroyed_later(child, later):
+    """The last reference goes while the stream is captured, where destroying is refused: the context closes all the same."""
+    child(f"""
+kv, kept = cache(), cache()
+F.fake_capturing(1)
+del kv
+try:
+    kept.close()
+    assert False
+except A.AesirError as e:
+    assert "captured" in str(e) and kept.h
+try:
+    ctx.close()
+    assert False
+except A.AesirError as e:
+    assert "captured" in str(e) and ctx.h
+F.fake_capturing(0)
+{later}
+ctx.close()
+assert not ctx.h and not kept.h
+""")
