@@ -451,16 +451,22 @@ class KV4Cache:
             if self.ctx is not None:
                 self.ctx._dropped.append(self.h)
 
+    def _open(self):
+        if not self.h:
+            raise AesirError(-1, "KV4Cache: the cache is closed")
+        return self.h
+
     @property
     def page_bytes(self) -> int:
-        return _L.aesir_kv4_page_bytes(self.h)
+        return _L.aesir_kv4_page_bytes(self._open())
 
     @property
     def free_pages(self) -> int:
-        return _L.aesir_kv4_free_pages(self.h)
+        return _L.aesir_kv4_free_pages(self._open())
 
     def length(self, seq: int) -> int:
-        return _L.aesir_kv4_length(self.h, seq)
+        """Positions of a sequence, -1 for one that the cache does not have."""
+        return _L.aesir_kv4_length(self._open(), seq)
 
     def pages(self, seq: int) -> list:
         """The page ids of a sequence in position order."""

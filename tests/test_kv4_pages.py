@@ -164,3 +164,14 @@ def test_null_handles_are_refused(A):
     kv = cache(A)
     assert L.aesir_kv4_begin(kv.h, None, None, 1) == -1
     assert L.aesir_kv4_pages(kv.h, 0, None, 4, None) == -1
+
+
+def test_a_closed_cache_answers_no_queries(A):
+    kv = cache(A)
+    kv.begin([0], [5])
+    kv.close()
+    for call in (lambda: kv.page_bytes, lambda: kv.free_pages, lambda: kv.length(0), lambda: kv.pages(0), kv.plan, kv.compact,
+                 lambda: kv.begin([0], [1]), lambda: kv.truncate(0, 0)):
+        with pytest.raises(A.AesirError, match="null|closed"):
+            call()
+    kv.close()
