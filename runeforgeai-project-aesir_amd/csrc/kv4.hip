@@ -17,7 +17,7 @@ constexpr int kThreads = 256;
 //
 // Batch descriptors, page table entries and page moves are written to pinned memory by the host and fetched by
 // one small launch: a copy engine's transfer costs more than the few KB it would move, and kernel arguments
-// hold too little.
+// (4 KB) hold the descriptors of 28 sequences at most.
 struct Kv4Upload {
     const uint32_t *src;
     uint32_t *dst;      // `words` words of src, then `fill` words of kNone
@@ -79,7 +79,7 @@ constexpr int kMaxSeqs = 4096;
 // minimum and maximum they exchange by DPP. Four consecutive rows of one head are neighbouring lane groups, so a
 // V tile of four positions leaves as one contiguous store. The quantization is exact: scales and levels are the
 // nearest ones of the real quotients, ties to even, as their definition says. Bound by instructions (some 20 an element of
-// scales, levels and packing): 8192 rows of 8 heads of 128, 13.4 us for 44 MB; one row by the launch and two reads, 3.4 us.
+// scales, levels and packing): 8192 rows of 8 heads of 128, 13.6 us for 44 MB; one row by the launch and two reads, 3.4 us.
 
 // The f16 nearest a double (ties to even): through f32 rounded to odd, so the second rounding decides alone.
 __device__ __forceinline__ h16 nearest_half(double x) {
@@ -277,7 +277,8 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(Kv4Dev c, Kv4ReadArg
 // ------------------------------------------------------------------ page copies
 //
 // 16 KB of a page per workgroup step, four 16-byte loads in flight per thread. Sources and destinations of one
-// launch are disjoint. Bound by memory: 32 pages of 2.6 MB 25 us, 6.7 TB/s read and written.
+// launch are disjoint. Bound by memory: 32 pages of 2.6 MB 25 us, 6.7 TB/s read and written (the last-level cache holds part
+// of them: a copy of 8 GiB reaches 5.2).
 constexpr int kCopyChunk = kThreads * 16 * 4;
 
 __global__ __launch_bounds__(kThreads) void kv4_copy_kernel(char *pool, int64_t page_bytes, const PageMove *moves, int n) {
@@ -304,7 +305,7 @@ __global__ __launch_bounds__(kThreads) void kv4_copy_kernel(char *pool, int64_t 
 // sequence and KV head, or a piece of its rounds of 32 keys, or pieces of several; its four or eight waves take the rounds in
 // turn, each for all columns (a key is unpacked by one wave, once a tile), and meet in LDS at the end; a tile's
 // pieces meet in kv4_merge_kernel. Bound by memory where there is much to read: 64 sequences of about 4096 positions, 8 KV
-// heads of 128 (335 MB), 63 us and 5 for the merge, 5.3 TB/s; else by the chain of reads that a workgroup starts
+// heads of 128 (335 MB), 63 us and 5 for the merge, 5.4 TB/s; else by the chain of reads that a workgroup starts
 // with (records, page ids, the first round) and the launches: 4.5 us for 100 positions.
 //
 //   scores   S^T = K q^T: a 16-key tile's A operand is unpacked nibbles; lane (i, g) holds key 8 (i / 4) + 4 t + i % 4
@@ -1178,8 +1179,8 @@ constexpr int64_t kPartCols = 65536;  // columns of split partials: 256 of every
 // - little work that one workgroup a CU can take in pieces of their own: kFewLeast rounds or more each (8 / 12 / 16 / 32
 //   rounds: one sequence of 1024 positions 8.8 / 9.5 / 10.2 / 10.5, of 4096 10.4 / 10.6 / 10.9 / 13.2), of eight
 //   waves where pieces are over 16 rounds (one of 65536 positions 25.4 with four, 22.9; of 100 4.7 with four, 5.0);
-// - else as many workgroups of four waves as run at once (three, two and one to a CU by the registers of 16, 32 and 64
-//   columns), kLeast rounds each or more (32 / 48 / 64: 24 sequences of 3000 26.0 / 25.6 / 31.0, 40 of 4000 43.1 / 43.4 /
+// - else as many workgroups of four waves as run at once at head_dim 128 (three, two and one to a CU by the registers of 16,
+//   32 and 64 columns; narrower heads leave places for more, and of head_dim 256's 512 half run at once), kLeast rounds each or more (32 / 48 / 64: 24 sequences of 3000 26.0 / 25.6 / 31.0, 40 of 4000 43.1 / 43.4 /
 //   47.3), half of that with little work (12 / 24 / 48: 8 of 2048 12.7 / 12.3 / 17.6); equal shares of all tiles where
 //   starts of their own don't fit (64 of 4096: 66.5 against 75.8).
 constexpr int64_t kWholeRounds = 96, kShortRounds = 24;
