@@ -287,7 +287,8 @@ int32_t aesir_kv_v_slice(const aesir_kv *kv, int64_t layer_idx, int64_t seq_len,
  * append() and attention() may be captured into a HIP graph on the context's stream. A replay there serves
  * the batch of its time: it stores or attends for the first rows of it, as many as the captured call had,
  * and does nothing when there is no batch. The other calls send host data to the device and are refused
- * while the stream is being captured. fork, copy, truncate and compact end the batch. */
+ * while the stream is being captured. fork, copy, truncate and compact end the batch. A call that fails leaves
+ * every sequence as it was. */
 
 /* Bytes of well that aesir_kv4_create takes for these sizes, or a negative error code. */
 int64_t aesir_kv4_well_bytes(int64_t num_layers, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,

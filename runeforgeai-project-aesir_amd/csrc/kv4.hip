@@ -1180,9 +1180,10 @@ constexpr int64_t kPartCols = 65536;  // columns of split partials: 256 of every
 //   rounds: one sequence of 1024 positions 8.8 / 9.5 / 10.2 / 10.5, of 4096 10.4 / 10.6 / 10.9 / 13.2), of eight
 //   waves where pieces are over 16 rounds (one of 65536 positions 25.4 with four, 22.9; of 100 4.7 with four, 5.0);
 // - else as many workgroups of four waves as run at once at head_dim 128 (three, two and one to a CU by the registers of 16,
-//   32 and 64 columns; narrower heads leave places for more, and of head_dim 256's 512 half run at once), kLeast rounds each or more (32 / 48 / 64: 24 sequences of 3000 26.0 / 25.6 / 31.0, 40 of 4000 43.1 / 43.4 /
-//   47.3), half of that with little work (12 / 24 / 48: 8 of 2048 12.7 / 12.3 / 17.6); equal shares of all tiles where
-//   starts of their own don't fit (64 of 4096: 66.5 against 75.8).
+//   32 and 64 columns; narrower heads leave places for more, and of head_dim 256's 512 half run at once), kLeast rounds
+//   each or more (32 / 48 / 64: 24 sequences of 3000 26.0 / 25.6 / 31.0, 40 of 4000 43.1 / 43.4 / 47.3), half of that with
+//   little work (12 / 24 / 48: 8 of 2048 12.7 / 12.3 / 17.6); equal shares of all tiles where starts of their own don't
+//   fit (64 of 4096: 66.5 against 75.8).
 constexpr int64_t kWholeRounds = 96, kShortRounds = 24;
 constexpr int64_t kFewRounds = 256 * 64, kFewLeast = 8;
 constexpr int64_t kGroups[3] = {768, 512, 256}, kLeast = 48;
