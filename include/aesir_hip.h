@@ -225,6 +225,46 @@ int32_t aesir_gemm_quant(aesir_ctx *ctx, const void *A, int64_t a_rows, int64_t 
 int32_t aesir_q8_0_matvec_f32(aesir_ctx *ctx, const void *blocks, int64_t n_rows, int64_t k, const float *x,
                               float *y);
 
+/* ======================================================================= 8-bit floating point
+ * Rows (activations) and weights in OCP e4m3 with an f32 scale for each block of 128, and the product that reads
+ * them. No counterpart in the reference's GGUF path.
+ *
+ * A matrix of rows x cols is a pair: codes [rows][ld] bytes, ld = cols rounded up to 128, 16-byte aligned, the bytes
+ * behind cols 0; and scales, of activations one for each 1 x 128 block, laid out [ld / 128][rows], of weights one for
+ * each 128 x 128 block (fewer rows in the last), laid out [ceil(rows / 128)][ld / 128]. An element is code * scale.
+ * The calls below that write one store, with y the values of a block and a the largest |y|, scale = a / 448 and the
+ * e4m3 numbers nearest 448 y / a, ties to even: a block of zeros has scale 0 and codes 0, one that holds an inf or a
+ * NaN reads as NaN throughout (all codes 0x7f, scale NaN). The codes are those of the formula whatever its rounding on
+ * the way, so a row's do not depend on the rows beside it.
+ *
+ * f16 tensors are rows of `cols` elements from row to row, of which the first q_cols (C: b_rows) count, so they may be
+ * parts of a wider matrix; any 2-byte alignment, 16 bytes with cols and q_cols multiples of 8 being the fast one. Up
+ * to 2^22 columns. Outputs must not overlap inputs or each other but where said. All of them may be captured into a
+ * HIP graph on the context's stream; they allocate nothing. */
+
+/* Codes and scales of x, blocks of block_rows = 1 (activations) or 128 (weights) rows. */
+int32_t aesir_quantize_fp8(aesir_ctx *ctx, const void *x, int64_t x_rows, int64_t x_cols, void *q, float *scales,
+                           int64_t q_rows, int64_t q_cols, int64_t block_rows);
+/* Activations of the RMSNorm of h = f16(x + residual): y = h w / sqrt(mean h^2 + epsilon), not rounded to f16 between
+ * (aesir_rmsnorm_f16 rounds twice). h is written to sum, which may be x or residual itself (with its row length).
+ * residual and sum NULL: h = x. A row that holds an inf or a NaN reads as NaN throughout. */
+int32_t aesir_rmsnorm_fp8(aesir_ctx *ctx, const void *x, int64_t x_rows, int64_t x_cols, const void *residual,
+                          int64_t residual_rows, int64_t residual_cols, void *sum, int64_t sum_rows, int64_t sum_cols,
+                          const void *weight, int64_t weight_size, float epsilon, void *q, float *scales, int64_t q_rows,
+                          int64_t q_cols);
+/* Activations of y = up * gate / (1 + exp(-gate)), not rounded between (aesir_swiglu_f16 rounds each step). A block
+ * without a |y| of 2^-64 or more is zeros. */
+int32_t aesir_swiglu_fp8(aesir_ctx *ctx, const void *gate, int64_t gate_rows, int64_t gate_cols, const void *up,
+                         int64_t up_rows, int64_t up_cols, void *q, float *scales, int64_t q_rows, int64_t q_cols);
+/* C[m, n] = sum over blocks b of a_scale[b][m] b_scale[n / 128][b] sum_k A[m, k] B[n, k], of activations A
+ * [a_rows x a_cols] and weights B [b_rows x a_cols], all sums in f32, rounded once to c_type (AESIR_GGML_F16 or
+ * AESIR_GGML_F32); rows of C are c_cols >= b_rows elements apart. The sums' order goes by the sizes alone. The product
+ * of two scales has to be an f32 number. Raises "gemm_fp8: matrix dimensions must be positive", "gemm_fp8: inner matrix
+ * dimension mismatch", "gemm_fp8: output matrix shape mismatch". */
+int32_t aesir_gemm_fp8(aesir_ctx *ctx, const void *A, const float *a_scales, int64_t a_rows, int64_t a_cols, const void *B,
+                       const float *b_scales, int64_t b_rows, int64_t b_cols, void *C, int32_t c_type, int64_t c_rows,
+                       int64_t c_cols);
+
 /* ======================================================================= sampler
  * sample_token_from_logits (core/sampler.mojo:217-305): the whole sampler stack on the device.
  * Parameter meaning as in the reference: temperature <= 0 or top_k == 1 is the greedy branch

@@ -84,6 +84,10 @@ _sig("aesir_argmax_f16", [P, P, I64, C.POINTER(I64)])
 _sig("aesir_gemm_q8_0", [P, P, I64, I64, P, I64, P, I64, I64])
 _sig("aesir_gemm_quant", [P, P, I64, I64, P, I32, I64, P, I64, I64])
 _sig("aesir_q8_0_matvec_f32", [P, P, I64, I64, P, P])
+_sig("aesir_quantize_fp8", [P, P, I64, I64, P, P, I64, I64, I64])
+_sig("aesir_rmsnorm_fp8", [P, P, I64, I64, P, I64, I64, P, I64, I64, P, I64, F32, P, P, I64, I64])
+_sig("aesir_swiglu_fp8", [P, P, I64, I64, P, I64, I64, P, P, I64, I64])
+_sig("aesir_gemm_fp8", [P, P, P, I64, I64, P, P, I64, I64, P, I32, I64, I64])
 _sig("aesir_kv_create", [P, I64, I64, I64, C.POINTER(P)])
 _sig("aesir_kv_destroy", [P])
 _sig("aesir_kv_append", [P, P, I64, I64, P, I64, P, I64])
@@ -338,6 +342,98 @@ def gemm_quant(ctx: Context, A: Tensor, blocks_ptr: int, ggml_type: int, b_rows:
 
 def q8_0_matvec_f32(ctx: Context, blocks_ptr: int, n_rows: int, k: int, x: Tensor, y: Tensor):
     _check(_L.aesir_q8_0_matvec_f32(ctx.h, blocks_ptr, n_rows, k, x.ptr, y.ptr))
+
+
+class FP8Tensor:
+    """A rows x cols matrix of e4m3 codes [rows][ld] (ld: cols rounded up to 128) with f32 scales: of activations
+    (block_rows 1) for 1 x 128 blocks, [ld / 128][rows], of weights (block_rows 128) for 128 x 128 blocks,
+    [ceil(rows / 128)][ld / 128]. An element is code * scale."""
+
+    def __init__(self, ctx: Context, ptr: int, scales_ptr: int, rows: int, cols: int, block_rows: int = 1):
+        if block_rows not in (1, 128):
+            raise ValueError("FP8Tensor: blocks have 1 or 128 rows")
+        self.ctx, self.ptr, self.scales_ptr = ctx, ptr, scales_ptr
+        self.rows, self.cols, self.block_rows = rows, cols, block_rows
+
+    @classmethod
+    def empty(cls, ctx: Context, rows: int, cols: int, block_rows: int = 1) -> "FP8Tensor":
+        """Room in the context's well."""
+        t = cls(ctx, 0, 0, rows, cols, block_rows)
+        t.ptr = ctx.tensor(rows, t.ld, np.uint8).ptr
+        t.scales_ptr = ctx.tensor(*t.scales_shape, np.float32).ptr
+        return t
+
+    @property
+    def ld(self) -> int:
+        return (self.cols + 127) // 128 * 128
+
+    @property
+    def scales_shape(self) -> tuple:
+        return (self.ld // 128, self.rows) if self.block_rows == 1 else ((self.rows + 127) // 128, self.ld // 128)
+
+    def codes(self) -> np.ndarray:
+        return Tensor(self.ctx, self.ptr, self.rows, self.ld, np.uint8).numpy()
+
+    def scales(self) -> np.ndarray:
+        return Tensor(self.ctx, self.scales_ptr, *self.scales_shape, np.float32).numpy()
+
+    def upload(self, codes: np.ndarray, scales: np.ndarray) -> "FP8Tensor":
+        Tensor(self.ctx, self.ptr, self.rows, self.ld, np.uint8).upload(codes)
+        Tensor(self.ctx, self.scales_ptr, *self.scales_shape, np.float32).upload(scales)
+        return self
+
+    def numpy(self) -> np.ndarray:
+        """The f32 values code * scale."""
+        c = np.arange(256)
+        e, f = c >> 3 & 15, c & 7
+        number = np.where(e == 0, f * 2.0**-9, (8 + f) * 2.0 ** (e - 10.0)) * np.where(c & 128, -1, 1)
+        number[c & 127 == 127] = np.nan
+        s = self.scales()
+        s = s.T if self.block_rows == 1 else np.repeat(s, 128, 0)[: self.rows]
+        return (number.astype(np.float32)[self.codes()] * np.repeat(s, 128, 1))[:, : self.cols]
+
+
+def quantize_fp8(ctx: Context, x: Tensor, out: FP8Tensor):
+    """Codes and scales of x, whose rows are x.cols elements apart (out.cols of them count)."""
+    _check(_L.aesir_quantize_fp8(ctx.h, x.ptr, x.rows, x.cols, out.ptr, out.scales_ptr, out.rows, out.cols, out.block_rows))
+
+
+def _activations(name: str, t: FP8Tensor):
+    if t.block_rows != 1:
+        raise AesirError(-2, f"{name}: activations have blocks of one row")
+
+
+def rmsnorm_fp8(ctx: Context, x: Tensor, weight: Tensor, out: FP8Tensor, epsilon: float = 1e-5, residual: Tensor = None,
+                total: Tensor = None):
+    """Activations of the RMSNorm of x, or with a residual of f16(x + residual), which goes to total (or back to x)."""
+    _activations("rmsnorm_fp8", out)
+    r = (None, 0, 0, None, 0, 0)
+    if residual is not None:
+        total = x if total is None else total
+        r = (residual.ptr, residual.rows, residual.cols, total.ptr, total.rows, total.cols)
+    elif total is not None:
+        raise AesirError(-1, "rmsnorm_fp8: a residual and the place of its sum come together")
+    _check(_L.aesir_rmsnorm_fp8(ctx.h, x.ptr, x.rows, x.cols, *r, weight.ptr, weight.size, epsilon, out.ptr, out.scales_ptr,
+                                out.rows, out.cols))
+
+
+def swiglu_fp8(ctx: Context, gate: Tensor, up: Tensor, out: FP8Tensor):
+    """Activations up * gate / (1 + exp(-gate)); gate and up may be parts of one product's rows."""
+    _activations("swiglu_fp8", out)
+    _check(_L.aesir_swiglu_fp8(ctx.h, gate.ptr, gate.rows, gate.cols, up.ptr, up.rows, up.cols, out.ptr, out.scales_ptr, out.rows,
+                               out.cols))
+
+
+def gemm_fp8(ctx: Context, A: FP8Tensor, B: FP8Tensor, C_: Tensor):
+    """C[m, n] = sum_k A[m, k] B[n, k] of activations A and weights B, in f16 or f32 by C's dtype."""
+    _activations("gemm_fp8", A)
+    if B.block_rows != 128:
+        raise AesirError(-2, "gemm_fp8: weights have blocks of 128 rows")
+    _check(_L.aesir_gemm_fp8(ctx.h, A.ptr, A.scales_ptr, A.rows, A.cols, B.ptr, B.scales_ptr, B.rows, B.cols, C_.ptr,
+                             _C_TYPES.get(C_.dtype, -1), C_.rows, C_.cols))
+
+
+_C_TYPES = {np.dtype(np.float16): 1, np.dtype(np.float32): 0}  # AESIR_GGML_F16, AESIR_GGML_F32
 
 
 class SamplerConfig(C.Structure):

@@ -36,7 +36,7 @@ CXXFLAGS = [
 ]
 
 SOURCES = ["ctx.hip", "gemv.hip", "quant.hip", "skinny.hip", "skinny_raw.hip", "attention.hip", "kv4.hip", "basic.hip", "q8_0.hip", "abi_ops.hip", "model.hip",
-           "prefill.hip", "gguf.hip", "sampler.hip", "blas.hip"]
+           "prefill.hip", "gguf.hip", "sampler.hip", "blas.hip", "fp8.hip"]
 
 
 # accumulators of the matrix instructions in vector registers: kernels that rescale them each time a maximum rises

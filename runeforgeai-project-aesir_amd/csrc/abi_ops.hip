@@ -321,6 +321,89 @@ int32_t aesir_q8_0_matvec_f32(aesir_ctx *ctx, const void *blocks, int64_t n_rows
     return launch_q8_0_matvec_f32(ctx->stream, blocks, n_rows, k, x, y);
 }
 
+// ------------------------------------------------------------------ 8-bit floating point
+
+}  // extern "C"
+
+// Checks of codes and scales that a call of `name` reads or writes. Rows of codes are read and written 16 bytes at a
+// time; offsets inside 256 rows are 32-bit ones.
+static int32_t fp8_matrix(const char *name, const void *q, const void *scales, int64_t rows, int64_t cols) {
+    if (rows <= 0 || cols <= 0) return fail(AESIR_ERR_INVALID, "%s: matrix dimensions must be positive", name);
+    if (!q || !scales) return fail(AESIR_ERR_INVALID, "%s: null tensor pointer", name);
+    if (((uintptr_t)q & 15) || ((uintptr_t)scales & 3))
+        return fail(AESIR_ERR_INVALID, "%s: codes must be 16-byte and scales 4-byte aligned", name);
+    if (cols > ((int64_t)1 << 22)) return fail(AESIR_ERR_UNSUPPORTED, "%s: more than 2^22 columns", name);
+    if (rows > ((int64_t)1 << 40)) return fail(AESIR_ERR_UNSUPPORTED, "%s: more than 2^40 rows", name);
+    return AESIR_OK;
+}
+
+// The same of f16 rows of `stride` elements from row to row, of which the first `cols` count.
+static int32_t fp8_rows(const char *name, const void *x, int64_t x_rows, int64_t stride, int64_t rows, int64_t cols) {
+    if (x_rows <= 0 || stride <= 0) return fail(AESIR_ERR_INVALID, "%s: tensor dimensions must be positive", name);
+    if (x_rows != rows || stride < cols) return fail(AESIR_ERR_SHAPE, "%s: tensor shape mismatch", name);
+    if (!x) return fail(AESIR_ERR_INVALID, "%s: null tensor pointer", name);
+    if ((uintptr_t)x & 1) return fail(AESIR_ERR_INVALID, "%s: f16 tensors must be 2-byte aligned", name);
+    if (mul_checked(x_rows, stride, 2) < 0) return fail(AESIR_ERR_UNSUPPORTED, "%s: tensor too large", name);
+    return AESIR_OK;
+}
+
+extern "C" {
+
+int32_t aesir_quantize_fp8(aesir_ctx *ctx, const void *x, int64_t x_rows, int64_t x_cols, void *q, float *scales, int64_t q_rows,
+                           int64_t q_cols, int64_t block_rows) {
+    AESIR_TRY(bind(ctx));
+    AESIR_TRY(fp8_matrix("quantize_fp8", q, scales, q_rows, q_cols));
+    AESIR_TRY(fp8_rows("quantize_fp8", x, x_rows, x_cols, q_rows, q_cols));
+    if (block_rows != 1 && block_rows != 128) return fail(AESIR_ERR_INVALID, "quantize_fp8: blocks have 1 or 128 rows");
+    return launch_quantize_fp8(ctx->stream, x, x_cols, q_rows, q_cols, block_rows == 128, q, scales);
+}
+
+int32_t aesir_rmsnorm_fp8(aesir_ctx *ctx, const void *x, int64_t x_rows, int64_t x_cols, const void *residual, int64_t residual_rows,
+                          int64_t residual_cols, void *sum, int64_t sum_rows, int64_t sum_cols, const void *weight,
+                          int64_t weight_size, float epsilon, void *q, float *scales, int64_t q_rows, int64_t q_cols) {
+    AESIR_TRY(bind(ctx));
+    AESIR_TRY(fp8_matrix("rmsnorm_fp8", q, scales, q_rows, q_cols));
+    AESIR_TRY(fp8_rows("rmsnorm_fp8", x, x_rows, x_cols, q_rows, q_cols));
+    if ((residual == nullptr) != (sum == nullptr))
+        return fail(AESIR_ERR_INVALID, "rmsnorm_fp8: a residual and the place of its sum come together");
+    if (residual) {
+        AESIR_TRY(fp8_rows("rmsnorm_fp8", residual, residual_rows, residual_cols, q_rows, q_cols));
+        AESIR_TRY(fp8_rows("rmsnorm_fp8", sum, sum_rows, sum_cols, q_rows, q_cols));
+        if ((sum == x && sum_cols != x_cols) || (sum == residual && sum_cols != residual_cols))
+            return fail(AESIR_ERR_SHAPE, "rmsnorm_fp8: a sum in place has its tensor's rows");
+    }
+    if (weight_size < q_cols) return fail(AESIR_ERR_SHAPE, "rmsnorm_fp8: weight dimension mismatch");
+    if (!(epsilon > 0.0f)) return fail(AESIR_ERR_INVALID, "rmsnorm_fp8: epsilon must be positive");
+    if (!weight) return fail(AESIR_ERR_INVALID, "rmsnorm_fp8: null tensor pointer");
+    if ((uintptr_t)weight & 1) return fail(AESIR_ERR_INVALID, "rmsnorm_fp8: f16 tensors must be 2-byte aligned");
+    return launch_rmsnorm_fp8(ctx->stream, x, x_cols, residual, residual_cols, sum, sum_cols, weight, epsilon, q_rows, q_cols, q,
+                              scales);
+}
+
+int32_t aesir_swiglu_fp8(aesir_ctx *ctx, const void *gate, int64_t gate_rows, int64_t gate_cols, const void *up, int64_t up_rows,
+                         int64_t up_cols, void *q, float *scales, int64_t q_rows, int64_t q_cols) {
+    AESIR_TRY(bind(ctx));
+    AESIR_TRY(fp8_matrix("swiglu_fp8", q, scales, q_rows, q_cols));
+    AESIR_TRY(fp8_rows("swiglu_fp8", gate, gate_rows, gate_cols, q_rows, q_cols));
+    AESIR_TRY(fp8_rows("swiglu_fp8", up, up_rows, up_cols, q_rows, q_cols));
+    return launch_swiglu_fp8(ctx->stream, gate, gate_cols, up, up_cols, q_rows, q_cols, q, scales);
+}
+
+int32_t aesir_gemm_fp8(aesir_ctx *ctx, const void *A, const float *a_scales, int64_t a_rows, int64_t a_cols, const void *B,
+                       const float *b_scales, int64_t b_rows, int64_t b_cols, void *C, int32_t c_type, int64_t c_rows,
+                       int64_t c_cols) {
+    AESIR_TRY(bind(ctx));
+    AESIR_TRY(fp8_matrix("gemm_fp8", A, a_scales, a_rows, a_cols));
+    AESIR_TRY(fp8_matrix("gemm_fp8", B, b_scales, b_rows, b_cols));
+    if (a_cols != b_cols) return fail(AESIR_ERR_SHAPE, "gemm_fp8: inner matrix dimension mismatch");
+    if (c_rows != a_rows || c_cols < b_rows) return fail(AESIR_ERR_SHAPE, "gemm_fp8: output matrix shape mismatch");
+    if (c_type != AESIR_GGML_F16 && c_type != AESIR_GGML_F32) return fail(AESIR_ERR_UNSUPPORTED, "gemm_fp8: output type must be F16 or F32");
+    if (!C) return fail(AESIR_ERR_INVALID, "gemm_fp8: null tensor pointer");
+    if ((uintptr_t)C & (c_type == AESIR_GGML_F32 ? 3 : 1)) return fail(AESIR_ERR_INVALID, "gemm_fp8: output is not aligned to its type");
+    if (mul_checked(c_rows, c_cols, 4) < 0) return fail(AESIR_ERR_UNSUPPORTED, "gemm_fp8: output too large");
+    return launch_gemm_fp8(ctx->stream, A, a_scales, a_rows, B, b_scales, b_rows, a_cols, C, c_type == AESIR_GGML_F32, c_cols);
+}
+
 // ------------------------------------------------------------------ KV cache
 
 int32_t aesir_kv_create(aesir_ctx *ctx, int64_t max_seq_len, int64_t hidden_dim, int64_t num_layers, aesir_kv **out) {
