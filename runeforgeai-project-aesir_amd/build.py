@@ -41,7 +41,7 @@ SOURCES = ["ctx.hip", "gemv.hip", "quant.hip", "skinny.hip", "skinny_raw.hip", "
 
 # accumulators of the matrix instructions in vector registers: kernels that rescale them each time a maximum rises
 # would otherwise move them from the accumulation registers and back
-EXTRA = {"kv4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for f in ("kv4.hip", "fp8.hip")}
 
 
 def _compile(src: str) -> str:

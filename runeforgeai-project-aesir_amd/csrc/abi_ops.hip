@@ -401,7 +401,8 @@ int32_t aesir_gemm_fp8(aesir_ctx *ctx, const void *A, const float *a_scales, int
     if (!C) return fail(AESIR_ERR_INVALID, "gemm_fp8: null tensor pointer");
     if ((uintptr_t)C & (c_type == AESIR_GGML_F32 ? 3 : 1)) return fail(AESIR_ERR_INVALID, "gemm_fp8: output is not aligned to its type");
     if (mul_checked(c_rows, c_cols, 4) < 0) return fail(AESIR_ERR_UNSUPPORTED, "gemm_fp8: output too large");
-    return launch_gemm_fp8(ctx->stream, A, a_scales, a_rows, B, b_scales, b_rows, a_cols, C, c_type == AESIR_GGML_F32, c_cols);
+    return launch_gemm_fp8(ctx->stream, A, a_scales, a_rows, B, b_scales, b_rows, a_cols, C, c_type == AESIR_GGML_F32, c_cols,
+                           ctx->scratch.attn_part, ctx->scratch.attn_part_floats);
 }
 
 // ------------------------------------------------------------------ KV cache

@@ -362,99 +362,420 @@ struct Fp8Args {
     const float *as, *bs;  // scales [ld / 128][M], [ceil(N / 128)][ld / 128]
     void *c;
     int64_t M, N, ldc;
-    int nb;  // blocks along k
-    bool f32;
+    int nb;     // blocks along k
+    int splits; // workgroups that share a tile of C, each with a stretch of the blocks along k
+    float *part;  // their sums [splits][M][N] where there are more than one
+    bool f32;   // type of c
+    bool quad;  // whether rows of c are 16-byte aligned
 };
 
 __device__ __forceinline__ void fp8_store(const Fp8Args &p, int64_t m, int64_t n, f32x4 v) {
-    if (m >= p.M) return;
+    if (m >= p.M || n >= p.N) return;
+    const int64_t at = m * p.ldc + n;
+    if (p.quad && n + 3 < p.N) {
+        if (p.f32)
+            *(f32x4 *)((float *)p.c + at) = v;
+        else
+            *(u32x2 *)((h16 *)p.c + at) = u32x2{h2_bits(h16x2{(h16)v[0], (h16)v[1]}), h2_bits(h16x2{(h16)v[2], (h16)v[3]})};
+        return;
+    }
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         if (n + e >= p.N) return;
         if (p.f32)
-            ((float *)p.c)[m * p.ldc + n + e] = v[e];
+            ((float *)p.c)[at + e] = v[e];
         else
-            ((h16 *)p.c)[m * p.ldc + n + e] = (h16)v[e];
+            ((h16 *)p.c)[at + e] = (h16)v[e];
     }
 }
 
-// Tile of 128 rows of A by 128 of B, 4 waves of 64 x 64, two LDS stages of one k-block. Weights are the first
-// operand of the matrix instruction, so a lane's elements are 4 neighbouring columns of one row of C.
+constexpr int kPastBuffers = 0x70000000;  // an offset behind every buffer here, with room for a tile's rows
+
+#define FP8_LDS(p) ((__attribute__((address_space(3))) void *)(p))
+
+// A copy instruction fills 1 KiB of LDS, 8 rows of 128 bytes: lane l brings slot l % 8 of row l / 8, which holds granule
+// (l % 8) ^ (row / 2 % 8) of the row's k-block, so that the 16 rows that a fragment reads at once lie in different banks.
+// The lane's offset from the first of the 8 rows, rows `ld` bytes apart; odd: whether they are rows 8 .. 15 of 16.
+__device__ __forceinline__ int copy_offset(int lane, int ld, bool odd) {
+    return lane / 8 * ld + ((lane & 7) ^ ((lane >> 4) + (odd ? 4 : 0))) * 16;
+}
+
+// Lane's fragment of the 16 rows at `rows`, from LDS.
 template <bool EXACT>
-__global__ __launch_bounds__(256) void fp8_gemm_kernel(Fp8Args p) {
+__device__ __forceinline__ auto read_frag(const uint8_t *rows, int at) {
+    const Frag8 f{ld16(rows + at), ld16(rows + (at ^ 64))};
+    if constexpr (EXACT)
+        return to_f16(f);
+    else
+        return f;
+}
+
+// Few rows of A: every weight is used by all of them as it arrives. A workgroup owns 16 NR rows of B; its W waves take
+// the k-blocks in turn, each through a ring of S stages of its own in LDS (no barriers), and their sums meet in a fixed
+// order. MH: rows of A in eighths of 8.
+template <int MH, int NR, int W, int S, bool EXACT>
+__global__ __launch_bounds__(64 * W) void fp8_stream_kernel(Fp8Args p) {
+    constexpr int MT = (MH + 1) / 2, kA = NR * 2048, kScales = kA + MH * 1024, kStage = kScales + 512, kLoads = 2 * NR + MH + 2;
     extern __shared__ __align__(16) uint8_t lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t mt = (p.M + 127) / 128, m0 = blockIdx.x % mt * 128, n0 = blockIdx.x / mt * 128;
-    const int64_t ld = (int64_t)p.nb * 128;
-    const int rows_a = (int)min((int64_t)128, p.M - m0), rows_b = (int)min((int64_t)128, p.N - n0);
-    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void *)(p.a + m0 * ld), 0, (int)(rows_a * ld), kBufferDword3);
-    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void *)(p.b + n0 * ld), 0, (int)(rows_b * ld), kBufferDword3);
-    // a copy instruction moves 8 rows of 128 bytes: lane l fills slot l % 8 of row l / 8 with granule
-    // (l % 8) ^ (row / 2 % 8), so that the 16 rows a fragment reads at once lie in different banks
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15;
+    const int64_t n0 = (int64_t)blockIdx.x * (16 * NR);
+    const int ld = p.nb * 128, M = (int)p.M;
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void *)p.a, 0, M * ld, kBufferDword3);
+    const __amdgpu_buffer_rsrc_t rb =
+        __builtin_amdgcn_make_buffer_rsrc((void *)(p.b + n0 * ld), 0, (int)min((int64_t)16 * NR, p.N - n0) * ld, kBufferDword3);
+    const __amdgpu_buffer_rsrc_t rsa = __builtin_amdgcn_make_buffer_rsrc((void *)p.as, 0, p.nb * M * 4, kBufferDword3);
+    const __amdgpu_buffer_rsrc_t rsb = __builtin_amdgcn_make_buffer_rsrc((void *)(p.bs + n0 / 128 * p.nb), 0, p.nb * 4, kBufferDword3);
+    uint8_t *ring = lds + wave * (S * kStage);
+    const int even = copy_offset(lane, ld, false), odd = copy_offset(lane, ld, true);
+    // blocks past the last: addresses past the buffers, which read as zeros, so that every stage has as many copies
     auto request = [&](int stage, int kb) {
+        uint8_t *to = ring + stage * kStage;
+        const int k = kb < p.nb ? kb * 128 : kPastBuffers;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int r = (wave * 8 + i) % 16 * 8 + lane / 8;
-            const int off = (int)(r * ld) + kb * 128 + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
-            uint8_t *dst = lds + stage * 32768 + (wave * 8 + i) * 1024;
-            if (wave < 2)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void *)dst, 16, off, 0, 0, 0);
-            else
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void *)dst, 16, off, 0, 0, 0);
-        }
+        for (int i = 0; i < 2 * NR; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, FP8_LDS(to + i * 1024), 16, (i & 1 ? odd : even) + i * 8 * ld + k, 0, 0, 2);
+#pragma unroll
+        for (int i = 0; i < MH; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, FP8_LDS(to + kA + i * 1024), 16, (i & 1 ? odd : even) + i * 8 * ld + k, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, FP8_LDS(to + kScales), 4, kb < p.nb ? kb * M * 4 + lane * 4 : kPastBuffers, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsb, FP8_LDS(to + kScales + 256), 4, kb < p.nb ? kb * 4 : kPastBuffers, 0, 0, 0);
     };
-    const int wm = wave % 2 * 64, wn = wave / 2 * 64, i16 = lane & 15;
     const int at = i16 * 128 + ((lane >> 4) ^ (i16 >> 1)) * 16;
-    f32x4 acc[4][4] = {};
-    request(0, 0);
-    for (int kb = 0; kb < p.nb; kb++) {
-        __builtin_amdgcn_s_waitcnt(vm_wait(0));
-        __syncthreads();
-        if (kb + 1 < p.nb) request((kb + 1) & 1, kb + 1);
-        const uint8_t *la = lds + (kb & 1) * 32768 + wm * 128, *lb = lds + (kb & 1) * 32768 + 16384 + wn * 128;
-        const float sb = p.bs[n0 / 128 * p.nb + kb];
-        using Frag = std::conditional_t<EXACT, Frag16, Frag8>;
-        auto frag = [&](const uint8_t *row) {
-            const Frag8 f{ld16(row + at), ld16(row + (at ^ 64))};
-            if constexpr (EXACT)
-                return to_f16(f);
-            else
-                return f;
-        };
-        Frag a[4];
-        float s[4];
+    f32x4 acc[NR][MT] = {};
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int64_t m = m0 + wm + 16 * j + i16;
-            s[j] = m < p.M ? p.as[kb * p.M + m] * sb : 0.0f;
-            a[j] = frag(la + 2048 * j);
+    for (int i = 0; i < S - 1; i++) request(i, wave + i * W);
+    int stage = 0;
+    for (int kb = wave; kb < p.nb; kb += W) {
+        request(stage == 0 ? S - 1 : stage - 1, kb + (S - 1) * W);
+        __builtin_amdgcn_s_waitcnt(vm_wait((S - 1) * kLoads));
+        const uint8_t *from = ring + stage * kStage;
+        const float sb = *(const float *)(from + kScales + 256);
+        decltype(read_frag<EXACT>(from, at)) b[NR];
+#pragma unroll
+        for (int i = 0; i < NR; i++) b[i] = read_frag<EXACT>(from + i * 2048, at);
+#pragma unroll
+        for (int j = 0; j < MT; j++) {
+            const float s = *(const float *)(from + kScales + (16 * j + i16) * 4) * sb;
+            const auto a = read_frag<EXACT>(from + kA + j * 2048, at);
+#pragma unroll
+            for (int i = 0; i < NR; i++) {
+                const f32x4 d = mma_block(b[i], a);
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(d[e], s, acc[i][j][e]);
+            }
+        }
+        stage = stage == S - 1 ? 0 : stage + 1;
+    }
+    __builtin_amdgcn_s_waitcnt(vm_wait(0));
+    __syncthreads();
+    f32x4 *part = (f32x4 *)lds;
+#pragma unroll
+    for (int i = 0; i < NR; i++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) part[(wave * NR * MT + i * MT + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    for (int t = wave; t < NR * MT; t += W) {
+        f32x4 v = part[t * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < W; w++) v += part[(w * NR * MT + t) * 64 + lane];
+        fp8_store(p, 16 * (t % MT) + i16, n0 + 16 * (t / MT) + 4 * (lane >> 4), v);
+    }
+}
+
+// Barrier of the workgroup's waves that neither the compiler's memory operations nor its schedule cross.
+__device__ __forceinline__ void barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
+// A wave's sums to C, T's rows from (m, n) on, whole along n and 16-byte aligned.
+template <typename T, int NF, int MF>
+__device__ __forceinline__ void store_rows(const Fp8Args &p, T *c, uint8_t *lds, const f32x4 (&acc)[NF][MF], int64_t m, int64_t n, int wave,
+                                           int lane) {
+    constexpr int kRow = NF * 16 * sizeof(T), kStride = kRow + 16, kLanes = kRow / 16, kRows = 64 / kLanes;
+    uint8_t *own = lds + wave * 16 * kStride;
+#pragma unroll
+    for (int j = 0; j < MF; j++) {
+#pragma unroll
+        for (int i = 0; i < NF; i++) {
+            uint8_t *to = own + (lane & 15) * kStride + (16 * i + 4 * (lane >> 4)) * sizeof(T);
+            const f32x4 v = acc[i][j];
+            if constexpr (sizeof(T) == 4)
+                *(f32x4 *)to = v;
+            else
+                *(u32x2 *)to = u32x2{h2_bits(h16x2{(h16)v[0], (h16)v[1]}), h2_bits(h16x2{(h16)v[2], (h16)v[3]})};
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const Frag b = frag(lb + 2048 * i);
+        for (int r = lane / kLanes; r < 16; r += kRows) {
+            const u32x4 v = ld16(own + r * kStride + lane % kLanes * 16);
+            if (m + 16 * j + r < p.M) st16((uint8_t *)(c + (m + 16 * j + r) * p.ldc + n) + lane % kLanes * 16, v);
+        }
+    }
+}
+
+// Tile of BM rows of A by BN of B on WM x WN waves, through a ring of S stages of one k-block in LDS. Weights are the
+// first operand of the matrix instruction, so a lane's elements are 4 neighbouring columns of one row of C.
+template <int BM, int BN, int WM, int WN, int S, bool EXACT, bool ONCE = false>
+__global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(Fp8Args p) {
+    constexpr int W = WM * WN, MF = BM / WM / 16, NF = BN / WN / 16, IA = BM / 8 / W, IB = BN / 8 / W;
+    constexpr int kB = BM * 128, kScales = kB + BN * 128, kStage = kScales + (BM + 64) * 4, kLoads = IA + IB + 1;
+    static_assert(BM / 8 % W == 0 && BN / 8 % W == 0 && BM / 64 < W && BM % 64 == 0 && 128 % (BN / WN) == 0);
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15;
+    // each XCD (workgroups go to the 8 in turn) takes a stretch of the tiles, which run through bands of 8 rows of
+    // tiles of C, column by column, so that the tiles it works on at a time share rows of A and B in its L2
+    const unsigned mt = (unsigned)((p.M + BM - 1) / BM), nt = (unsigned)((p.N + BN - 1) / BN), all = gridDim.x, xcd = blockIdx.x % 8;
+    const unsigned place = blockIdx.x / 8 + xcd * (all / 8) + min(xcd, all % 8), split = place / (mt * nt), tile = place - split * mt * nt;
+    const unsigned band = tile / (8 * nt), in_band = tile - band * 8 * nt, high = min(8u, mt - 8 * band);
+    const int64_t m0 = (int64_t)(8 * band + in_band % high) * BM, n0 = (int64_t)(in_band / high) * BN;
+    const int ld = p.nb * 128;
+    const int rows_a = (int)min((int64_t)BM, p.M - m0), rows_b = (int)min((int64_t)BN, p.N - n0);
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void *)(p.a + m0 * ld), 0, rows_a * ld, kBufferDword3);
+    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void *)(p.b + n0 * ld), 0, rows_b * ld, kBufferDword3);
+    // scales: waves 0 .. BM / 64 - 1 bring those of 64 rows of A each, the others those of the tile's rows of B
+    const bool sa = wave < BM / 64;
+    const int nblocks = (rows_b + 127) / 128;
+    const float *bs = p.bs + n0 / 128 * p.nb;
+    const int scales_to = kScales + (sa ? wave : BM / 64) * 256;
+    const float *scales = sa ? p.as + m0 : bs;  // of the block requested next
+    const int64_t scales_step = sa ? p.M : 1;
+    const int scales_bytes = sa ? rows_a * 4 : (nblocks - 1) * p.nb * 4 + 4;
+    const int scales_from = sa ? min(wave * 64 + lane, rows_a - 1) * 4 : min(lane, nblocks - 1) * p.nb * 4;
+    // A copy instruction fills 1 KiB of LDS, 8 rows of 128 bytes: lane l brings slot l % 8 of row l / 8, which holds
+    // granule (l % 8) ^ (row / 2 % 8) of the row's k-block, so that the 16 rows that a fragment reads at once lie in
+    // different banks. Rows past the last and blocks past the last are the last ones again, whose products nothing takes.
+    int from[IA + IB];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const f32x4 d = mma_block(b, a[j]);
+    for (int i = 0; i < IA + IB; i++) {
+        const int r = (i < IA ? wave * IA + i : wave * IB + i - IA) * 8 + lane / 8;
+        from[i] = min(r, (i < IA ? rows_a : rows_b) - 1) * ld + ((lane & 7) ^ (r >> 1 & 7)) * 16;
+    }
+    const int k0 = (int)((int64_t)p.nb * split / p.splits), k1 = (int)((int64_t)p.nb * (split + 1) / p.splits);
+    scales += k0 * scales_step;
+    auto request = [&](int stage, int kb) {
+        uint8_t *to = lds + stage * kStage;
+        const int k = min(kb, k1 - 1) * 128;
 #pragma unroll
-                for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(d[e], s[j], acc[i][j][e]);
+        for (int i = 0; i < IA; i++) {
+            const int at = from[i];
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, FP8_LDS(to + (wave * IA + i) * 1024), 16, at, k, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < IB; i++) {
+            const int at = from[IA + i];
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, FP8_LDS(to + kB + (wave * IB + i) * 1024), 16, at, k, 0, ONCE ? 2 : 0);
+        }
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)scales, 0, scales_bytes, kBufferDword3);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, FP8_LDS(to + scales_to), 4, scales_from, 0, 0, 0);
+        if (kb + 1 < k1) scales += scales_step;
+    };
+    const int wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
+    const int at = i16 * 128 + ((lane >> 4) ^ (i16 >> 1)) * 16;
+    using Frag = decltype(read_frag<EXACT>(lds, at));
+    f32x4 acc[NF][MF] = {};
+#pragma unroll
+    for (int i = 0; i < S - 1; i++) request(i, k0 + i);
+    int stage = 0;
+    for (int kb = k0; kb < k1; kb++) {
+        __builtin_amdgcn_s_waitcnt(vm_wait((S - 2) * kLoads));
+        barrier();
+        const uint8_t *la = lds + stage * kStage + wm * 128, *lb = lds + stage * kStage + kB + wn * 128;
+        const float *sc = (const float *)(lds + stage * kStage + kScales);
+        const float sb = sc[BM + wn / 128];
+        Frag a[MF], b[3];
+        float s[MF];
+        b[0] = read_frag<EXACT>(lb, at);
+#pragma unroll
+        for (int j = 0; j < MF; j++) {
+            a[j] = read_frag<EXACT>(la + 2048 * j, at);
+            s[j] = sc[wm + 16 * j + i16] * sb;
+            if (j == 0) b[1] = read_frag<EXACT>(lb + 2048, at);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        request(stage == 0 ? S - 1 : stage - 1, kb + S - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        // a product is added to its sum when the two after it have been issued; a row of B's fragment is read two rows ahead
+        constexpr int D = 3, kBehind = 2;
+        f32x4 d[D];
+#pragma unroll
+        for (int t = 0; t < MF * NF + kBehind; t++) {
+            const int i = t / MF;
+            if (t % MF == 0 && i + 2 < NF) b[(i + 2) % 3] = read_frag<EXACT>(lb + 2048 * (i + 2), at);
+            if (t < MF * NF) d[t % D] = mma_block(b[i % 3], a[t % MF]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (t >= kBehind) {
+                const int u = t - kBehind;
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[u / MF][u % MF][e] = fmaf(d[u % D][e], s[u % MF], acc[u / MF][u % MF][e]);
+                asm volatile("" : "+v"(acc[u / MF][u % MF]));  // here: the compiler would put all of them off to the end
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        stage = stage == S - 1 ? 0 : stage + 1;
+    }
+    __builtin_amdgcn_s_waitcnt(vm_wait(0));
+    if (p.splits > 1) {  // sums of a stretch of k: f32 rows of N elements
+        p.c = p.part + split * p.M * p.N;
+        p.ldc = p.N;
+        p.f32 = true;
+        p.quad = p.N % 4 == 0;
+    }
+    // Rows of C through LDS, so that a store fills whole lines: 16 rows at a time, in a place of the wave's own.
+    if (p.quad && n0 + BN <= p.N) {
+        barrier();
+        if (p.f32)
+            store_rows<float>(p, (float *)p.c, lds, acc, m0 + wm, n0 + wn, wave, lane);
+        else
+            store_rows<h16>(p, (h16 *)p.c, lds, acc, m0 + wm, n0 + wn, wave, lane);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < NF; i++)
+#pragma unroll
+        for (int j = 0; j < MF; j++) fp8_store(p, m0 + wm + 16 * j + i16, n0 + wn + 16 * i + 4 * (lane >> 4), acc[i][j]);
+}
+
+// C from the sums of `splits` stretches of k, in their order; fewer than 2^31 elements. VEC: 4 a thread, N a multiple of 4.
+template <bool VEC>
+__global__ __launch_bounds__(256) void fp8_join_kernel(Fp8Args p) {
+    const unsigned e = (blockIdx.x * 256 + threadIdx.x) * (VEC ? 4 : 1), all = (unsigned)(p.M * p.N), N = (unsigned)p.N;
+    if (e >= all) return;
+    if constexpr (VEC) {
+        f32x4 v = *(const f32x4 *)(p.part + e);
+        for (int z = 1; z < p.splits; z++) v += *(const f32x4 *)(p.part + (int64_t)z * all + e);
+        fp8_store(p, e / N, e % N, v);
+    } else {
+        float v = p.part[e];
+        for (int z = 1; z < p.splits; z++) v += p.part[(int64_t)z * all + e];
+        const int64_t at = e / N * p.ldc + e % N;
+        if (p.f32)
+            ((float *)p.c)[at] = v;
+        else
+            ((h16 *)p.c)[at] = (h16)v;
+    }
+}
+
+template <int MH, int NR, int W, int S, bool EXACT>
+static int32_t stream(hipStream_t s, const Fp8Args &p) {
+    constexpr int kParts = W * NR * ((MH + 1) / 2) * 1024, kRing = W * S * (NR * 2048 + MH * 1024 + 512), kLds = kParts > kRing ? kParts : kRing;
+    static std::atomic<uint64_t> done{0};
+    const auto kernel = fp8_stream_kernel<MH, NR, W, S, EXACT>;
+    if (kLds > 65536) AESIR_TRY(raise_lds_limit((const void *)kernel, kLds, done));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((p.N + 16 * NR - 1) / (16 * NR))), dim3(64 * W), kLds, s, p);
+    AESIR_LAUNCH_CHECK("fp8_stream_kernel");
+    return AESIR_OK;
+}
+
+template <int BM, int BN, int WM, int WN, int S, bool EXACT, bool ONCE = false>
+static int32_t tile(hipStream_t s, const Fp8Args &p) {
+    constexpr int kLds = S * ((BM + BN) * 128 + (BM + 64) * 4);
+    static std::atomic<uint64_t> done{0};
+    const auto kernel = fp8_tile_kernel<BM, BN, WM, WN, S, EXACT, ONCE>;
+    if (kLds > 65536) AESIR_TRY(raise_lds_limit((const void *)kernel, kLds, done));
+    const int64_t tiles = (p.M + BM - 1) / BM * ((p.N + BN - 1) / BN);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * p.splits)), dim3(64 * WM * WN), kLds, s, p);
+    AESIR_LAUNCH_CHECK("fp8_tile_kernel");
+    if (p.splits > 1) {
+        const bool vec = p.N % 4 == 0;
+        const unsigned groups = (unsigned)((p.M * p.N / (vec ? 4 : 1) + 255) / 256);
+        hipLaunchKernelGGL(vec ? fp8_join_kernel<true> : fp8_join_kernel<false>, dim3(groups), dim3(256), 0, s, p);
+        AESIR_LAUNCH_CHECK("fp8_join_kernel");
+    }
+    return AESIR_OK;
+}
+
+// Up to 16 rows of A: memory's rate decides. More rows of B a workgroup (NR) are fewer workgroups and fewer copies of A,
+// and pay where B alone fills the 256 CUs; long rows want 8 waves along k. Measured, us of 1 / 16 rows, by NR and waves:
+// 4096 x 4096 NR 1, 4 waves 5.3 / 5.7, NR 2 6.0 / 6.6; 6144 x 4096 7.0 / 8.2, NR 2 6.8 / 7.3; 28672 x 4096 21.7 / 25.7, NR 4
+// 20.8 / 23.1; 4096 x 14336 NR 1, 4 waves 11.3 / 12.4, 8 waves 10.8 / 13.0; 57344 x 8192 8 waves 68 / 83, NR 4 81 / 87.
+template <int MH>
+static int32_t stream_16(hipStream_t s, const Fp8Args &p) {
+    if (p.N > 4096) {
+        if (p.N <= 8192 && p.nb <= 64) return stream<MH, 2, 4, 3, true>(s, p);
+        if (p.N > 8192 && p.nb <= 32) return stream<MH, 4, 4, 2, true>(s, p);
+    } else if (p.nb <= 32) {
+        return stream<MH, 1, 4, 3, true>(s, p);
+    }
+    return stream<MH, 1, 8, 2, true>(s, p);
+}
+
+// 17 to 64 rows of at most 8192 of B: as above, with 4 waves, since the rows of A take most of a ring's stage.
+template <bool EXACT>
+static int32_t stream_64(hipStream_t s, const Fp8Args &p) {
+    if (p.N <= 4096)
+        return p.M <= 32   ? stream<4, 1, 4, 3, EXACT>(s, p)
+               : p.M <= 48 ? stream<6, 1, 4, 2, EXACT>(s, p)
+                           : stream<8, 1, 4, 2, EXACT>(s, p);
+    return p.M <= 32   ? stream<4, 2, 4, 3, EXACT>(s, p)
+           : p.M <= 48 ? stream<6, 2, 4, 3, EXACT>(s, p)
+                       : stream<8, 2, 4, 2, EXACT>(s, p);
+}
+
+// A tile's shape and how many of its workgroups a CU holds, with what a k-block takes a CU (us) that holds one of them and
+// one that is full, as measured on products of 1000 to 4096 rows of 2048 to 28672 columns.
+struct TileCost {
+    int bm, bn, per_cu;
+    float one, full;
+};
+constexpr TileCost kTiles[] = {{64, 64, 2, 0.28f, 0.38f}, {128, 128, 1, 0.56f, 0.56f}, {192, 128, 1, 0.72f, 0.72f}, {128, 128, 2, 0.8f, 1.07f}, {256, 256, 1, 1.73f, 1.73f}};
+constexpr TileCost kExactTiles[] = {{64, 64, 2, 0.43f, 0.66f}, {128, 128, 1, 1.12f, 1.12f}, {128, 128, 2, 1.4f, 1.85f}};
+
+// The tile and the number of stretches of k that the product is cut into, by the time that they come to: rounds of
+// workgroups, or what A and B take from memory at 4.5 TB/s where that is more, 4.5 us around each round, and for the
+// stretches' sums another launch and their bytes.
+template <int N>
+static int choose_tile(const TileCost (&tiles)[N], const Fp8Args &p, int64_t part_floats, int *splits) {
+    int best = 0;
+    float least = 1e30f;
+    *splits = 1;
+    for (int i = 0; i < N; i++) {
+        const TileCost &c = tiles[i];
+        const int64_t count = (p.M + c.bm - 1) / c.bm * ((p.N + c.bn - 1) / c.bn);
+        for (int z = 1; z <= 8 && (z == 1 || (p.nb >= 4 * z && p.M * p.N <= part_floats / z)); z *= 2) {
+            const int64_t all = count * z, rounds = (all + 256 * c.per_cu - 1) / (256 * c.per_cu);
+            const float step = all <= 256 ? c.one : c.full, blocks = (float)((p.nb + z - 1) / z);
+            const float work = fmaxf((float)rounds * blocks * step, (float)(p.M + p.N) * (float)p.nb * (128 / 4.5e6f));
+            const float t = (float)rounds * 4.5f + work + (z > 1 ? 2.2f + (float)(z * p.M * p.N) * 2.5e-6f : 0.0f);
+            if (t < least) {
+                least = t;
+                best = i;
+                *splits = z;
             }
         }
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) fp8_store(p, m0 + wm + 16 * j + i16, n0 + wn + 16 * i + 4 * (lane >> 4), acc[i][j]);
+    return best;
 }
 
 int32_t launch_gemm_fp8(hipStream_t s, const void *A, const float *as, int64_t M, const void *B, const float *bs, int64_t N,
-                        int64_t K, void *C, bool f32, int64_t ldc) {
-    const int64_t nb = fp8_blocks(K);
-    const Fp8Args p{(const uint8_t *)A, (const uint8_t *)B, as, bs, C, M, N, ldc, (int)nb, f32};
-    const int64_t tiles = (M + 127) / 128 * ((N + 127) / 128);
-    if (tiles > 0x7fffffff) return fail(AESIR_ERR_UNSUPPORTED, "gemm_fp8: output larger than one launch takes");
-    hipLaunchKernelGGL(f32 ? fp8_gemm_kernel<true> : fp8_gemm_kernel<false>, dim3((unsigned)tiles), dim3(256), 65536, s, p);
-    AESIR_LAUNCH_CHECK("fp8_gemm_kernel");
-    return AESIR_OK;
+                        int64_t K, void *C, bool f32, int64_t ldc, float *part, int64_t part_floats) {
+    const bool quad = ldc % (f32 ? 4 : 8) == 0 && ((uintptr_t)C & 15) == 0;
+    Fp8Args p{(const uint8_t *)A, (const uint8_t *)B, as, bs, C, M, N, ldc, (int)fp8_blocks(K), 1, part, f32, quad};
+    if ((M + 63) / 64 > 0x7fffffff / ((N + 15) / 16)) return fail(AESIR_ERR_UNSUPPORTED, "gemm_fp8: output larger than one launch takes");
+    if (M <= 16) return M <= 8 ? stream_16<1>(s, p) : stream_16<2>(s, p);
+    if (M <= 64) {
+        // Tiles of 64 x 64 share the rows of A among 64 of B: they pay once they fill half the CUs, by B's rows (64 rows
+        // 28672 x 4096 31.1 us against 37.7) or, from 33 rows on, by stretches of long rows (64 rows 4096 x 14336 18.5
+        // against 22.2, 2048 x 5632 9.8 both, 4096 x 4096 10.2 against 8.5).
+        if (N < 8192 && (M <= 32 || p.nb < 96)) return f32 ? stream_64<true>(s, p) : stream_64<false>(s, p);
+        const TileCost one[1] = {f32 ? kExactTiles[0] : kTiles[0]};
+        choose_tile(one, p, part_floats, &p.splits);
+        return f32 ? tile<64, 64, 2, 2, 4, true, true>(s, p) : tile<64, 64, 2, 2, 4, false, true>(s, p);
+    }
+    if (f32) switch (choose_tile(kExactTiles, p, part_floats, &p.splits)) {
+        case 0: return tile<64, 64, 2, 2, 4, true>(s, p);
+        case 1: return tile<128, 128, 4, 2, 3, true>(s, p);
+        default: return tile<128, 128, 2, 2, 2, true>(s, p);
+    }
+    switch (choose_tile(kTiles, p, part_floats, &p.splits)) {
+        case 0: return tile<64, 64, 2, 2, 4, false>(s, p);
+        case 1: return tile<128, 128, 4, 2, 3, false>(s, p);
+        case 2: return tile<192, 128, 4, 2, 3, false>(s, p);
+        case 3: return tile<128, 128, 2, 2, 2, false>(s, p);
+        default: return tile<256, 256, 4, 2, 2, false>(s, p);
+    }
 }
 
 }  // namespace aesir

@@ -293,7 +293,7 @@ int32_t launch_q8_0_matvec_f32(hipStream_t s, const void *blocks, int64_t N, int
 
 // ------------------------------------------------------------------ 8-bit floating point (fp8.hip)
 // Codes [rows][cols rounded up to 128] and scales of rows (1 x 128 blocks) or of weights (128 x 128 blocks); strides
-// in elements.
+// in elements. part: scratch for sums of stretches of k.
 int32_t launch_quantize_fp8(hipStream_t s, const void *x, int64_t stride, int64_t rows, int64_t cols, bool weight, void *q,
                             float *scales);
 int32_t launch_rmsnorm_fp8(hipStream_t s, const void *x, int64_t x_stride, const void *residual, int64_t res_stride, void *sum,
@@ -301,6 +301,6 @@ int32_t launch_rmsnorm_fp8(hipStream_t s, const void *x, int64_t x_stride, const
 int32_t launch_swiglu_fp8(hipStream_t s, const void *gate, int64_t g_stride, const void *up, int64_t u_stride, int64_t rows,
                           int64_t cols, void *q, float *scales);
 int32_t launch_gemm_fp8(hipStream_t s, const void *A, const float *as, int64_t M, const void *B, const float *bs, int64_t N,
-                        int64_t K, void *C, bool f32, int64_t ldc);
+                        int64_t K, void *C, bool f32, int64_t ldc, float *part, int64_t part_floats);
 
 }  // namespace aesir
