@@ -3,9 +3,9 @@
 // the matrix cores.
 //
 // With y the values of a block and a = max |y|: scale = f32(a / 448), code = the e4m3 number nearest 448 y / a,
-// ties to even. The kernels find t = 448 y / a in f32, a few units of its last place off, and convert it; where t
-// lies that near the middle of two codes it is found again in f64, so that every code is the one of
-// the formula.
+// ties to even. The kernels find t = 448 y / a in f32, a few units of its last place off, and round both ends of an
+// interval that holds the exact quotient: rounding is monotone, so where both give the same code so does the quotient.
+// Elsewhere (one element in some 10^5) it is found again in f64, so that every code is the one of the formula.
 #include "device.hpp"
 #include "kernels.hpp"
 #include "mfma_gemm.hpp"
@@ -19,15 +19,6 @@ constexpr float kE4m3Max = 448.0f;  // largest e4m3 number
 constexpr unsigned kInfBits = 0x7f800000u;
 
 // ------------------------------------------------------------------ codes
-
-// Whether t, up to `near` units of the last place off, may lie on the other side of the middle of two e4m3 numbers:
-// the 20 low bits of an f32 are what e4m3 drops, and its numbers below 2^-6 are as far apart as those just above,
-// where adding 2^-6 takes them.
-__device__ __forceinline__ bool near_middle(float t, unsigned near) {
-    float v = fabsf(t);
-    v = v < 0.015625f ? v + 0.015625f : v;
-    return (__builtin_bit_cast(unsigned, v) & 0xfffffu) - (0x80000u - near) <= 2 * near;
-}
 
 // f32 of t cut towards zero, its last bit set where something was cut: rounding it to e4m3 gives what rounding t does.
 __device__ __forceinline__ float to_odd(double t) {
@@ -52,6 +43,14 @@ __device__ __forceinline__ unsigned top_bits(const float (&p)[8]) {
     for (int j = 0; j < 8; j++) m = max(m, __builtin_bit_cast(unsigned, p[j]) & 0x7fffffffu);
     return m;
 }
+// The same of 8 f16 numbers, as f32 bits.
+__device__ __forceinline__ unsigned top_bits(u32x4 v) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 m = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; j++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[j] & 0x7fff7fffu));
+    return __builtin_bit_cast(unsigned, (float)bits_to_h(max(m.x, m.y)));
+}
 
 // Maximum over each 16 lanes; every one gets it.
 __device__ __forceinline__ unsigned row_max(unsigned m) {
@@ -71,33 +70,34 @@ __device__ __forceinline__ unsigned wave_max_u(unsigned m) {
 constexpr u32x2 kNanCodes = {0x7f7f7f7fu, 0x7f7f7f7fu};
 
 // Codes of 8 values p that are exact in f32 with at most 22 bits (f16 numbers or products of two), top the bits of
-// their block's largest |p|. t is off by at most 2 units of its last place (the quotient and the product are rounded
-// once each); 448 p is exact in f64, and a quotient that is no middle is at least 2^-28 of one away from it.
+// their block's largest |p|. p times 448 / a, itself rounded once, is off by less than 2^-22 of it; 448 p is exact in
+// f64, and a quotient that is not the middle of two codes is at least 2^-28 of it away from one.
 __device__ __forceinline__ u32x2 codes_of(const float (&p)[8], unsigned top) {
     if (top >= kInfBits) return kNanCodes;
     const float a = __builtin_bit_cast(float, top), inv = top ? kE4m3Max / a : 0.0f;
-    float t[8];
-    bool near = false;
+    const float less = inv * (1.0f - 0x1p-22f), more = inv * (1.0f + 0x1p-22f);
+    float lo[8], hi[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        t[j] = p[j] * inv;
-        near |= near_middle(t[j], 4);
+        lo[j] = p[j] * less;
+        hi[j] = p[j] * more;
     }
-    if (near) {
+    const u32x2 c = to_e4m3(lo), d = to_e4m3(hi);
+    if (((c.x ^ d.x) | (c.y ^ d.y)) == 0) return c;
 #pragma unroll
-        for (int j = 0; j < 8; j++) t[j] = to_odd((double)p[j] * 448.0 / (double)a);
-    }
-    return to_e4m3(t);
+    for (int j = 0; j < 8; j++) lo[j] = to_odd((double)p[j] * 448.0 / (double)a);
+    return to_e4m3(lo);
 }
 
 // ------------------------------------------------------------------ rows
 
 // 8 f16 elements of a row from column c on, zeros behind its `cols`. whole: every row holds whole, 16-byte aligned
-// groups of 8.
+// groups of 8. ONCE: nothing reads them again (non-temporal: SwiGLU of 4096 x 14336 67 -> 60 us).
+template <bool ONCE = true>
 __device__ __forceinline__ u32x4 load8(const h16 *row, int64_t c, int64_t cols, bool whole) {
     u32x4 v = {0, 0, 0, 0};
     if (whole) {
-        if (c < cols) v = ld16(row + c);
+        if (c < cols) v = ONCE ? ld16_stream(row + c) : ld16(row + c);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; j++)
@@ -130,18 +130,34 @@ static int64_t fp8_blocks(int64_t cols) { return (cols + kFp8Block - 1) / kFp8Bl
 
 // ------------------------------------------------------------------ quantize
 
-// 16 lanes a block: 8 neighbouring elements each.
+// 16 lanes a block, 8 neighbouring elements each; a wave has 4 blocks of a row, a workgroup 4 rows at a time, kSteps
+// times, all of them requested at first.
+constexpr int kSteps = 2;
+__device__ __forceinline__ int64_t unit_row() { return (int64_t)blockIdx.x * (4 * kSteps) + threadIdx.x / 64; }
+__device__ __forceinline__ int64_t unit_block() { return (int64_t)blockIdx.y * 4 + threadIdx.x % 64 / 16; }
+static dim3 unit_grid(int64_t rows, int64_t nb) { return dim3((unsigned)((rows + 4 * kSteps - 1) / (4 * kSteps)), (unsigned)((nb + 3) / 4)); }
+
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(const h16 *__restrict__ x, int64_t stride, int64_t rows, int64_t cols,
                                                            bool whole, uint8_t *__restrict__ q, float *__restrict__ scales) {
-    const int64_t nb = (cols + kFp8Block - 1) / kFp8Block, unit = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
-    if (unit >= rows * nb) return;
-    const int64_t r = unit / nb, b = unit % nb, c = b * kFp8Block + 8 * (threadIdx.x % 16);
-    float p[8];
-    unpack8(load8(x + r * stride, c, cols, whole), p);
-    const unsigned top = row_max(top_bits(p));
-    *reinterpret_cast<u32x2 *>(q + r * nb * kFp8Block + c) = codes_of(p, top);
-    if (threadIdx.x % 16 == 0)
-        scales[b * rows + r] = top >= kInfBits ? __builtin_nanf("") : __builtin_bit_cast(float, top) / kE4m3Max;
+    const int64_t nb = (cols + kFp8Block - 1) / kFp8Block, r0 = unit_row(), b = unit_block(), c = b * kFp8Block + 8 * (threadIdx.x % 16);
+    if (b >= nb) return;
+    u32x4 v[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) {
+        v[i] = {0, 0, 0, 0};
+        if (r0 + 4 * i < rows) v[i] = load8(x + (r0 + 4 * i) * stride, c, cols, whole);
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) {
+        const int64_t r = r0 + 4 * i;
+        if (r >= rows) return;
+        float p[8];
+        unpack8(v[i], p);
+        const unsigned top = row_max(top_bits(v[i]));
+        *reinterpret_cast<u32x2 *>(q + r * nb * kFp8Block + c) = codes_of(p, top);
+        if (threadIdx.x % 16 == 0)
+            scales[b * rows + r] = top >= kInfBits ? __builtin_nanf("") : __builtin_bit_cast(float, top) / kE4m3Max;
+    }
 }
 
 // A workgroup per 128 x 128 block, its 16384 elements in registers between the maximum and the codes.
@@ -160,10 +176,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_weight_kernel(const h16 *__r
     unsigned top = 0;
     float p[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        unpack8(v[i], p);
-        top = max(top, top_bits(p));
-    }
+    for (int i = 0; i < 8; i++) top = max(top, top_bits(v[i]));
     top = wave_max_u(top);
     if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
     __syncthreads();
@@ -180,13 +193,13 @@ __global__ __launch_bounds__(256) void fp8_quantize_weight_kernel(const h16 *__r
 int32_t launch_quantize_fp8(hipStream_t s, const void *x, int64_t stride, int64_t rows, int64_t cols, bool weight, void *q,
                             float *scales) {
     const bool whole = whole_rows(cols, stride, x);
-    const int64_t nb = fp8_blocks(cols), groups = weight ? (rows + 127) / 128 * nb : (rows * nb + 15) / 16;
+    const int64_t nb = fp8_blocks(cols), groups = weight ? (rows + 127) / 128 * nb : (rows + 4 * kSteps - 1) / (4 * kSteps);
     if (groups > 0x7fffffff) return fail(AESIR_ERR_UNSUPPORTED, "quantize_fp8: more elements than one launch takes");
     if (weight)
         hipLaunchKernelGGL(fp8_quantize_weight_kernel, dim3((unsigned)groups), dim3(256), 0, s, (const h16 *)x, stride, rows, cols,
                            whole, (uint8_t *)q, scales);
     else
-        hipLaunchKernelGGL(fp8_quantize_kernel, dim3((unsigned)groups), dim3(256), 0, s, (const h16 *)x, stride, rows, cols, whole,
+        hipLaunchKernelGGL(fp8_quantize_kernel, unit_grid(rows, nb), dim3(256), 0, s, (const h16 *)x, stride, rows, cols, whole,
                            (uint8_t *)q, scales);
     AESIR_LAUNCH_CHECK("fp8_quantize_kernel");
     return AESIR_OK;
@@ -196,44 +209,71 @@ int32_t launch_quantize_fp8(hipStream_t s, const void *x, int64_t stride, int64_
 
 // A workgroup per row. h = f16(x + residual), y = h w / sqrt(mean h^2 + eps): the row's factor changes no code, so the
 // codes are those of h w, exact in f32, and the factor goes into the scales. A row with an inf or NaN is NaN whole.
-__global__ __launch_bounds__(256) void fp8_norm_kernel(const h16 *x, int64_t x_stride, const h16 *residual,
-                                                       int64_t res_stride, h16 *sum, int64_t sum_stride,
-                                                       const h16 *__restrict__ w, float eps, int64_t rows, int64_t cols, bool whole,
-                                                       bool w_whole, uint8_t *__restrict__ q, float *__restrict__ scales) {
+// V: groups of 2048 columns, which stay in registers; 0: any number of them, read twice.
+template <int V>
+__global__ __launch_bounds__(256) void fp8_norm_kernel(const h16 *x, int64_t x_stride, const h16 *residual, int64_t res_stride, h16 *sum,
+                                                       int64_t sum_stride, const h16 *__restrict__ w, float eps, int64_t rows,
+                                                       int64_t cols, bool whole, bool w_whole, uint8_t *__restrict__ q,
+                                                       float *__restrict__ scales) {
     __shared__ float red[4];
     const int64_t r = blockIdx.x, nb = (cols + kFp8Block - 1) / kFp8Block;
-    const h16 *xr = x + r * x_stride;
+    const h16 *xr = x + r * x_stride, *rr = residual + r * res_stride;
+    h16 *sr = sum + r * sum_stride;
     float ss = 0.0f;
-    for (int64_t c = 8 * threadIdx.x; c < nb * kFp8Block; c += 2048) {
-        u32x4 v = load8(xr, c, cols, whole);
+    auto add = [&](u32x4 v, u32x4 d, int64_t c) {
+        float h[8];
         if (residual) {
-            const u32x4 d = load8(residual + r * res_stride, c, cols, whole);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const h16x2 a = as_h2(v[j]), b = as_h2(d[j]);
                 v[j] = h2_bits(h16x2{hadd(a.x, b.x), hadd(a.y, b.y)});
             }
-            store8(sum + r * sum_stride, c, cols, whole, v);
+            store8(sr, c, cols, whole, v);
         }
-        float h[8];
         unpack8(v, h);
 #pragma unroll
         for (int j = 0; j < 8; j++) ss = fmaf(h[j], h[j], ss);
-    }
-    ss = block_sum<4>(ss, red);
-    const float factor = 1.0f / sqrtf(ss / (float)cols + eps);
-    for (int64_t c = 8 * threadIdx.x; c < nb * kFp8Block; c += 2048) {
+        return v;
+    };
+    float factor = 0.0f;
+    auto finish = [&](u32x4 v, u32x4 g8, int64_t c) {
         float p[8], g[8];
-        unpack8(residual ? load8(sum + r * sum_stride, c, cols, whole) : load8(xr, c, cols, whole), p);
-        unpack8(load8(w, c, cols, w_whole), g);
+        unpack8(v, p);
+        unpack8(g8, g);
 #pragma unroll
         for (int j = 0; j < 8; j++) p[j] *= g[j];
         unsigned top = row_max(top_bits(p));
         if (!(ss < __builtin_inff())) top = kInfBits;
         *reinterpret_cast<u32x2 *>(q + r * nb * kFp8Block + c) = codes_of(p, top);
         if (threadIdx.x % 16 == 0)
-            scales[c / kFp8Block * rows + r] =
-                top >= kInfBits ? __builtin_nanf("") : __builtin_bit_cast(float, top) * factor / kE4m3Max;
+            scales[c / kFp8Block * rows + r] = top >= kInfBits ? __builtin_nanf("") : __builtin_bit_cast(float, top) * factor / kE4m3Max;
+    };
+    const u32x4 none = {0, 0, 0, 0};
+    if constexpr (V > 0) {
+        u32x4 v[V], d[V], g[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const int64_t c = 8 * threadIdx.x + 2048 * i;
+            v[i] = load8(xr, c, cols, whole);
+            d[i] = residual ? load8(rr, c, cols, whole) : none;
+            g[i] = load8<false>(w, c, cols, w_whole);
+        }
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = add(v[i], d[i], 8 * threadIdx.x + 2048 * i);
+        ss = block_sum<4, false>(ss, red);
+        factor = 1.0f / sqrtf(ss / (float)cols + eps);
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const int64_t c = 8 * threadIdx.x + 2048 * i;
+            if (c < nb * kFp8Block) finish(v[i], g[i], c);
+        }
+    } else {
+        for (int64_t c = 8 * threadIdx.x; c < nb * kFp8Block; c += 2048)
+            add(load8<false>(xr, c, cols, whole), residual ? load8(rr, c, cols, whole) : none, c);
+        ss = block_sum<4, false>(ss, red);
+        factor = 1.0f / sqrtf(ss / (float)cols + eps);
+        for (int64_t c = 8 * threadIdx.x; c < nb * kFp8Block; c += 2048)
+            finish(load8<false>(residual ? sr : xr, c, cols, whole), load8<false>(w, c, cols, w_whole), c);
     }
 }
 
@@ -241,75 +281,95 @@ int32_t launch_rmsnorm_fp8(hipStream_t s, const void *x, int64_t x_stride, const
                            int64_t sum_stride, const void *w, float eps, int64_t rows, int64_t cols, void *q, float *scales) {
     if (rows > 0x7fffffff) return fail(AESIR_ERR_UNSUPPORTED, "rmsnorm_fp8: too many rows");
     const bool whole = whole_rows(cols, x_stride, x) && (!residual || (whole_rows(cols, res_stride, residual) && whole_rows(cols, sum_stride, sum)));
-    hipLaunchKernelGGL(fp8_norm_kernel, dim3((unsigned)rows), dim3(256), 0, s, (const h16 *)x, x_stride, (const h16 *)residual,
-                       res_stride, (h16 *)sum, sum_stride, (const h16 *)w, eps, rows, cols, whole, whole_rows(cols, 8, w),
-                       (uint8_t *)q, scales);
+    const auto kernel = cols <= 2048 ? fp8_norm_kernel<1> : cols <= 4096 ? fp8_norm_kernel<2> : cols <= 8192 ? fp8_norm_kernel<4> : fp8_norm_kernel<0>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(256), 0, s, (const h16 *)x, x_stride, (const h16 *)residual, res_stride, (h16 *)sum,
+                       sum_stride, (const h16 *)w, eps, rows, cols, whole, whole_rows(cols, 8, w), (uint8_t *)q, scales);
     AESIR_LAUNCH_CHECK("fp8_norm_kernel");
     return AESIR_OK;
 }
 
 // ------------------------------------------------------------------ SwiGLU
 
-// y = u g / (1 + exp(-g)), at most 4 units of f32's last place off: u g is exact, the exponential is 2^hi (1 + lo ln 2)
-// with hi + lo = -g log2(e), and the quotient is rounded once.
+// y = u g / (1 + exp(-g)), off by at most 7 * 2^-24 of it: u g is exact, the exponential is 2^hi (1 + lo ln 2) with
+// hi + lo = -g log2(e) (the instruction's 2^-23, a product's 2^-24), the sum 2^-24, its reciprocal 2^-23 and the product
+// 2^-24.
 __device__ __forceinline__ float swiglu_f(float g, float u) {
     const float hi = g * -1.44269504088896341f;
-    const float lo = fmaf(g, -1.44269504088896341f, -hi) + g * -1.92596299112661746e-8f;
-    return u * g / (1.0f + __builtin_amdgcn_exp2f(hi) * fmaf(lo, 0.693147180559945309f, 1.0f));
+    const float lo = fmaf(g, -1.92596299112661746e-8f, fmaf(g, -1.44269504088896341f, -hi));
+    const float d = fmaf(__builtin_amdgcn_exp2f(hi), fmaf(lo, 0.693147180559945309f, 1.0f), 1.0f);
+    return u * g * __builtin_amdgcn_rcpf(d);
 }
 __device__ __forceinline__ double swiglu_d(float g, float u) { return (double)u * (double)g / (1.0 + exp(-(double)g)); }
 
 constexpr float kSwigluLeast = 0x1p-64f;  // a block of smaller values is zeros
 
-// 16 lanes a block, as fp8_quantize_kernel. Where a quotient or the maximum is in doubt the block's lanes find all its
-// values in f64.
+// Lanes as in fp8_quantize_kernel. 448 y / a is off by at most 7 + 7 + 4 times 2^-24 of it (y, a, and the roundings of
+// the quotient, the interval's end and the product), less than 2^-19. Where a code or the maximum is in doubt the
+// block's 16 lanes find all its values in f64, so a row's codes and scales do not depend on the rows beside it.
 __global__ __launch_bounds__(256) void fp8_swiglu_kernel(const h16 *__restrict__ gate, int64_t g_stride, const h16 *__restrict__ up,
                                                          int64_t u_stride, int64_t rows, int64_t cols, bool whole,
                                                          uint8_t *__restrict__ q, float *__restrict__ scales) {
-    const int64_t nb = (cols + kFp8Block - 1) / kFp8Block, unit = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
-    if (unit >= rows * nb) return;
-    const int64_t r = unit / nb, b = unit % nb, c = b * kFp8Block + 8 * (threadIdx.x % 16);
-    float g[8], u[8], y[8];
-    unpack8(load8(gate + r * g_stride, c, cols, whole), g);
-    unpack8(load8(up + r * u_stride, c, cols, whole), u);
+    const int64_t nb = (cols + kFp8Block - 1) / kFp8Block, r0 = unit_row(), b = unit_block(), c = b * kFp8Block + 8 * (threadIdx.x % 16);
+    if (b >= nb) return;
+    u32x4 gv[kSteps], uv[kSteps];
 #pragma unroll
-    for (int j = 0; j < 8; j++) y[j] = swiglu_f(g[j], u[j]);
-    const unsigned top = row_max(top_bits(y));
-    const float a = __builtin_bit_cast(float, top);
-    float scale = a >= kSwigluLeast ? a / kE4m3Max : 0.0f;
-    const float inv = a >= kSwigluLeast ? kE4m3Max / a : 0.0f;
-    bool near = fabsf(a - kSwigluLeast) <= 0x1p-84f;
-    float t[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        t[j] = y[j] * inv;
-        near |= near_middle(t[j], 16);
+    for (int i = 0; i < kSteps; i++) {
+        gv[i] = uv[i] = {0, 0, 0, 0};
+        if (r0 + 4 * i < rows) {
+            gv[i] = load8(gate + (r0 + 4 * i) * g_stride, c, cols, whole);
+            uv[i] = load8(up + (r0 + 4 * i) * u_stride, c, cols, whole);
+        }
     }
-    if (row_max(near)) {
-        double yd[8], m = 0.0;
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) {
+        const int64_t r = r0 + 4 * i;
+        if (r >= rows) return;
+        float g[8], u[8], y[8];
+        unpack8(gv[i], g);
+        unpack8(uv[i], u);
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = swiglu_f(g[j], u[j]);
+        const unsigned top = row_max(top_bits(y));
+        const float a = __builtin_bit_cast(float, top);
+        float scale = a >= kSwigluLeast ? a / kE4m3Max : 0.0f;
+        const float inv = a >= kSwigluLeast ? kE4m3Max / a : 0.0f, less = inv * (1.0f - 0x1p-19f), more = inv * (1.0f + 0x1p-19f);
+        float lo[8], hi[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            yd[j] = swiglu_d(g[j], u[j]);
-            m = fmax(m, fabs(yd[j]));
+            lo[j] = y[j] * less;
+            hi[j] = y[j] * more;
         }
+        u32x2 codes = to_e4m3(lo);
+        const u32x2 d = to_e4m3(hi);
+        const bool bad = top >= kInfBits;
+        const bool doubt = ((codes.x ^ d.x) | (codes.y ^ d.y)) != 0 || fabsf(a - kSwigluLeast) <= 0x1p-83f;
+        if (bad) {
+            codes = kNanCodes;
+        } else if (row_max(doubt)) {
+            double yd[8], m = 0.0;
 #pragma unroll
-        for (int i = 1; i < 16; i <<= 1) m = fmax(m, __shfl_xor(m, i));
-        const bool some = m >= (double)kSwigluLeast;
-        scale = some ? (float)(m / 448.0) : 0.0f;
+            for (int j = 0; j < 8; j++) {
+                yd[j] = swiglu_d(g[j], u[j]);
+                m = fmax(m, fabs(yd[j]));
+            }
 #pragma unroll
-        for (int j = 0; j < 8; j++) t[j] = some ? to_odd(yd[j] * 448.0 / m) : 0.0f;
+            for (int k = 1; k < 16; k <<= 1) m = fmax(m, __shfl_xor(m, k));
+            const bool some = m >= (double)kSwigluLeast;
+            scale = some ? (float)(m / 448.0) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) lo[j] = some ? to_odd(yd[j] * 448.0 / m) : 0.0f;
+            codes = to_e4m3(lo);
+        }
+        *reinterpret_cast<u32x2 *>(q + r * nb * kFp8Block + c) = codes;
+        if (threadIdx.x % 16 == 0) scales[b * rows + r] = bad ? __builtin_nanf("") : scale;
     }
-    const bool bad = top >= kInfBits;
-    *reinterpret_cast<u32x2 *>(q + r * nb * kFp8Block + c) = bad ? kNanCodes : to_e4m3(t);
-    if (threadIdx.x % 16 == 0) scales[b * rows + r] = bad ? __builtin_nanf("") : scale;
 }
 
 int32_t launch_swiglu_fp8(hipStream_t s, const void *gate, int64_t g_stride, const void *up, int64_t u_stride, int64_t rows,
                           int64_t cols, void *q, float *scales) {
-    const int64_t groups = (rows * fp8_blocks(cols) + 15) / 16;
-    if (groups > 0x7fffffff) return fail(AESIR_ERR_UNSUPPORTED, "swiglu_fp8: more elements than one launch takes");
-    hipLaunchKernelGGL(fp8_swiglu_kernel, dim3((unsigned)groups), dim3(256), 0, s, (const h16 *)gate, g_stride, (const h16 *)up,
-                       u_stride, rows, cols, whole_rows(cols, g_stride, gate) && whole_rows(cols, u_stride, up), (uint8_t *)q, scales);
+    if ((rows + 4 * kSteps - 1) / (4 * kSteps) > 0x7fffffff) return fail(AESIR_ERR_UNSUPPORTED, "swiglu_fp8: more elements than one launch takes");
+    hipLaunchKernelGGL(fp8_swiglu_kernel, unit_grid(rows, fp8_blocks(cols)), dim3(256), 0, s, (const h16 *)gate, g_stride, (const h16 *)up, u_stride,
+                       rows, cols, whole_rows(cols, g_stride, gate) && whole_rows(cols, u_stride, up), (uint8_t *)q, scales);
     AESIR_LAUNCH_CHECK("fp8_swiglu_kernel");
     return AESIR_OK;
 }
