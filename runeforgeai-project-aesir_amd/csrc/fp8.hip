@@ -642,6 +642,8 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(Fp8Args p) {
     for (int kb = k0; kb < k1; kb++) {
         __builtin_amdgcn_s_waitcnt(vm_wait((S - 2) * kLoads));
         barrier();
+        request(stage == 0 ? S - 1 : stage - 1, kb + S - 1);
+        __builtin_amdgcn_sched_barrier(0);
         const uint8_t *la = lds + stage * kStage + wm * 128, *lb = lds + stage * kStage + kB + wn * 128;
         const float *sc = (const float *)(lds + stage * kStage + kScales);
         const float sb = sc[BM + wn / 128];
@@ -654,9 +656,6 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(Fp8Args p) {
             s[j] = sc[wm + 16 * j + i16] * sb;
             if (j == 0) b[1] = read_frag<EXACT>(lb + 2048, at);
         }
-        __builtin_amdgcn_sched_barrier(0);
-        request(stage == 0 ? S - 1 : stage - 1, kb + S - 1);
-        __builtin_amdgcn_sched_barrier(0);
         // a product is added to its sum when the two after it have been issued; a row of B's fragment is read two rows ahead
         constexpr int D = 3, kBehind = 2;
         f32x4 d[D];
