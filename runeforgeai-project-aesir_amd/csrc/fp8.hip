@@ -6,6 +6,10 @@
 // ties to even. The kernels find t = 448 y / a in f32, a few units of its last place off, and round both ends of an
 // interval that holds the exact quotient: rounding is monotone, so where both give the same code so does the quotient.
 // Elsewhere (one element in some 10^5) it is found again in f64, so that every code is the one of the formula.
+#include <algorithm>
+#include <cmath>
+#include <limits>
+
 #include "device.hpp"
 #include "kernels.hpp"
 #include "mfma_gemm.hpp"
@@ -130,16 +134,19 @@ static int64_t fp8_blocks(int64_t cols) { return (cols + kFp8Block - 1) / kFp8Bl
 
 // ------------------------------------------------------------------ quantize
 
+// Rows that one launch takes: a launch has less than 2^32 threads.
+constexpr int64_t kLaunchRows = (int64_t)1 << 23;
+
 // 16 lanes a block, 8 neighbouring elements each; a wave has 4 blocks of a row, a workgroup 4 rows at a time, kSteps
 // times, all of them requested at first.
 constexpr int kSteps = 2;
-__device__ __forceinline__ int64_t unit_row() { return (int64_t)blockIdx.x * (4 * kSteps) + threadIdx.x / 64; }
+__device__ __forceinline__ int64_t unit_row(int64_t first) { return first + (int64_t)blockIdx.x * (4 * kSteps) + threadIdx.x / 64; }
 __device__ __forceinline__ int64_t unit_block() { return (int64_t)blockIdx.y * 4 + threadIdx.x % 64 / 16; }
 static dim3 unit_grid(int64_t rows, int64_t nb) { return dim3((unsigned)((rows + 4 * kSteps - 1) / (4 * kSteps)), (unsigned)((nb + 3) / 4)); }
 
-__global__ __launch_bounds__(256) void fp8_quantize_kernel(const h16 *__restrict__ x, int64_t stride, int64_t rows, int64_t cols,
-                                                           bool whole, uint8_t *__restrict__ q, float *__restrict__ scales) {
-    const int64_t nb = (cols + kFp8Block - 1) / kFp8Block, r0 = unit_row(), b = unit_block(), c = b * kFp8Block + 8 * (threadIdx.x % 16);
+__global__ __launch_bounds__(256) void fp8_quantize_kernel(const h16 *__restrict__ x, int64_t stride, int64_t first, int64_t rows,
+                                                           int64_t cols, bool whole, uint8_t *__restrict__ q, float *__restrict__ scales) {
+    const int64_t nb = (cols + kFp8Block - 1) / kFp8Block, r0 = unit_row(first), b = unit_block(), c = b * kFp8Block + 8 * (threadIdx.x % 16);
     if (b >= nb) return;
     u32x4 v[kSteps];
 #pragma unroll
@@ -193,15 +200,20 @@ __global__ __launch_bounds__(256) void fp8_quantize_weight_kernel(const h16 *__r
 int32_t launch_quantize_fp8(hipStream_t s, const void *x, int64_t stride, int64_t rows, int64_t cols, bool weight, void *q,
                             float *scales) {
     const bool whole = whole_rows(cols, stride, x);
-    const int64_t nb = fp8_blocks(cols), groups = weight ? (rows + 127) / 128 * nb : (rows + 4 * kSteps - 1) / (4 * kSteps);
-    if (groups > 0x7fffffff) return fail(AESIR_ERR_UNSUPPORTED, "quantize_fp8: more elements than one launch takes");
-    if (weight)
-        hipLaunchKernelGGL(fp8_quantize_weight_kernel, dim3((unsigned)groups), dim3(256), 0, s, (const h16 *)x, stride, rows, cols,
-                           whole, (uint8_t *)q, scales);
-    else
-        hipLaunchKernelGGL(fp8_quantize_kernel, unit_grid(rows, nb), dim3(256), 0, s, (const h16 *)x, stride, rows, cols, whole,
+    const int64_t nb = fp8_blocks(cols);
+    if (weight) {
+        const int64_t groups = (rows + 127) / 128 * nb;
+        if (groups >= 1 << 24) return fail(AESIR_ERR_UNSUPPORTED, "quantize_fp8: more elements than one launch takes");
+        hipLaunchKernelGGL(fp8_quantize_weight_kernel, dim3((unsigned)groups), dim3(256), 0, s, (const h16 *)x, stride, rows, cols, whole,
                            (uint8_t *)q, scales);
-    AESIR_LAUNCH_CHECK("fp8_quantize_kernel");
+        AESIR_LAUNCH_CHECK("fp8_quantize_weight_kernel");
+        return AESIR_OK;
+    }
+    for (int64_t first = 0; first < rows; first += kLaunchRows) {
+        hipLaunchKernelGGL(fp8_quantize_kernel, unit_grid(std::min(rows - first, kLaunchRows), nb), dim3(256), 0, s, (const h16 *)x, stride, first,
+                           rows, cols, whole, (uint8_t *)q, scales);
+        AESIR_LAUNCH_CHECK("fp8_quantize_kernel");
+    }
     return AESIR_OK;
 }
 
@@ -212,11 +224,11 @@ int32_t launch_quantize_fp8(hipStream_t s, const void *x, int64_t stride, int64_
 // V: groups of 2048 columns, which stay in registers; 0: any number of them, read twice.
 template <int V>
 __global__ __launch_bounds__(256) void fp8_norm_kernel(const h16 *x, int64_t x_stride, const h16 *residual, int64_t res_stride, h16 *sum,
-                                                       int64_t sum_stride, const h16 *__restrict__ w, float eps, int64_t rows,
-                                                       int64_t cols, bool whole, bool w_whole, uint8_t *__restrict__ q,
+                                                       int64_t sum_stride, const h16 *__restrict__ w, float eps, int64_t first,
+                                                       int64_t rows, int64_t cols, bool whole, bool w_whole, uint8_t *__restrict__ q,
                                                        float *__restrict__ scales) {
     __shared__ float red[4];
-    const int64_t r = blockIdx.x, nb = (cols + kFp8Block - 1) / kFp8Block;
+    const int64_t r = first + blockIdx.x, nb = (cols + kFp8Block - 1) / kFp8Block;
     const h16 *xr = x + r * x_stride, *rr = residual + r * res_stride;
     h16 *sr = sum + r * sum_stride;
     float ss = 0.0f;
@@ -279,12 +291,14 @@ __global__ __launch_bounds__(256) void fp8_norm_kernel(const h16 *x, int64_t x_s
 
 int32_t launch_rmsnorm_fp8(hipStream_t s, const void *x, int64_t x_stride, const void *residual, int64_t res_stride, void *sum,
                            int64_t sum_stride, const void *w, float eps, int64_t rows, int64_t cols, void *q, float *scales) {
-    if (rows > 0x7fffffff) return fail(AESIR_ERR_UNSUPPORTED, "rmsnorm_fp8: too many rows");
     const bool whole = whole_rows(cols, x_stride, x) && (!residual || (whole_rows(cols, res_stride, residual) && whole_rows(cols, sum_stride, sum)));
     const auto kernel = cols <= 2048 ? fp8_norm_kernel<1> : cols <= 4096 ? fp8_norm_kernel<2> : cols <= 8192 ? fp8_norm_kernel<4> : fp8_norm_kernel<0>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(256), 0, s, (const h16 *)x, x_stride, (const h16 *)residual, res_stride, (h16 *)sum,
-                       sum_stride, (const h16 *)w, eps, rows, cols, whole, whole_rows(cols, 8, w), (uint8_t *)q, scales);
-    AESIR_LAUNCH_CHECK("fp8_norm_kernel");
+    for (int64_t first = 0; first < rows; first += kLaunchRows) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(rows - first, kLaunchRows)), dim3(256), 0, s, (const h16 *)x, x_stride,
+                           (const h16 *)residual, res_stride, (h16 *)sum, sum_stride, (const h16 *)w, eps, first, rows, cols, whole,
+                           whole_rows(cols, 8, w), (uint8_t *)q, scales);
+        AESIR_LAUNCH_CHECK("fp8_norm_kernel");
+    }
     return AESIR_OK;
 }
 
@@ -307,9 +321,9 @@ constexpr float kSwigluLeast = 0x1p-64f;  // a block of smaller values is zeros
 // the quotient, the interval's end and the product), less than 2^-19. Where a code or the maximum is in doubt the
 // block's 16 lanes find all its values in f64, so a row's codes and scales do not depend on the rows beside it.
 __global__ __launch_bounds__(256) void fp8_swiglu_kernel(const h16 *__restrict__ gate, int64_t g_stride, const h16 *__restrict__ up,
-                                                         int64_t u_stride, int64_t rows, int64_t cols, bool whole,
+                                                         int64_t u_stride, int64_t first, int64_t rows, int64_t cols, bool whole,
                                                          uint8_t *__restrict__ q, float *__restrict__ scales) {
-    const int64_t nb = (cols + kFp8Block - 1) / kFp8Block, r0 = unit_row(), b = unit_block(), c = b * kFp8Block + 8 * (threadIdx.x % 16);
+    const int64_t nb = (cols + kFp8Block - 1) / kFp8Block, r0 = unit_row(first), b = unit_block(), c = b * kFp8Block + 8 * (threadIdx.x % 16);
     if (b >= nb) return;
     u32x4 gv[kSteps], uv[kSteps];
 #pragma unroll
@@ -367,10 +381,12 @@ __global__ __launch_bounds__(256) void fp8_swiglu_kernel(const h16 *__restrict__
 
 int32_t launch_swiglu_fp8(hipStream_t s, const void *gate, int64_t g_stride, const void *up, int64_t u_stride, int64_t rows,
                           int64_t cols, void *q, float *scales) {
-    if ((rows + 4 * kSteps - 1) / (4 * kSteps) > 0x7fffffff) return fail(AESIR_ERR_UNSUPPORTED, "swiglu_fp8: more elements than one launch takes");
-    hipLaunchKernelGGL(fp8_swiglu_kernel, unit_grid(rows, fp8_blocks(cols)), dim3(256), 0, s, (const h16 *)gate, g_stride, (const h16 *)up, u_stride,
-                       rows, cols, whole_rows(cols, g_stride, gate) && whole_rows(cols, u_stride, up), (uint8_t *)q, scales);
-    AESIR_LAUNCH_CHECK("fp8_swiglu_kernel");
+    const bool whole = whole_rows(cols, g_stride, gate) && whole_rows(cols, u_stride, up);
+    for (int64_t first = 0; first < rows; first += kLaunchRows) {
+        hipLaunchKernelGGL(fp8_swiglu_kernel, unit_grid(std::min(rows - first, kLaunchRows), fp8_blocks(cols)), dim3(256), 0, s, (const h16 *)gate,
+                           g_stride, (const h16 *)up, u_stride, first, rows, cols, whole, (uint8_t *)q, scales);
+        AESIR_LAUNCH_CHECK("fp8_swiglu_kernel");
+    }
     return AESIR_OK;
 }
 
@@ -782,18 +798,20 @@ struct TileCost {
 constexpr TileCost kTiles[] = {{64, 64, 2, 0.28f, 0.38f}, {128, 128, 1, 0.56f, 0.56f}, {192, 128, 1, 0.72f, 0.72f}, {128, 128, 2, 0.8f, 1.07f}, {256, 256, 1, 1.73f, 1.73f}};
 constexpr TileCost kExactTiles[] = {{64, 64, 2, 0.43f, 0.66f}, {128, 128, 1, 1.12f, 1.12f}, {128, 128, 2, 1.4f, 1.85f}};
 
-// The tile and the number of stretches of k that the product is cut into, by the time that they come to: rounds of
+constexpr int64_t kLaunchGroups = (1 << 23) - 1;  // a launch has less than 2^32 threads, a workgroup up to 512
+
+// The tile and the number of stretches of k that the product is cut into (-1: none in one launch), by the time that they come to: rounds of
 // workgroups, or what A and B take from memory at 4.5 TB/s where that is more, 4.5 us around each round, and for the
 // stretches' sums another launch and their bytes.
 template <int N>
 static int choose_tile(const TileCost (&tiles)[N], const Fp8Args &p, int64_t part_floats, int *splits) {
-    int best = 0;
-    float least = 1e30f;
+    int best = -1;
+    float least = std::numeric_limits<float>::infinity();
     *splits = 1;
     for (int i = 0; i < N; i++) {
         const TileCost &c = tiles[i];
         const int64_t count = (p.M + c.bm - 1) / c.bm * ((p.N + c.bn - 1) / c.bn);
-        for (int z = 1; z <= 8 && (z == 1 || (p.nb >= 4 * z && p.M * p.N <= part_floats / z)); z *= 2) {
+        for (int z = 1; z <= 8 && count * z <= kLaunchGroups && (z == 1 || (p.nb >= 4 * z && p.M * p.N <= part_floats / z)); z *= 2) {
             const int64_t all = count * z, rounds = (all + 256 * c.per_cu - 1) / (256 * c.per_cu);
             const float step = all <= 256 ? c.one : c.full, blocks = (float)((p.nb + z - 1) / z);
             const float work = fmaxf((float)rounds * blocks * step, (float)(p.M + p.N) * (float)p.nb * (128 / 4.5e6f));
@@ -812,7 +830,8 @@ int32_t launch_gemm_fp8(hipStream_t s, const void *A, const float *as, int64_t M
                         int64_t K, void *C, bool f32, int64_t ldc, float *part, int64_t part_floats) {
     const bool quad = ldc % (f32 ? 4 : 8) == 0 && ((uintptr_t)C & 15) == 0;
     Fp8Args p{(const uint8_t *)A, (const uint8_t *)B, as, bs, C, M, N, ldc, (int)fp8_blocks(K), 1, part, f32, quad};
-    if ((M + 63) / 64 > 0x7fffffff / ((N + 15) / 16)) return fail(AESIR_ERR_UNSUPPORTED, "gemm_fp8: output larger than one launch takes");
+    const auto too_large = [] { return fail(AESIR_ERR_UNSUPPORTED, "gemm_fp8: output larger than one launch takes"); };
+    if (M <= 64 && (N + 15) / 16 > kLaunchGroups) return too_large();
     if (M <= 16) return M <= 8 ? stream_16<1>(s, p) : stream_16<2>(s, p);
     if (M <= 64) {
         // Tiles of 64 x 64 share the rows of A among 64 of B: they pay once they fill half the CUs, by B's rows (64 rows
@@ -826,14 +845,16 @@ int32_t launch_gemm_fp8(hipStream_t s, const void *A, const float *as, int64_t M
     if (f32) switch (choose_tile(kExactTiles, p, part_floats, &p.splits)) {
         case 0: return tile<64, 64, 2, 2, 4, true>(s, p);
         case 1: return tile<128, 128, 4, 2, 3, true>(s, p);
-        default: return tile<128, 128, 2, 2, 2, true>(s, p);
+        case 2: return tile<128, 128, 2, 2, 2, true>(s, p);
+        default: return too_large();
     }
     switch (choose_tile(kTiles, p, part_floats, &p.splits)) {
         case 0: return tile<64, 64, 2, 2, 4, false>(s, p);
         case 1: return tile<128, 128, 4, 2, 3, false>(s, p);
         case 2: return tile<192, 128, 4, 2, 3, false>(s, p);
         case 3: return tile<128, 128, 2, 2, 2, false>(s, p);
-        default: return tile<256, 256, 4, 2, 2, false>(s, p);
+        case 4: return tile<256, 256, 4, 2, 2, false>(s, p);
+        default: return too_large();
     }
 }
 

@@ -126,6 +126,11 @@ refused(-1, n + ": output is not aligned to its type", g, q, b, T(c, shift=1))
 refused(-1, n + ": output is not aligned to its type", g, q, b, A.Tensor(ctx, c.ptr + 2, 4, 200, np.float32))
 refused(-7, n + ": output type must be F16 or F32", g, q, b, A.Tensor(ctx, c.ptr, 4, 200, np.float64))
 refused(-7, n + ": output too large", g, q, b, T(c, cols=1 << 61))
+for m in (4, 30, 64):
+    refused(-7, n + ": output larger than one launch takes", g, Q(q, rows=m), Q(b, rows=1 << 28), T(c, rows=m, cols=1 << 28))
+for t in (c, A.Tensor(ctx, c.ptr, 4, 200, np.float32)):
+    refused(-7, n + ": output larger than one launch takes", g, Q(q, rows=1 << 36), b, T(t, rows=1 << 36))
+refused(-7, "quantize_fp8: more elements than one launch takes", A.quantize_fp8, T(x, rows=1 << 36), Q(b, rows=1 << 36))
 refused(-2, n + ": activations have blocks of one row", g, b, b, T(c, rows=200))
 refused(-2, n + ": weights have blocks of 128 rows", g, q, q, T(c, cols=4))
 """

@@ -330,6 +330,36 @@ def test_product_of_whole_numbers(A, ctx, M, N, K):
     assert np.array_equal(got, (values(*a) @ values(*b, 128).T).astype(np.float32))
 
 
+@pytest.mark.parametrize("M", [1, 9, 40, 70, 300, 2000])
+def test_every_code(A, ctx, M):
+    """Each code alone in its row, times one: every product is that number, in both types."""
+    rows = np.arange(M)
+    codes, scales = np.zeros((M, 384), np.uint8), np.ones((3, M), np.float32)
+    ones = np.full((256, 384), nearest(np.array([1.0]))[0], np.uint8)
+    for first in range(0, 256, 128 if M < 256 else 256):
+        codes[:] = 0
+        c = (first + rows) % 256
+        c = np.where(c & 127 == 127, 0, c).astype(np.uint8)
+        codes[rows, (7 * rows) % 384] = c
+        for f32 in (True, False):
+            got = product(A, ctx, (codes, scales), (ones, np.ones((2, 3), np.float32)), 384, f32)
+            assert np.array_equal(got, np.repeat(NUMBERS[c][:, None], 256, 1).astype(got.dtype))
+
+
+@pytest.mark.parametrize("M,N", [(1, 40), (20, 40), (40, 130), (70, 130)])
+def test_long_rows(A, ctx, M, N):
+    """A quarter of a million columns of whole numbers: exact sums, in stretches too."""
+    K = (1 << 18) - 5
+    rng = np.random.default_rng(M)
+    ones = nearest(np.arange(-2.0, 3.0))
+    values8 = [rng.integers(0, 5, (n, K)) for n in (M, N)]
+    nb = -(-K // 128)
+    a, b = (np.zeros((n, nb * 128), np.uint8) for n in (M, N))
+    a[:, :K], b[:, :K] = ones[values8[0]], ones[values8[1]]
+    got = product(A, ctx, (a, np.ones((nb, M), np.float32)), (b, np.ones((-(-N // 128), nb), np.float32)), K, True)
+    assert np.array_equal(got, (values8[0] - 2.0).astype(np.float32) @ (values8[1] - 2.0).T.astype(np.float32))
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 300, 512), (20, 300, 512), (64, 500, 384), (150, 300, 640), (520, 700, 256)])
 def test_product_nan_stays_in_its_rows(A, ctx, M, N, K):
     """A NaN code or scale reaches its row of A or its rows of B, and nothing else."""
@@ -382,6 +412,22 @@ def test_offsets_past_32_bits(A):
         assert same_codes(A.Tensor(ctx, t.ptr + (rows - last) * cols, last, cols, np.uint8).numpy(), codes)
         A.swiglu_fp8(ctx, tx, tx, t)
         assert same_codes(A.Tensor(ctx, t.ptr + (rows - last) * cols, last, cols, np.uint8).numpy(), swiglu64(x, x)[0])
+
+
+def test_more_rows_than_a_launch_takes(A):
+    """The row calls past 2^23 rows: first, last and middle rows, whose scales lie far apart."""
+    rows, cols = (1 << 23) + 1000, 40
+    rng = np.random.default_rng(8)
+    x = rng.standard_normal((rows, cols), dtype=np.float32).astype(np.float16)
+    at = np.r_[0:50, (1 << 23) - 50:(1 << 23) + 50, rows - 50:rows]
+    w = rng.standard_normal(cols).astype(np.float16)
+    with A.Context(4 << 30) as ctx:
+        t, tx, tw = A.FP8Tensor.empty(ctx, rows, cols), ctx.from_numpy(x), ctx.from_numpy(w)
+        for call, want in ((lambda: A.quantize_fp8(ctx, tx, t), quantize(x[at].astype(np.float64))), (lambda: A.swiglu_fp8(ctx, tx, tx, t), swiglu64(x[at], x[at])),
+                           (lambda: A.rmsnorm_fp8(ctx, tx, tw, t), norm64(x[at], None, w[None], 1e-5)[1:])):
+            call()
+            assert same_codes(t.codes()[at], want[0])
+            assert np.allclose(t.scales()[:, at], want[1], rtol=1e-6, atol=0)
 
 
 # ------------------------------------------------------------------ a layer's MLP
