@@ -74,12 +74,13 @@ __device__ __forceinline__ unsigned wave_max_u(unsigned m) {
 constexpr u32x2 kNanCodes = {0x7f7f7f7fu, 0x7f7f7f7fu};
 
 // Codes of 8 values p that are exact in f32 with at most 22 bits (f16 numbers or products of two), top the bits of
-// their block's largest |p|. p times 448 / a, itself rounded once, is off by less than 2^-22 of it; 448 p is exact in
-// f64, and a quotient that is not the middle of two codes is at least 2^-28 of it away from one.
+// their block's largest |p|. p times 448 / a is off by at most 2^-22 of it (the reciprocal's 2^-23 and two products'
+// 2^-24), so that the ends of an interval 2^-21 either way hold it; 448 p is exact in f64, and a quotient that is not the
+// middle of two codes is at least 2^-28 of it away from one.
 __device__ __forceinline__ u32x2 codes_of(const float (&p)[8], unsigned top) {
     if (top >= kInfBits) return kNanCodes;
-    const float a = __builtin_bit_cast(float, top), inv = top ? kE4m3Max / a : 0.0f;
-    const float less = inv * (1.0f - 0x1p-22f), more = inv * (1.0f + 0x1p-22f);
+    const float a = __builtin_bit_cast(float, top), inv = top ? __builtin_amdgcn_rcpf(a) : 0.0f;
+    const float less = inv * (kE4m3Max * (1.0f - 0x1p-21f)), more = inv * (kE4m3Max * (1.0f + 0x1p-21f));
     float lo[8], hi[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -96,7 +97,7 @@ __device__ __forceinline__ u32x2 codes_of(const float (&p)[8], unsigned top) {
 // ------------------------------------------------------------------ rows
 
 // 8 f16 elements of a row from column c on, zeros behind its `cols`. whole: every row holds whole, 16-byte aligned
-// groups of 8. ONCE: nothing reads them again (non-temporal: SwiGLU of 4096 x 14336 67 -> 60 us).
+// groups of 8. ONCE: nothing reads them again (non-temporal: SwiGLU of 4096 x 14336 60 us against 67).
 template <bool ONCE = true>
 __device__ __forceinline__ u32x4 load8(const h16 *row, int64_t c, int64_t cols, bool whole) {
     u32x4 v = {0, 0, 0, 0};
@@ -137,27 +138,40 @@ static int64_t fp8_blocks(int64_t cols) { return (cols + kFp8Block - 1) / kFp8Bl
 // Rows that one launch takes: a launch has less than 2^32 threads.
 constexpr int64_t kLaunchRows = (int64_t)1 << 23;
 
-// 16 lanes a block, 8 neighbouring elements each; a wave has 4 blocks of a row, a workgroup 4 rows at a time, kSteps
-// times, all of them requested at first. 2048 x 4096 in 8.9 us: a wave's latency and the 20 instructions an element
-// of waves that all start at once (1 step 8.9, 4 steps 9.8).
+// 16 lanes a block, 8 neighbouring elements each; a workgroup has 1 << wide blocks of 16 >> wide rows at a time, kSteps
+// times, all of them requested at first. Large matrices go faster by longer runs of a row, small ones by rows whose scales
+// lie side by side: SwiGLU with wide 4 / 2, us: 4096 x 14336 56.1 / 60.6, 8192 x 4096 33.2 / 34.9, 4096 x 5632 25.5 / 25.0,
+// 65536 x 256 31.3 / 28.2. Rows of 2048 x 4096 are quantized in 8.9 us, 2.7 of them the stores, the rest a wave's latency
+// (1 step 8.9, 4 steps 9.8).
 constexpr int kSteps = 2;
-__device__ __forceinline__ int64_t unit_row(int64_t first) { return first + (int64_t)blockIdx.x * (4 * kSteps) + threadIdx.x / 64; }
-__device__ __forceinline__ int64_t unit_block() { return (int64_t)blockIdx.y * 4 + threadIdx.x % 64 / 16; }
-static dim3 unit_grid(int64_t rows, int64_t nb) { return dim3((unsigned)((rows + 4 * kSteps - 1) / (4 * kSteps)), (unsigned)((nb + 3) / 4)); }
+struct Unit {
+    int64_t row, block;
+    int step;  // rows between a thread's steps
+};
+__device__ __forceinline__ Unit unit_of(int64_t first, int wide) {
+    const int g = threadIdx.x / 16, step = 16 >> wide;
+    return {first + (int64_t)blockIdx.x * (step * kSteps) + (g >> wide), ((int64_t)blockIdx.y << wide) + (g & ((1 << wide) - 1)), step};
+}
+static int unit_wide(int64_t rows, int64_t nb) { return nb >= 16 && rows * nb >= 1 << 18 ? 4 : 2; }
+static dim3 unit_grid(int64_t rows, int64_t nb, int wide) {
+    const int64_t step = (16 >> wide) * kSteps;
+    return dim3((unsigned)((rows + step - 1) / step), (unsigned)((nb + (1 << wide) - 1) >> wide));
+}
 
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(const h16 *__restrict__ x, int64_t stride, int64_t first, int64_t rows,
-                                                           int64_t cols, bool whole, uint8_t *__restrict__ q, float *__restrict__ scales) {
-    const int64_t nb = (cols + kFp8Block - 1) / kFp8Block, r0 = unit_row(first), b = unit_block(), c = b * kFp8Block + 8 * (threadIdx.x % 16);
+                                                           int64_t cols, int wide, bool whole, uint8_t *__restrict__ q, float *__restrict__ scales) {
+    const Unit u8 = unit_of(first, wide);
+    const int64_t nb = (cols + kFp8Block - 1) / kFp8Block, r0 = u8.row, b = u8.block, c = b * kFp8Block + 8 * (threadIdx.x % 16);
     if (b >= nb) return;
     u32x4 v[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
         v[i] = {0, 0, 0, 0};
-        if (r0 + 4 * i < rows) v[i] = load8(x + (r0 + 4 * i) * stride, c, cols, whole);
+        if (r0 + u8.step * i < rows) v[i] = load8(x + (r0 + u8.step * i) * stride, c, cols, whole);
     }
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
-        const int64_t r = r0 + 4 * i;
+        const int64_t r = r0 + u8.step * i;
         if (r >= rows) return;
         float p[8];
         unpack8(v[i], p);
@@ -211,9 +225,10 @@ int32_t launch_quantize_fp8(hipStream_t s, const void *x, int64_t stride, int64_
         AESIR_LAUNCH_CHECK("fp8_quantize_weight_kernel");
         return AESIR_OK;
     }
+    const int wide = unit_wide(rows, nb);
     for (int64_t first = 0; first < rows; first += kLaunchRows) {
-        hipLaunchKernelGGL(fp8_quantize_kernel, unit_grid(std::min(rows - first, kLaunchRows), nb), dim3(256), 0, s, (const h16 *)x, stride, first,
-                           rows, cols, whole, (uint8_t *)q, scales);
+        hipLaunchKernelGGL(fp8_quantize_kernel, unit_grid(std::min(rows - first, kLaunchRows), nb, wide), dim3(256), 0, s, (const h16 *)x, stride,
+                           first, rows, cols, wide, whole, (uint8_t *)q, scales);
         AESIR_LAUNCH_CHECK("fp8_quantize_kernel");
     }
     return AESIR_OK;
@@ -320,27 +335,28 @@ __device__ __forceinline__ double swiglu_d(float g, float u) { return (double)u 
 
 constexpr float kSwigluLeast = 0x1p-64f;  // a block of smaller values is zeros
 
-// Lanes as in fp8_quantize_kernel. 448 y / a is off by at most 7 + 7 + 4 times 2^-24 of it (y, a, and the roundings of
-// the quotient, the interval's end and the product), less than 2^-19. Where a code or the maximum is in doubt the
+// Lanes as in fp8_quantize_kernel. 448 y / a is off by at most 7 + 7 + 4 times 2^-24 of it (y, a, the reciprocal and two
+// products), less than 2^-19. Where a code or the maximum is in doubt the
 // block's 16 lanes find all its values in f64, so a row's codes and scales do not depend on the rows beside it.
-// 4096 x 14336 in 60 us, 4.9 TB/s; a copy of as many bytes takes 58.
+// 4096 x 14336 in 56 us, 5.3 TB/s; a copy of as many bytes takes 58.
 __global__ __launch_bounds__(256) void fp8_swiglu_kernel(const h16 *__restrict__ gate, int64_t g_stride, const h16 *__restrict__ up,
-                                                         int64_t u_stride, int64_t first, int64_t rows, int64_t cols, bool whole,
+                                                         int64_t u_stride, int64_t first, int64_t rows, int64_t cols, int wide, bool whole,
                                                          uint8_t *__restrict__ q, float *__restrict__ scales) {
-    const int64_t nb = (cols + kFp8Block - 1) / kFp8Block, r0 = unit_row(first), b = unit_block(), c = b * kFp8Block + 8 * (threadIdx.x % 16);
+    const Unit u8 = unit_of(first, wide);
+    const int64_t nb = (cols + kFp8Block - 1) / kFp8Block, r0 = u8.row, b = u8.block, c = b * kFp8Block + 8 * (threadIdx.x % 16);
     if (b >= nb) return;
     u32x4 gv[kSteps], uv[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
         gv[i] = uv[i] = {0, 0, 0, 0};
-        if (r0 + 4 * i < rows) {
-            gv[i] = load8(gate + (r0 + 4 * i) * g_stride, c, cols, whole);
-            uv[i] = load8(up + (r0 + 4 * i) * u_stride, c, cols, whole);
+        if (r0 + u8.step * i < rows) {
+            gv[i] = load8(gate + (r0 + u8.step * i) * g_stride, c, cols, whole);
+            uv[i] = load8(up + (r0 + u8.step * i) * u_stride, c, cols, whole);
         }
     }
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
-        const int64_t r = r0 + 4 * i;
+        const int64_t r = r0 + u8.step * i;
         if (r >= rows) return;
         float g[8], u[8], y[8];
         unpack8(gv[i], g);
@@ -350,7 +366,8 @@ __global__ __launch_bounds__(256) void fp8_swiglu_kernel(const h16 *__restrict__
         const unsigned top = row_max(top_bits(y));
         const float a = __builtin_bit_cast(float, top);
         float scale = a >= kSwigluLeast ? a / kE4m3Max : 0.0f;
-        const float inv = a >= kSwigluLeast ? kE4m3Max / a : 0.0f, less = inv * (1.0f - 0x1p-19f), more = inv * (1.0f + 0x1p-19f);
+        const float inv = a >= kSwigluLeast ? __builtin_amdgcn_rcpf(a) : 0.0f;
+        const float less = inv * (kE4m3Max * (1.0f - 0x1p-19f)), more = inv * (kE4m3Max * (1.0f + 0x1p-19f));
         float lo[8], hi[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -386,9 +403,11 @@ __global__ __launch_bounds__(256) void fp8_swiglu_kernel(const h16 *__restrict__
 int32_t launch_swiglu_fp8(hipStream_t s, const void *gate, int64_t g_stride, const void *up, int64_t u_stride, int64_t rows,
                           int64_t cols, void *q, float *scales) {
     const bool whole = whole_rows(cols, g_stride, gate) && whole_rows(cols, u_stride, up);
+    const int64_t nb = fp8_blocks(cols);
+    const int wide = unit_wide(rows, nb);
     for (int64_t first = 0; first < rows; first += kLaunchRows) {
-        hipLaunchKernelGGL(fp8_swiglu_kernel, unit_grid(std::min(rows - first, kLaunchRows), fp8_blocks(cols)), dim3(256), 0, s, (const h16 *)gate,
-                           g_stride, (const h16 *)up, u_stride, first, rows, cols, whole, (uint8_t *)q, scales);
+        hipLaunchKernelGGL(fp8_swiglu_kernel, unit_grid(std::min(rows - first, kLaunchRows), nb, wide), dim3(256), 0, s, (const h16 *)gate, g_stride,
+                           (const h16 *)up, u_stride, first, rows, cols, wide, whole, (uint8_t *)q, scales);
         AESIR_LAUNCH_CHECK("fp8_swiglu_kernel");
     }
     return AESIR_OK;
@@ -498,7 +517,7 @@ __device__ __forceinline__ auto read_frag(const uint8_t *rows, int at) {
 // 64 bytes, cost the address unit 50 cycles each (1 x 28672 x 4096 23.6 us against 20.7). A stage is read no earlier than
 // its copies are counted down, and a fragment read in one turn feeds a product of that turn, so it is in registers when
 // the next turn gives its stage away. Measured: 1 x 6144 x 4096 in 6.4 us, 1 x 57344 x 8192 in 68 (6.9 TB/s), 16 x 32000 x
-// 2048 to f32 in 13.3; memory's rate and 3 to 4 us of starting and ending bound it.
+// 2048 to f32 in 12.1; memory's rate and 3 to 4 us of starting and ending bound it.
 template <int MH, int NR, int W, int S, bool EXACT>
 __global__ __launch_bounds__(64 * W) void fp8_stream_kernel(Fp8Args p) {
     constexpr int MT = (MH + 1) / 2, kA = NR * 2048, kScales = kA + MH * 1024, kStage = kScales + 512, kLoads = 2 * NR + MH + 2;
@@ -787,11 +806,13 @@ static int32_t tile(hipStream_t s, const Fp8Args &p) {
 // Up to 16 rows of A: memory's rate decides. More rows of B a workgroup (NR) are fewer workgroups and fewer copies of A,
 // and pay where B alone fills the 256 CUs; long rows want 8 waves along k. Measured, us of 1 / 16 rows, by NR and waves:
 // 4096 x 4096 NR 1, 4 waves 5.3 / 5.7, NR 2 6.0 / 6.6; 6144 x 4096 7.0 / 8.2, NR 2 6.8 / 7.3; 28672 x 4096 21.7 / 25.7, NR 4
-// 20.8 / 23.1; 4096 x 14336 NR 1, 4 waves 11.3 / 12.4, 8 waves 10.8 / 13.0; 57344 x 8192 8 waves 68 / 83, NR 4 81 / 87.
+// 20.8 / 23.1; 32000 x 2048 NR 4 12.0 / 13.5, NR 2 11.6 / 12.4; 4096 x 14336 NR 1, 4 waves 11.3 / 12.4, 8 waves 10.8 / 13.0;
+// 57344 x 8192 8 waves 68 / 83, NR 4 81 / 87.
 template <int MH>
 static int32_t stream_16(hipStream_t s, const Fp8Args &p) {
     if (p.N > 4096) {
         if (p.N <= 8192 && p.nb <= 64) return stream<MH, 2, 4, 3, true>(s, p);
+        if (p.N > 8192 && p.nb <= 16) return stream<MH, 2, 4, 2, true>(s, p);
         if (p.N > 8192 && p.nb <= 32) return stream<MH, 4, 4, 2, true>(s, p);
     } else if (p.nb <= 32) {
         return stream<MH, 1, 4, 3, true>(s, p);

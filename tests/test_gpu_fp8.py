@@ -414,12 +414,13 @@ def test_offsets_past_32_bits(A):
         assert same_codes(A.Tensor(ctx, t.ptr + (rows - last) * cols, last, cols, np.uint8).numpy(), swiglu64(x, x)[0])
 
 
-def test_more_rows_than_a_launch_takes(A):
-    """The row calls past 2^23 rows: first, last and middle rows, whose scales lie far apart."""
-    rows, cols = (1 << 23) + 1000, 40
+@pytest.mark.parametrize("rows,cols", [((1 << 23) + 1000, 40), (16387, 2100)])
+def test_many_rows(A, rows, cols):
+    """The row calls past 2^23 rows, more than a launch takes, and of 2^18 blocks or more of long rows: first, last and
+    middle rows, whose scales lie far apart."""
     rng = np.random.default_rng(8)
     x = rng.standard_normal((rows, cols), dtype=np.float32).astype(np.float16)
-    at = np.r_[0:50, (1 << 23) - 50:(1 << 23) + 50, rows - 50:rows]
+    at = np.r_[0:50, rows - 1050:rows - 950, rows - 50:rows]
     w = rng.standard_normal(cols).astype(np.float16)
     with A.Context(4 << 30) as ctx:
         t, tx, tw = A.FP8Tensor.empty(ctx, rows, cols), ctx.from_numpy(x), ctx.from_numpy(w)
