@@ -441,7 +441,7 @@ __device__ __forceinline__ Frag16 to_f16(Frag8 f) {
 //
 // The 8-bit matrix instructions do not keep all of f32: of the products of 8 neighbouring k they drop what lies under
 // 2^-13 of the power of two at the largest (measured: both 16x16x128 and 16x16x32, 1.3e-5 of a sum of near normal
-// products, its norm against f64), which f16 results, rounded by 2.8e-4, do not show. f32 results and products that
+// products, its norm against f64), which f16 results, whose rounding is 2.1e-4, do not show. f32 results and products that
 // wait for memory anyway take the f16 instruction, whose sums are f32, on the numbers converted; it runs at half the
 // rate.
 __device__ __forceinline__ f32x4 mma_block(Frag8 a, Frag8 b) {
@@ -596,12 +596,15 @@ __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
 }
 
-// A wave's sums to C, T's rows from (m, n) on, whole along n and 16-byte aligned. Stores of 4 elements straight from the
-// registers cost 8192 x 28672 x 4096 another 110 us.
-template <typename T, int NF, int MF>
+// A wave's sums to C, T's rows from (m, n) on, 16 rows at a time through a place of the wave's own in LDS, so that a
+// store fills whole lines. WHOLE: all columns are C's and rows are 16-byte aligned; else element by element. Stores
+// straight from the registers cost 8192 x 28672 x 4096 another 110 us, and odd rows of 2756 x 3338 x 232 27.9 us for 17.7.
+template <bool WHOLE, typename T, int NF, int MF>
 __device__ __forceinline__ void store_rows(const Fp8Args &p, T *c, uint8_t *lds, const f32x4 (&acc)[NF][MF], int64_t m, int64_t n, int wave,
                                            int lane) {
-    constexpr int kRow = NF * 16 * sizeof(T), kStride = kRow + 16, kLanes = kRow / 16, kRows = 64 / kLanes;
+    constexpr int kCols = NF * 16, kStride = kCols * sizeof(T) + 16, kEach = WHOLE ? 16 / sizeof(T) : 1;
+    constexpr int kLanes = kCols / kEach < 64 ? kCols / kEach : 64, kRows = 64 / kLanes;
+    static_assert(16 % kRows == 0);
     uint8_t *own = lds + wave * 16 * kStride;
 #pragma unroll
     for (int j = 0; j < MF; j++) {
@@ -615,9 +618,19 @@ __device__ __forceinline__ void store_rows(const Fp8Args &p, T *c, uint8_t *lds,
                 *(u32x2 *)to = u32x2{h2_bits(h16x2{(h16)v[0], (h16)v[1]}), h2_bits(h16x2{(h16)v[2], (h16)v[3]})};
         }
 #pragma unroll
-        for (int r = lane / kLanes; r < 16; r += kRows) {
-            const u32x4 v = ld16(own + r * kStride + lane % kLanes * 16);
-            if (m + 16 * j + r < p.M) st16((uint8_t *)(c + (m + 16 * j + r) * p.ldc + n) + lane % kLanes * 16, v);
+        for (int r0 = 0; r0 < 16; r0 += kRows) {
+            const int r = r0 + lane / kLanes;
+            T *row = c + (m + 16 * j + r) * p.ldc + n;
+#pragma unroll
+            for (int e = 0; e < kCols; e += kLanes * kEach) {
+                const int col = e + lane % kLanes * kEach;
+                const uint8_t *from = own + r * kStride + col * sizeof(T);
+                if constexpr (WHOLE) {
+                    if (m + 16 * j + r < p.M) st16(row + col, ld16(from));
+                } else {
+                    if (m + 16 * j + r < p.M && n + col < p.N) row[col] = *(const T *)from;
+                }
+            }
         }
     }
 }
@@ -738,19 +751,19 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tile_kernel(Fp8Args p) {
         p.f32 = true;
         p.quad = p.N % 4 == 0;
     }
-    // Rows of C through LDS, so that a store fills whole lines: 16 rows at a time, in a place of the wave's own.
-    if (p.quad && n0 + BN <= p.N) {
-        barrier();
-        if (p.f32)
-            store_rows<float>(p, (float *)p.c, lds, acc, m0 + wm, n0 + wn, wave, lane);
+    barrier();  // no wave reads a stage any more
+    const bool whole = p.quad && n0 + BN <= p.N;
+    if (p.f32) {
+        if (whole)
+            store_rows<true>(p, (float *)p.c, lds, acc, m0 + wm, n0 + wn, wave, lane);
         else
-            store_rows<h16>(p, (h16 *)p.c, lds, acc, m0 + wm, n0 + wn, wave, lane);
-        return;
+            store_rows<false>(p, (float *)p.c, lds, acc, m0 + wm, n0 + wn, wave, lane);
+    } else {
+        if (whole)
+            store_rows<true>(p, (h16 *)p.c, lds, acc, m0 + wm, n0 + wn, wave, lane);
+        else
+            store_rows<false>(p, (h16 *)p.c, lds, acc, m0 + wm, n0 + wn, wave, lane);
     }
-#pragma unroll
-    for (int i = 0; i < NF; i++)
-#pragma unroll
-        for (int j = 0; j < MF; j++) fp8_store(p, m0 + wm + 16 * j + i16, n0 + wn + 16 * i + 4 * (lane >> 4), acc[i][j]);
 }
 
 // C from the sums of `splits` stretches of k, in their order; fewer than 2^31 elements. VEC: 4 a thread, N a multiple of 4.
