@@ -393,8 +393,18 @@ class FP8Tensor:
         return (number.astype(np.float32)[self.codes()] * np.repeat(s, 128, 1))[:, : self.cols]
 
 
+_F16 = np.dtype(np.float16)
+
+
+def _halves(name: str, *tensors: Tensor):
+    for t in tensors:
+        if t.dtype != _F16:
+            raise AesirError(-7, f"{name}: tensors must be f16")
+
+
 def quantize_fp8(ctx: Context, x: Tensor, out: FP8Tensor):
     """Codes and scales of x, whose rows are x.cols elements apart (out.cols of them count)."""
+    _halves("quantize_fp8", x)
     _check(_L.aesir_quantize_fp8(ctx.h, x.ptr, x.rows, x.cols, out.ptr, out.scales_ptr, out.rows, out.cols, out.block_rows))
 
 
@@ -407,9 +417,11 @@ def rmsnorm_fp8(ctx: Context, x: Tensor, weight: Tensor, out: FP8Tensor, epsilon
                 total: Tensor = None):
     """Activations of the RMSNorm of x, or with a residual of f16(x + residual), which goes to total (or back to x)."""
     _activations("rmsnorm_fp8", out)
+    _halves("rmsnorm_fp8", x, weight)
     r = (None, 0, 0, None, 0, 0)
     if residual is not None:
         total = x if total is None else total
+        _halves("rmsnorm_fp8", residual, total)
         r = (residual.ptr, residual.rows, residual.cols, total.ptr, total.rows, total.cols)
     elif total is not None:
         raise AesirError(-1, "rmsnorm_fp8: a residual and the place of its sum come together")
@@ -420,6 +432,7 @@ def rmsnorm_fp8(ctx: Context, x: Tensor, weight: Tensor, out: FP8Tensor, epsilon
 def swiglu_fp8(ctx: Context, gate: Tensor, up: Tensor, out: FP8Tensor):
     """Activations up * gate / (1 + exp(-gate)); gate and up may be parts of one product's rows."""
     _activations("swiglu_fp8", out)
+    _halves("swiglu_fp8", gate, up)
     _check(_L.aesir_swiglu_fp8(ctx.h, gate.ptr, gate.rows, gate.cols, up.ptr, up.rows, up.cols, out.ptr, out.scales_ptr, out.rows,
                                out.cols))
 

@@ -135,8 +135,17 @@ refused(-2, n + ": activations have blocks of one row", g, b, b, T(c, rows=200))
 refused(-2, n + ": weights have blocks of 128 rows", g, q, q, T(c, cols=4))
 """
 
+TYPES = """
+f = A.Tensor(ctx, x.ptr, 4, 512, np.uint8)
+refused(-7, "quantize_fp8: tensors must be f16", A.quantize_fp8, f, q)
+for args in ((f, x), (x, f)):
+    refused(-7, "swiglu_fp8: tensors must be f16", A.swiglu_fp8, *args, q)
+    refused(-7, "rmsnorm_fp8: tensors must be f16", A.rmsnorm_fp8, *args, q)
+    refused(-7, "rmsnorm_fp8: tensors must be f16", A.rmsnorm_fp8, x, w, q, 1e-5, *args)
+"""
 
-@pytest.mark.parametrize("script", [CODES, NORM, PRODUCT])
+
+@pytest.mark.parametrize("script", [CODES, NORM, PRODUCT, TYPES])
 def test_refusals(child, script):
     child(script)
 
