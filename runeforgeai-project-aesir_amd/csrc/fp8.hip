@@ -79,7 +79,8 @@ constexpr u32x2 kNanCodes = {0x7f7f7f7fu, 0x7f7f7f7fu};
 // middle of two codes is at least 2^-28 of it away from one.
 __device__ __forceinline__ u32x2 codes_of(const float (&p)[8], unsigned top) {
     if (top >= kInfBits) return kNanCodes;
-    const float a = __builtin_bit_cast(float, top), inv = top ? __builtin_amdgcn_rcpf(a) : 0.0f;
+    if (top == 0) return {0, 0};  // of zeros of either sign
+    const float a = __builtin_bit_cast(float, top), inv = __builtin_amdgcn_rcpf(a);
     const float less = inv * (kE4m3Max * (1.0f - 0x1p-21f)), more = inv * (kE4m3Max * (1.0f + 0x1p-21f));
     float lo[8], hi[8];
 #pragma unroll
@@ -365,8 +366,9 @@ __global__ __launch_bounds__(256) void fp8_swiglu_kernel(const h16 *__restrict__
         for (int j = 0; j < 8; j++) y[j] = swiglu_f(g[j], u[j]);
         const unsigned top = row_max(top_bits(y));
         const float a = __builtin_bit_cast(float, top);
-        float scale = a >= kSwigluLeast ? a / kE4m3Max : 0.0f;
-        const float inv = a >= kSwigluLeast ? __builtin_amdgcn_rcpf(a) : 0.0f;
+        const bool some = a >= kSwigluLeast;
+        float scale = some ? a / kE4m3Max : 0.0f;
+        const float inv = some ? __builtin_amdgcn_rcpf(a) : 0.0f;
         const float less = inv * (kE4m3Max * (1.0f - 0x1p-19f)), more = inv * (kE4m3Max * (1.0f + 0x1p-19f));
         float lo[8], hi[8];
 #pragma unroll
@@ -389,11 +391,13 @@ __global__ __launch_bounds__(256) void fp8_swiglu_kernel(const h16 *__restrict__
             }
 #pragma unroll
             for (int k = 1; k < 16; k <<= 1) m = fmax(m, __shfl_xor(m, k));
-            const bool some = m >= (double)kSwigluLeast;
-            scale = some ? (float)(m / 448.0) : 0.0f;
+            const bool some_d = m >= (double)kSwigluLeast;
+            scale = some_d ? (float)(m / 448.0) : 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; j++) lo[j] = some ? to_odd(yd[j] * 448.0 / m) : 0.0f;
+            for (int j = 0; j < 8; j++) lo[j] = some_d ? to_odd(yd[j] * 448.0 / m) : 0.0f;
             codes = to_e4m3(lo);
+        } else if (!some) {
+            codes = {0, 0};  // of values of either sign
         }
         *reinterpret_cast<u32x2 *>(q + r * nb * kFp8Block + c) = codes;
         if (threadIdx.x % 16 == 0) scales[b * rows + r] = bad ? __builtin_nanf("") : scale;
