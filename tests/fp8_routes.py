@@ -15,6 +15,7 @@ PRODUCTS = [
     for f32 in (False, True)
 ] + [
     (40, 132, 12400, False, "fp8_tile_kernel<64,64,2,2,4,0,1>", 8),
+    (50, 1001, 12400, False, "fp8_tile_kernel<64,64,2,2,4,0,1>", 8),
     (50, 1001, 12400, True, "fp8_tile_kernel<64,64,2,2,4,1,1>", 8),
     (40, 4200, 12400, False, "fp8_tile_kernel<64,64,2,2,4,0,1>", 4),
     (65, 130, 600, False, "fp8_tile_kernel<64,64,2,2,4,0,0>", 1),
