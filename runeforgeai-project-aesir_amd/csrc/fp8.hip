@@ -839,7 +839,15 @@ static int32_t stream_16(hipStream_t s, const Fp8Args &p) {
     return stream<MH, 1, 8, 2, true>(s, p);
 }
 
-// 17 to 64 rows of at most 8192 of B: as above, with 4 waves, since the rows of A take most of a ring's stage.
+// 17 to 64 rows by at most 8192 of B: as above, with 4 waves, since the rows of A take most of a ring's stage. NR 2 pays where B
+// has more than 16 rows for each CU, and more of A want fewer stages. Measured at k 4096, us of NR 1 with 2 and 3 stages, then
+// of NR 2 with 2 and 3:
+//   f16  24 x 4096  6.5  6.3  7.3  7.4    24 x 7168   9.7   9.7   8.2   8.4
+//        40 x 4096  7.3  7.4  8.5  8.7    40 x 7168  11.7  12.9   9.4   9.7
+//        64 x 4096  8.6  8.8  9.8 10.3    64 x 7168  14.9  15.5  10.7  11.2
+//   f32  24 x 4096  6.8  6.3  7.8  7.7    24 x 7168   9.9   9.9   8.5   8.7
+//        40 x 4096  8.1  7.9  9.2  9.5    40 x 7168  12.3  14.0   9.9  10.4
+//        64 x 4096  8.9  9.4 10.1 10.6    64 x 7168  15.7  16.7  10.9  11.6
 template <bool EXACT>
 static int32_t stream_64(hipStream_t s, const Fp8Args &p) {
     if (p.N <= 4096)
@@ -896,10 +904,16 @@ int32_t launch_gemm_fp8(hipStream_t s, const void *A, const float *as, int64_t M
     if (M <= 64 && (N + 15) / 16 > kLaunchGroups) return too_large();
     if (M <= 16) return M <= 8 ? stream_16<1>(s, p) : stream_16<2>(s, p);
     if (M <= 64) {
-        // Tiles of 64 x 64 share the rows of A among 64 of B: they pay once they fill half the CUs, by B's rows (64 rows
-        // 28672 x 4096 31.1 us against 37.7) or, from 33 rows on, by stretches of long rows (64 rows 4096 x 14336 18.5
-        // against 22.2, 2048 x 5632 9.8 both, 4096 x 4096 10.2 against 8.5).
-        if (N < 8192 && (M <= 32 || p.nb < 96)) return f32 ? stream_64<true>(s, p) : stream_64<false>(s, p);
+        // Tiles of 64 x 64 share the rows of A among 64 of B. They pay once B alone makes more of them than half the CUs, or, from 33
+        // rows on, cut into stretches of long rows. Measured, us streamed and in tiles, f16 then f32:
+        //   24 x 8192 x 4096    9.3  13.5   9.6  14.1    64 x 8192 x 4096   11.4  13.7  11.6  15.9
+        //   24 x 11264 x 4096  14.9  13.8  15.3  18.9    64 x 11264 x 4096  19.1  14.8  19.6  19.0
+        //   24 x 28672 x 4096  30.3  25.6  31.0  29.1    64 x 28672 x 4096  37.9  28.6  39.2  31.5
+        //   64 x 4096 x 8192   13.5  13.8  14.2  16.0    64 x 7168 x 8192   18.2  19.1  18.4  22.9
+        //   64 x 4096 x 11264  18.4  16.2  19.2  19.4    64 x 7168 x 11264  23.9  23.2  24.3  28.6
+        //   64 x 4096 x 14336  22.3  18.2  23.0  22.2    64 x 7168 x 14336  29.3  26.6  29.6  34.3
+        //   24 x 4096 x 14336  14.6  16.4  14.7  20.9    40 x 4096 x 14336  18.4  16.9  20.1  21.3
+        if (N <= 8192 && (M <= 32 || p.nb < 96)) return f32 ? stream_64<true>(s, p) : stream_64<false>(s, p);
         const TileCost one[1] = {f32 ? kExactTiles[0] : kTiles[0]};
         choose_tile(one, p, part_floats, &p.splits);
         return f32 ? tile<64, 64, 2, 2, 4, true, true>(s, p) : tile<64, 64, 2, 2, 4, false, true>(s, p);

@@ -11,6 +11,7 @@ PRODUCTS = [
     (m, n, k, f32, kernel % f32, 1)
     for m, n, k, kernel in ((18, 301, 600, "fp8_stream_kernel<4,1,4,3,%d>"), (41, 301, 600, "fp8_stream_kernel<6,1,4,2,%d>"), (61, 301, 600, "fp8_stream_kernel<8,1,4,2,%d>"),
                             (31, 4201, 600, "fp8_stream_kernel<4,2,4,3,%d>"), (47, 4201, 600, "fp8_stream_kernel<6,2,4,3,%d>"), (63, 4201, 600, "fp8_stream_kernel<8,2,4,2,%d>"),
+                            (20, 8192, 600, "fp8_stream_kernel<4,2,4,3,%d>"), (64, 8192, 520, "fp8_stream_kernel<8,2,4,2,%d>"),
                             (20, 8300, 600, "fp8_tile_kernel<64,64,2,2,4,%d,1>"), (61, 8301, 600, "fp8_tile_kernel<64,64,2,2,4,%d,1>"))
     for f32 in (False, True)
 ] + [
