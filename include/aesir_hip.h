@@ -230,12 +230,15 @@ int32_t aesir_q8_0_matvec_f32(aesir_ctx *ctx, const void *blocks, int64_t n_rows
  * them. No counterpart in the reference's GGUF path.
  *
  * A matrix of rows x cols is a pair: codes [rows][ld] bytes, ld = cols rounded up to 128, 16-byte aligned, the bytes
- * behind cols 0; and scales, of activations one for each 1 x 128 block, laid out [ld / 128][rows], of weights one for
- * each 128 x 128 block (fewer rows in the last), laid out [ceil(rows / 128)][ld / 128]. An element is code * scale.
+ * behind cols 0 (in a block that reads as NaN as its others); and scales, of activations one for each 1 x 128 block, laid
+ * out [ld / 128][rows], of weights one for each 128 x 128 block (fewer rows in the last), laid out
+ * [ceil(rows / 128)][ld / 128]. An element is code * scale.
  * The calls below that write one store, with y the values of a block and a the largest |y|, scale = a / 448 and the
- * e4m3 numbers nearest 448 y / a, ties to even: a block of zeros has scale 0 and zeros for codes, one that holds an inf
- * or a NaN reads as NaN throughout (all codes 0x7f, scale NaN). The codes are those of the formula, whatever its
- * rounding on the way, so a row's do not depend on the rows beside it.
+ * e4m3 numbers nearest 448 y / a, ties to even: a block of zeros of either sign has scale 0 and code bytes 0, one that holds
+ * an inf or a NaN reads as NaN throughout (all codes 0x7f, scale NaN). The codes are those of the formula, whatever its
+ * rounding on the way, so a row's do not depend on the rows beside it. Scales are f32: quantize's the nearest, SwiGLU's within
+ * 9 * 2^-24 of the formula's, the norm's by an f32 sum of squares. Blocks with many ties of two codes take longer (quantize
+ * up to twice).
  *
  * f16 tensors are rows of `cols` elements from row to row, of which the first q_cols (C: b_rows) count, so they may be
  * parts of a wider matrix; any 2-byte alignment, 16 bytes with cols and q_cols multiples of 8 being the fast one. Up
@@ -261,7 +264,9 @@ int32_t aesir_swiglu_fp8(aesir_ctx *ctx, const void *gate, int64_t gate_rows, in
  * [a_rows x a_cols] and weights B [b_rows x a_cols], rounded once to c_type (AESIR_GGML_F16 or AESIR_GGML_F32); rows of C
  * are c_cols >= b_rows elements apart. Sums are f32, and with c_type F32 or up to 16 rows of A all of them are; f16
  * results of more rows may add a block up on the 8-bit matrix instruction, which of 8 neighbouring products drops what
- * lies under 2^-13 of the largest (some 1.3e-5 of a result where the f16 rounding is 2e-4). The order of sums goes by the
+ * lies under 2^-13 of the largest, each (1e-5 to 3e-5 by the norm of a matrix where the f16 rounding is 2.1e-4; but it goes by
+ * the size of the products, not of their sum, so that about one f16 result in 12 is more than half a step off, and sums that
+ * all but cancel may be many steps off; c_type F32 is the call without it). The order of sums goes by the
  * sizes alone: the same call gives the same bits, another number of rows may give others. The product of two scales has
  * to be an f32 number. Raises "gemm_fp8: matrix dimensions must be positive", "gemm_fp8: inner matrix dimension mismatch",
  * "gemm_fp8: output matrix shape mismatch". */

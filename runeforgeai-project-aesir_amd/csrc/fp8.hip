@@ -5,7 +5,11 @@
 // With y the values of a block and a = max |y|: scale = f32(a / 448), code = the e4m3 number nearest 448 y / a,
 // ties to even. The kernels find t = 448 y / a in f32, a few units of its last place off, and round both ends of an
 // interval that holds the exact quotient: rounding is monotone, so where both give the same code so does the quotient.
-// Elsewhere (one element in some 10^5) it is found again in f64, so that every code is the one of the formula.
+// Elsewhere it is found again in f64, so that every code is the one of the formula: one element in 9 * 10^4 of
+// quantize and RMSNorm (ends 2^-21 of it off), one in 2 * 10^4 of SwiGLU (2^-19), whose whole block is done again, one in 180.
+// That is for values of many bits. Ties of two codes come often where all the values of a block are whole multiples of a
+// 7 * 2^n-th of its largest and take more than e4m3's 4 bits: quantizing 28672 x 4096 weights takes 65 us if they are normal, 55 if
+// they are integers up to 7, 15 or 127, and 107 if integers up to 28 or 112.
 #include <algorithm>
 #include <cmath>
 #include <limits>
@@ -444,10 +448,14 @@ __device__ __forceinline__ Frag16 to_f16(Frag8 f) {
 // l % 16, in element e.
 //
 // The 8-bit matrix instructions do not keep all of f32: of the products of 8 neighbouring k they drop what lies under
-// 2^-13 of the power of two at the largest (measured: both 16x16x128 and 16x16x32, 1.3e-5 of a sum of near normal
-// products, its norm against f64), which f16 results, whose rounding is 2.1e-4, do not show. f32 results and products that
-// wait for memory anyway take the f16 instruction, whose sums are f32, on the numbers converted; it runs at half the
-// rate.
+// 2^-13 of the power of two at the largest (measured: both 16x16x128 and 16x16x32). By the norm of a matrix that is 1.3e-5 of
+// near normal products and 2e-5 to 3e-5 where channels differ much in size, beside f16's rounding of 2.1e-4: f16 results are
+// 2.08e-4 to 2.10e-4 off f64, those of f32 sums 2.07e-4. But it goes by the size of the products, not of their sum: one result in 12
+// is more than half an f16 step off, one in 50 more than a step, sums that all but cancel many steps (64 x 4096 x 14336 to
+// 5207 x 744 x 128, channels as above); of results over a quarter of the root mean square one in 35 is more than half a step off,
+// none more than 3. That is the choice for f16 results of many rows, which it makes up to twice as fast (8192 x 28672 x 4096 830 us,
+// to f32 1631); f32 results and products of few rows, which wait for memory anyway, take the f16 instruction, whose sums are
+// f32, on the numbers converted, at half the rate.
 __device__ __forceinline__ f32x4 mma_block(Frag8 a, Frag8 b) {
     const i32x8 av = {(int)a.lo.x, (int)a.lo.y, (int)a.lo.z, (int)a.lo.w, (int)a.hi.x, (int)a.hi.y, (int)a.hi.z, (int)a.hi.w};
     const i32x8 bv = {(int)b.lo.x, (int)b.lo.y, (int)b.lo.z, (int)b.lo.w, (int)b.hi.x, (int)b.hi.y, (int)b.hi.z, (int)b.hi.w};
@@ -823,10 +831,20 @@ static int32_t tile(hipStream_t s, const Fp8Args &p) {
 }
 
 // Up to 16 rows of A: memory's rate decides. More rows of B a workgroup (NR) are fewer workgroups and fewer copies of A,
-// and pay where B alone fills the 256 CUs; long rows want 8 waves along k. Measured, us of 1 / 16 rows, by NR and waves:
-// 4096 x 4096 NR 1, 4 waves 5.3 / 5.7, NR 2 6.0 / 6.6; 6144 x 4096 7.0 / 8.2, NR 2 6.8 / 7.3; 28672 x 4096 21.7 / 25.7, NR 4
-// 20.8 / 23.1; 32000 x 2048 NR 4 12.0 / 13.5, NR 2 11.6 / 12.4; 4096 x 14336 NR 1, 4 waves 11.3 / 12.4, 8 waves 10.8 / 13.0;
-// 57344 x 8192 8 waves 68 / 83, NR 4 81 / 87.
+// and pay where B alone fills the 256 CUs; long rows want 8 waves along k. Measured, us of 1 / 16 rows, the taken one first:
+//   4096 x 4096   NR 1, 4 waves  5.5 /  5.8, NR 2  6.0 /  6.7
+//   4096 x 14336  NR 1, 8 waves 10.9 / 13.2, 4 waves 11.5 / 12.6
+//   6144 x 4096   NR 2  6.8 /  7.3, NR 1  7.1 /  8.3
+//   8192 x 6144   NR 2  9.4 / 10.0, NR 1  9.6 / 11.4
+//   28672 x 2048  NR 2 11.3 / 12.2, NR 4 11.2 / 12.9
+//   57344 x 2048  NR 2 19.0 / 20.3, NR 4 20.1 / 24.6
+//   28672 x 4096  NR 4 21.2 / 23.8, NR 2 22.7 / 24.2
+//   57344 x 4096  NR 4 40.1 / 46.5, NR 2 40.2 / 43.0
+//   28672 x 8192  NR 1, 8 waves 36.0 / 42.4, NR 4 39.4 / 43.4
+//   57344 x 8192  NR 1, 8 waves 68 / 83, NR 4 82 / 87
+// The borders in k lie between those sizes, and not at the best place everywhere: of 2048 to 57344 rows of B by 1024 to 14336, one
+// row's time is within 7% of the best one's but for 6144 and 8192 rows of B by 8192 and more (up to 16% behind NR 1, or NR 2 with 14336);
+// 16 rows by 6144 and more are up to 26% behind NR 2 or NR 4.
 template <int MH>
 static int32_t stream_16(hipStream_t s, const Fp8Args &p) {
     if (p.N > 4096) {
