@@ -652,7 +652,7 @@ __device__ __forceinline__ void store_rows(const Fp8Args &p, T *c, uint8_t *lds,
 // product of fragments starts from 0 and is added to the sums with the block's scale, 4 multiply-adds beside the 32
 // cycles of a matrix instruction. ONCE: every row of B is used by one workgroup only and need not stay in the caches.
 //
-// Measured: 8192 x 28672 x 4096 in 820 to 860 us (2.3 PFLOP/s), 64 x 4096 x 14336 in 17.8 (with the join below), 333 x
+// Measured: 8192 x 28672 x 4096 in 820 to 890 us by the card (2.2 to 2.3 PFLOP/s), 64 x 4096 x 14336 in 17.8 (with the join below), 333 x
 // 11264 x 2048 in 15.5. Of the first, matrix and vector instructions alone take 584 us at the clock they leave; reading
 // fragments 90 more, since a step begins with reads that nothing covers (LDS gives 205 bytes a cycle, without
 // conflicts); the copies 150, whose 64 KiB a step make a round trip of 1.5 to 1.8 us through L2, as long as a step. Tried
